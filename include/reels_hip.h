@@ -35,6 +35,7 @@ extern "C" {
 #define REELS_HIP_F32 0
 #define REELS_HIP_BF16 1
 #define REELS_HIP_F16 2
+#define REELS_HIP_I32 3 /* token positions only (reels_hip_rotary) */
 
 /* status codes */
 #define REELS_HIP_OK 0
@@ -42,6 +43,10 @@ extern "C" {
 #define REELS_HIP_EDTYPE (-2)     /* unsupported element type */
 #define REELS_HIP_EWORKSPACE (-3) /* workspace NULL or smaller than reels_hip_*_workspace_bytes */
 #define REELS_HIP_EHIP (-4)       /* HIP runtime or launch failure */
+
+/* activations of reels_hip_i8i8_linear */
+#define REELS_HIP_ACT_NONE 0
+#define REELS_HIP_ACT_GELU_TANH 1
 
 /* workspace selectors for reels_hip_i8lora_workspace_bytes */
 #define REELS_HIP_WS_FWD 0
@@ -340,6 +345,98 @@ int reels_hip_attention_bwd(const void* q, const void* k, const void* v, const v
                             int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t D, int dtype,
                             void* dq, void* dk, void* dv, void* workspace, size_t ws_bytes,
                             void* stream);
+
+/*
+ * Root-mean-square norm of rows with the residual's addition before it: rmsnorm,
+ * src/layers/normalization.jl:10-24, and the addition that precedes it in a block.
+ *   s    = rnd(x + residual)                      [rows][cols]  (x itself when residual is NULL)
+ *   rstd = (mean_c s^2 + eps)^(-1/2)              [rows] f32    (the mean in 64 bits)
+ *   y    = rnd(s * rstd * weight)                 [rows][cols]
+ * dtype REELS_HIP_F32, _BF16 or _F16 for x, residual, sum, y; weight [cols] of w_dtype (dtype or
+ * REELS_HIP_F32), NULL for ones. Rows of x and residual lie ld_x and ld_r elements apart (>= cols),
+ * rows of the outputs cols. Any alignment of the element type. sum receives s when residual is set
+ * (it may be x or residual themselves where their stride is cols) and is not written otherwise; y
+ * overlaps no other operand. A row of zeros with eps = 0 gives NaN, as the formula does.
+ *
+ * reels_hip_rms_norm_i8 writes the row in 8 bits instead, in the layout of reels_hip_i8_pack:
+ *   scales[m] = max_c |s weight| rstd / 127,  q = round_ties_even(127 s weight / max_c |s weight|)
+ * (q * scales is the norm's row; the quotient is formed in 64 bits). A zero row has scale 1. A row
+ * whose scale is not finite (NaN or infinities in it) has scale NaN and zero codes.
+ *
+ * reels_hip_rms_norm_bwd, with s the sum that the forward wrote (x where it had no residual), its
+ * rstd, and dsum the gradient that reaches s from elsewhere (the residual stream; NULL for none):
+ *   g = dy * weight;  dx = rnd(rstd (g - s rstd^2 mean_c(g s)) + dsum)   (of x and residual alike)
+ *   dw[c] = sum_m dy s rstd   (f32; NULL to skip)
+ * dw needs a workspace of reels_hip_rms_norm_workspace_bytes(rows, cols) bytes (NULL without it).
+ * Bitwise reproducible: no atomics, fixed orders of summation. rows = 0 gives dw = 0.
+ */
+int reels_hip_rms_norm(const void* x, int64_t ld_x, const void* residual, int64_t ld_r,
+                       const void* weight, int w_dtype, int dtype, int64_t rows, int64_t cols,
+                       float eps, void* sum, void* y, float* rstd, void* stream);
+int reels_hip_rms_norm_i8(const void* x, int64_t ld_x, const void* residual, int64_t ld_r,
+                          const void* weight, int w_dtype, int dtype, int64_t rows, int64_t cols,
+                          float eps, void* sum, int8_t* q, float* scales, void* stream);
+size_t reels_hip_rms_norm_workspace_bytes(int64_t rows, int64_t cols);
+int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void* dsum, const void* weight,
+                           int w_dtype, const float* rstd, int dtype, int64_t rows, int64_t cols,
+                           void* dx, float* dw, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Product of int8 rows with a packed int8 weight, for sampling with activations in 8 bits (the
+ * reference has no counterpart: its int8 path dequantizes the weight, quantization.jl:54-74):
+ *   y[m][n] = rnd(act(xs[m] * ws[n] * sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n])
+ *   x [M][K] int8, xs [M] f32: rows of reels_hip_rms_norm_i8 or reels_hip_i8_pack
+ *   w [N][K] int8, ws [N] f32: a weight of reels_hip_i8_pack
+ *   bias [N], residual [M][N] (either NULL) and y [M][N] of dtype REELS_HIP_F32, _BF16 or _F16;
+ *   y may be residual itself
+ *   activation REELS_HIP_ACT_NONE or REELS_HIP_ACT_GELU_TANH (reels_hip_gelu_tanh in f32)
+ * The sums are exact whole numbers (K < 131072), the rest runs in f32 and rounds once, so a row of
+ * y does not depend on M nor on its place. Any alignment. workspace:
+ * reels_hip_i8i8_workspace_bytes(M, K, N) bytes.
+ */
+size_t reels_hip_i8i8_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int reels_hip_i8i8_linear(const int8_t* x, const float* xs, const int8_t* w, const float* ws,
+                          const void* bias, const void* residual, int activation, int dtype,
+                          int64_t M, int64_t K, int64_t N, void* y, void* workspace,
+                          size_t ws_bytes, void* stream);
+
+/*
+ * Rotary positions over one to four axes (the video model's time, height and width), _rope!,
+ * src/layers/rope.jl:13-32, for the queries and the keys of one attention.
+ *   q, yq [B][S][Hq][D];  k, yk [B][S][Hk][D] (Hk = 0: q alone) of dtype REELS_HIP_F32, _BF16 or
+ *   _F16, tokens of q and k ld_q and ld_k elements apart (>= Hq D, Hk D; batches S of them), the
+ *   outputs dense; yq may be q itself, and yk k, where they are dense too
+ *   pos [pos_batches][S][axes], REELS_HIP_F32 or REELS_HIP_I32; pos_batches B or 1 (shared)
+ *   axis_pairs [axes], HOST memory: the pairs of each axis, P together, 2 P <= D
+ * Pair j of axis a turns by pos[token][a] * theta^(-j / axis_pairs[a]) (by its negative with
+ * inverse, which is the backward): (u, v) -> (u cos - v sin, u sin + v cos). With interleaved pair
+ * p is elements 2p and 2p + 1 of a head, otherwise p and p + P; elements past 2 P are copied.
+ * Angles are reduced in 64 bits, so far positions lose nothing; rotations run in f32 and round
+ * once. D even, up to 512. Any alignment of the element type.
+ */
+int reels_hip_rotary(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* pos,
+                     int pos_dtype, int64_t pos_batches, int dtype, int64_t B, int64_t S,
+                     int64_t Hq, int64_t Hk, int64_t D, const int32_t* axis_pairs, int axes,
+                     float theta, int interleaved, int inverse, void* yq, void* yk, void* stream);
+
+/*
+ * Global norm of a list of gradients and clipping by it: what the reference's training loop does
+ * between the backward and AdamW (src/training/wan_runner.jl:108-289).
+ *   norm[0] = sqrt(sum over all tensors of g^2)      (f32 on the device; summed in 64 bits)
+ *   outs[i] = rnd(grads[i] * min(1, max_norm / (norm + 1e-6)))
+ * grads, outs [count] HOST arrays of device pointers, sizes [count] elements, dtypes [count]
+ * REELS_HIP_F32, _BF16 or _F16 (of the gradient and its output); outs[i] may be grads[i] (in
+ * place) and overlaps nothing else, which is checked. Gradients whose norm is not finite are left
+ * (or copied) unscaled. The host arrays may be freed on return, and a call records into a graph,
+ * which then holds these pointers. Bitwise reproducible for the same sizes. workspace:
+ * reels_hip_grad_workspace_bytes(count) bytes.
+ */
+size_t reels_hip_grad_workspace_bytes(int64_t count);
+int reels_hip_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
+                        int64_t count, float* norm, void* workspace, size_t ws_bytes, void* stream);
+int reels_hip_clip_gradients(const void* const* grads, void* const* outs, const int64_t* sizes,
+                             const int32_t* dtypes, int64_t count, float max_norm, float* norm,
+                             void* workspace, size_t ws_bytes, void* stream);
 
 /*
  * Kernel timing instrumentation. No counterpart in the reference (it has no profiler hooks);

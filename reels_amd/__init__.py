@@ -9,6 +9,7 @@ from .attention import (  # noqa: F401
     memory_efficient_attention,
     memory_efficient_attention_backward,
 )
+from .gradients import clip_gradients, gradient_norm  # noqa: F401
 from .layers import (  # noqa: F401
     DenseLayer,
     FrozenWeightTransfer,
@@ -33,4 +34,23 @@ from .layers import (  # noqa: F401
     quantize_frozen_matrix,
     set_adapter_enabled,
     workspace_bytes,
+)
+from .normalization import (  # noqa: F401
+    RMSNormFunction,
+    RMSNormGradients,
+    RMSNormQuantized,
+    RMSNormResult,
+    rms_norm,
+    rms_norm_backward,
+    rms_norm_quantized,
+)
+from .quantized import quantize_rows, quantized_linear  # noqa: F401
+from .rotary import (  # noqa: F401
+    RotaryFunction,
+    grid_positions,
+    rotary,
+    rotary_axes,
+    rotary_backward,
+    rotary_qk,
+    rotary_qk_backward,
 )

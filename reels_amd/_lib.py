@@ -15,6 +15,8 @@ DEFAULT_LIB = os.path.join(HERE, "lib", "libreels_hip.so")
 
 ABI_VERSION = 1
 F32, BF16, F16 = 0, 1, 2
+I32 = 3  # token positions only
+ACT_NONE, ACT_GELU_TANH = 0, 1
 WS_FWD, WS_BWD, WS_FWD_NOALLOC = 0, 1, 2
 
 # every symbol include/reels_hip.h declares
@@ -48,6 +50,16 @@ EXPORTS = (
     "reels_hip_attention_workspace_bytes",
     "reels_hip_attention_fwd",
     "reels_hip_attention_bwd",
+    "reels_hip_rms_norm",
+    "reels_hip_rms_norm_i8",
+    "reels_hip_rms_norm_workspace_bytes",
+    "reels_hip_rms_norm_bwd",
+    "reels_hip_i8i8_workspace_bytes",
+    "reels_hip_i8i8_linear",
+    "reels_hip_rotary",
+    "reels_hip_grad_workspace_bytes",
+    "reels_hip_grad_norm",
+    "reels_hip_clip_gradients",
     "reels_hip_trace_start",
     "reels_hip_trace_only",
     "reels_hip_trace_stop",
@@ -130,6 +142,28 @@ def lib():
     L.reels_hip_attention_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, i64, i64, i64, i64, i64, ci,
                                           vp, vp, vp, vp, sz, vp]
     L.reels_hip_attention_bwd.restype = ci
+    cf = ctypes.c_float
+    L.reels_hip_rms_norm.argtypes = [vp, i64, vp, i64, vp, ci, ci, i64, i64, cf, vp, vp, vp, vp]
+    L.reels_hip_rms_norm.restype = ci
+    L.reels_hip_rms_norm_i8.argtypes = [vp, i64, vp, i64, vp, ci, ci, i64, i64, cf, vp, vp, vp, vp]
+    L.reels_hip_rms_norm_i8.restype = ci
+    L.reels_hip_rms_norm_workspace_bytes.argtypes = [i64, i64]
+    L.reels_hip_rms_norm_workspace_bytes.restype = sz
+    L.reels_hip_rms_norm_bwd.argtypes = [vp, vp, vp, vp, ci, vp, ci, i64, i64, vp, vp, vp, sz, vp]
+    L.reels_hip_rms_norm_bwd.restype = ci
+    L.reels_hip_i8i8_workspace_bytes.argtypes = [i64, i64, i64]
+    L.reels_hip_i8i8_workspace_bytes.restype = sz
+    L.reels_hip_i8i8_linear.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, i64, i64, i64, vp, vp, sz, vp]
+    L.reels_hip_i8i8_linear.restype = ci
+    L.reels_hip_rotary.argtypes = [vp, i64, vp, i64, vp, ci, i64, ci, i64, i64, i64, i64, i64, vp, ci,
+                                   cf, ci, ci, vp, vp, vp]
+    L.reels_hip_rotary.restype = ci
+    L.reels_hip_grad_workspace_bytes.argtypes = [i64]
+    L.reels_hip_grad_workspace_bytes.restype = sz
+    L.reels_hip_grad_norm.argtypes = [vp, vp, vp, i64, vp, vp, sz, vp]
+    L.reels_hip_grad_norm.restype = ci
+    L.reels_hip_clip_gradients.argtypes = [vp, vp, vp, vp, i64, cf, vp, vp, sz, vp]
+    L.reels_hip_clip_gradients.restype = ci
     L.reels_hip_trace_start.argtypes = [ctypes.c_int]
     L.reels_hip_trace_start.restype = ctypes.c_int
     L.reels_hip_trace_stop.restype = ctypes.c_int

@@ -1,0 +1,258 @@
+// Global norm of many gradient tensors and clipping by it (what the reference's training loop does
+// with the adapters' gradients before the optimizer, src/training/wan_runner.jl:108-289).
+//
+//   norm = sqrt(sum over tensors of g^2);  out = rnd(g min(1, max_norm / (norm + 1e-6)))
+//
+// Bound by memory: the gradients are read for the norm and again for the scaled copy, which needs
+// the finished norm. The tensors (their pointers, sizes and types) travel in kernel arguments to a
+// table in the workspace, 96 at a time, so a call records into a graph and the host keeps nothing.
+// The work is cut into pieces of 16384 elements; every workgroup takes a run of consecutive pieces.
+// Squares are summed in 64 bits, one partial per workgroup, and every workgroup of the second pass
+// adds the partials in the same order: the result does not depend on the run.
+#include "vec.h"
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+namespace reels {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kPiece = 16384;
+constexpr int kBlocks = 1024;   // workgroups of each pass: four per CU
+constexpr int kBatch = 96;      // tensors per table launch (32 bytes each in 4 KiB of arguments)
+
+struct Entry {
+  const void* g;
+  void* o;
+  int64_t n;
+  int64_t first;  // pieces before this tensor
+};
+// the type travels in the low bits of n's place: n < 2^61
+struct Batch { Entry e[kBatch]; };
+
+__global__ __launch_bounds__(128) void grad_table_kernel(Batch b, Entry* table, int count) {
+  const int i = threadIdx.x;
+  if (i < count) table[i] = b.e[i];
+}
+
+__device__ __forceinline__ int64_t entry_size(const Entry& e) { return e.n >> 2; }
+__device__ __forceinline__ int entry_type(const Entry& e) { return (int)(e.n & 3); }
+
+// index of the tensor that holds a piece
+__device__ __forceinline__ int find_entry(const Entry* table, int count, int64_t piece) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table[mid].first <= piece) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* slot) {
+  v = group_sum<64>(v);
+  if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = slot[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 64; ++i) v += slot[i];
+  return v;
+}
+
+template <int ELT> __device__ __forceinline__ double piece_sum(const void* g, int64_t n) {
+  constexpr int V = 16 / elt_bytes(ELT);
+  double t = 0.0;
+  for (int64_t i = (int64_t)threadIdx.x * V; i < n; i += kThreads * V) {
+    float f[V];
+    load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), n - i < V ? (int)(n - i) : V, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) t = fma((double)f[j], (double)f[j], t);
+  }
+  return t;
+}
+
+template <int ELT> __device__ __forceinline__ void piece_scale(const void* g, void* o, int64_t n, float factor) {
+  constexpr int V = 16 / elt_bytes(ELT);
+  for (int64_t i = (int64_t)threadIdx.x * V; i < n; i += kThreads * V) {
+    float f[V];
+    const int left = n - i < V ? (int)(n - i) : V;
+    load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), left, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] *= factor;
+    store_vec<ELT, V>((uint8_t*)o + i * elt_bytes(ELT), left, f);
+  }
+}
+
+template <typename F> __device__ __forceinline__ void with_type(int t, F&& f) {
+  if (t == REELS_HIP_F32) f(std::integral_constant<int, REELS_HIP_F32>{});
+  else if (t == REELS_HIP_F16) f(std::integral_constant<int, REELS_HIP_F16>{});
+  else f(std::integral_constant<int, REELS_HIP_BF16>{});
+}
+
+// f(entry, element offset, elements) for every piece of this workgroup
+template <typename F> __device__ __forceinline__ void each_piece(const Entry* table, int count, int64_t pieces, F&& f) {
+  const int64_t p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
+  if (p0 >= p1) return;
+  int at = find_entry(table, count, p0);
+  for (int64_t p = p0; p < p1; ++p) {
+    while (at + 1 < count && table[at + 1].first <= p) ++at;
+    const Entry e = table[at];
+    const int64_t off = (p - e.first) * kPiece, n = entry_size(e) - off;
+    f(e, off, n < kPiece ? n : kPiece);
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void grad_sum_kernel(const Entry* table, int count, int64_t pieces, double* part) {
+  __shared__ double slot[kThreads / 64];
+  double t = 0.0;
+  each_piece(table, count, pieces, [&](const Entry& e, int64_t off, int64_t n) {
+    with_type(entry_type(e), [&](auto ty) {
+      constexpr int E = decltype(ty)::value;
+      t += piece_sum<E>((const uint8_t*)e.g + off * elt_bytes(E), n);
+    });
+  });
+  t = block_sum(t, slot);
+  if (threadIdx.x == 0) part[blockIdx.x] = t;
+}
+
+__device__ __forceinline__ double total_norm(const double* part, int n, double* slot) {
+  double t = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) t += part[i];
+  return sqrt(block_sum(t, slot));
+}
+
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(const double* part, int n, float* norm) {
+  __shared__ double slot[kThreads / 64];
+  const double t = total_norm(part, n, slot);
+  if (threadIdx.x == 0) *norm = (float)t;
+}
+
+__global__ __launch_bounds__(kThreads) void grad_scale_kernel(const Entry* table, int count, int64_t pieces,
+                                                              const double* part, int n, float max_norm, float* norm) {
+  __shared__ double slot[kThreads / 64];
+  const double t = total_norm(part, n, slot);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)t;
+  // gradients whose norm is not finite are left as they are: a factor of 0 or NaN would hide which
+  // of them it came from
+  const double f = (double)max_norm / (t + 1e-6);
+  const float factor = __builtin_isfinite(t) && f < 1.0 ? (float)f : 1.0f;
+  each_piece(table, count, pieces, [&](const Entry& e, int64_t off, int64_t m) {
+    if (factor == 1.0f && e.g == e.o) return;  // in place and nothing to clip
+    with_type(entry_type(e), [&](auto ty) {
+      constexpr int E = decltype(ty)::value;
+      piece_scale<E>((const uint8_t*)e.g + off * elt_bytes(E), (uint8_t*)e.o + off * elt_bytes(E), m, factor);
+    });
+  });
+}
+
+size_t table_bytes(int64_t count) { return align_up((size_t)count * sizeof(Entry), 256); }
+
+// two ranges overlap, one of them an output, unless they are a tensor and its own output
+bool outputs_overlap(const void* const* g, void* const* o, const int64_t* n, const int32_t* ty, int64_t count) {
+  struct Span { uintptr_t a, b; bool out; };
+  std::vector<Span> v;
+  v.reserve((size_t)count * 2);
+  for (int64_t i = 0; i < count; ++i) {
+    const uintptr_t bytes = (uintptr_t)n[i] * elt_bytes(ty[i]);
+    if (bytes == 0) continue;
+    v.push_back({(uintptr_t)o[i], (uintptr_t)o[i] + bytes, true});
+    if (g[i] != o[i]) v.push_back({(uintptr_t)g[i], (uintptr_t)g[i] + bytes, false});
+  }
+  std::sort(v.begin(), v.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+  uintptr_t end_any = 0, end_out = 0;
+  for (const Span& s : v) {
+    if (s.a < end_out || (s.out && s.a < end_any)) return true;
+    end_any = std::max(end_any, s.b);
+    if (s.out) end_out = std::max(end_out, s.b);
+  }
+  return false;
+}
+
+int clip_run(const char* name, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* dtypes,
+             int64_t count, bool clip, float max_norm, float* norm, void* workspace, size_t ws_bytes, hipStream_t st) {
+  clear_error();
+  const std::string fn = std::string(name) + ": ";
+  if (count < 0 || count > ((int64_t)1 << 24)) return fail(REELS_HIP_EINVAL, fn + "0 to 2^24 tensors required");
+  if (norm == nullptr || (count > 0 && (grads == nullptr || sizes == nullptr || dtypes == nullptr || (clip && outs == nullptr))))
+    return fail(REELS_HIP_EINVAL, fn + "NULL operand");
+  if (clip && !(max_norm >= 0.0f)) return fail(REELS_HIP_EINVAL, fn + "max_norm must not be negative or NaN");
+  if (workspace == nullptr || ws_bytes < reels_hip_grad_workspace_bytes(count))
+    return fail(REELS_HIP_EWORKSPACE, fn + "workspace of reels_hip_grad_workspace_bytes required");
+  int64_t pieces = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!known_elt(dtypes[i])) return fail(REELS_HIP_EDTYPE, fn + "dtypes must be f32, bf16 or f16");
+    if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 48)) return fail(REELS_HIP_EINVAL, fn + "bad tensor size");
+    if (sizes[i] > 0 && (grads[i] == nullptr || (clip && outs[i] == nullptr))) return fail(REELS_HIP_EINVAL, fn + "NULL tensor");
+    pieces += ceil_div(sizes[i], kPiece);
+  }
+  if (clip && outputs_overlap(grads, outs, sizes, dtypes, count))
+    return fail(REELS_HIP_EINVAL, fn + "an output overlaps another tensor (the same gradient twice?)");
+  Entry* table = (Entry*)workspace;
+  double* part = (double*)((uint8_t*)workspace + table_bytes(count));
+  int64_t used = 0, first = 0;
+  Batch b;
+  int in = 0;
+  auto flush = [&]() -> int {
+    if (in == 0) return REELS_HIP_OK;
+    { TraceScope _ts(st, "grad_table_kernel");
+      grad_table_kernel<<<1, 128, 0, st>>>(b, table + used, in); }
+    used += in;
+    in = 0;
+    return check_launch("grad_table_kernel");
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] == 0) continue;
+    b.e[in++] = Entry{grads[i], clip ? outs[i] : nullptr, sizes[i] << 2 | dtypes[i], first};
+    first += ceil_div(sizes[i], kPiece);
+    if (in == kBatch)
+      if (int rc = flush()) return rc;
+  }
+  if (int rc = flush()) return rc;
+  const int grid = (int)(pieces < kBlocks ? (pieces > 0 ? pieces : 1) : kBlocks);
+  { TraceScope _ts(st, "grad_sum_kernel");
+    grad_sum_kernel<<<grid, kThreads, 0, st>>>(table, (int)used, pieces, part); }
+  if (int rc = check_launch("grad_sum_kernel")) return rc;
+  TraceScope _ts(st, clip ? "grad_scale_kernel" : "grad_norm_kernel");
+  if (clip) grad_scale_kernel<<<grid, kThreads, 0, st>>>(table, (int)used, pieces, part, grid, max_norm, norm);
+  else grad_norm_kernel<<<1, kThreads, 0, st>>>(part, grid, norm);
+  return check_launch("grad_scale_kernel");
+}
+
+// nothing thrown crosses the C boundary (the overlap check allocates)
+template <typename F> int guarded(const char* fn, F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(REELS_HIP_EINVAL, std::string(fn) + ": out of host memory");
+  }
+}
+
+}  // namespace
+}  // namespace reels
+
+extern "C" size_t reels_hip_grad_workspace_bytes(int64_t count) {
+  using namespace reels;
+  if (count < 0 || count > ((int64_t)1 << 24)) return 0;
+  return table_bytes(count) + kBlocks * sizeof(double);
+}
+
+extern "C" int reels_hip_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count,
+                                   float* norm, void* workspace, size_t ws_bytes, void* stream) {
+  using namespace reels;
+  return guarded("reels_hip_grad_norm", [&] {
+    return clip_run("reels_hip_grad_norm", grads, nullptr, sizes, dtypes, count, false, 0.0f, norm, workspace, ws_bytes,
+                    (hipStream_t)stream);
+  });
+}
+
+extern "C" int reels_hip_clip_gradients(const void* const* grads, void* const* outs, const int64_t* sizes,
+                                        const int32_t* dtypes, int64_t count, float max_norm, float* norm,
+                                        void* workspace, size_t ws_bytes, void* stream) {
+  using namespace reels;
+  return guarded("reels_hip_clip_gradients", [&] {
+    return clip_run("reels_hip_clip_gradients", grads, outs, sizes, dtypes, count, true, max_norm, norm, workspace,
+                    ws_bytes, (hipStream_t)stream);
+  });
+}

@@ -43,6 +43,25 @@ def _stream(device: torch.device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """The device as the current one for a launch (a stream belongs to its device); nothing where it
+    is current already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
 def _need_device(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a ROCm device tensor (got {t.device}); the int8 path "

@@ -41,3 +41,30 @@ def assert_parity(got, ref, what: str, tol: float = 1e-2):
     assert norm <= tol, f"{what}: normwise rel err {norm:.3e} > {tol}"
     assert elem <= tol, f"{what}: elementwise rel err {elem:.3e} > {tol}"
     return norm, elem
+
+
+# ---- bounds counted in roundings (the operators around the linears) -----------------------------
+U = 2.0 ** -24  # half a step of an f32 value
+
+
+def half_step(dtype) -> float:
+    """The largest relative error of one rounding to a torch dtype."""
+    import torch
+    return torch.finfo(dtype).eps / 2
+
+
+def assert_within(got, ref, slack, what: str):
+    """|got - ref| <= half a step of got's type on ref, its smallest step, and `slack` (the f32
+    errors before the rounding, elementwise); non-finite values agree exactly."""
+    import torch
+    g, r = got.detach().double().cpu(), ref.detach().double().cpu()
+    slack = slack.detach().double().cpu() if isinstance(slack, torch.Tensor) else slack
+    assert g.shape == r.shape, f"{what}: shape {tuple(g.shape)}, expected {tuple(r.shape)}"
+    fin = torch.isfinite(r)
+    assert torch.equal(torch.isnan(g), torch.isnan(r)), f"{what}: NaN in other places"
+    assert torch.equal(g[~fin & ~torch.isnan(r)], r[~fin & ~torch.isnan(r)]), f"{what}: infinities differ"
+    info = torch.finfo(got.dtype)
+    tol = r.abs() * half_step(got.dtype) * (1 + 2 ** -7) + info.smallest_normal * info.eps + slack
+    bad = fin & ~((g - r).abs() <= tol)
+    assert not bool(bad.any()), (f"{what}: {int(bad.sum())} of {g.numel()} off, worst "
+                                 f"{float(((g - r).abs() / tol)[bad].max()):.3g} times the bound")
