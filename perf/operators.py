@@ -259,6 +259,14 @@ def _plain_clip(st):
     return st["flat"], norm
 
 
+def _values(rows):
+    """The values of int8 rows in their type: code times f32 scale, rounded once (dequantize rounds
+    the scale to binary16 first where that is the type)."""
+    if rows.compute_dtype == torch.float16:
+        return rows.dequantize(torch.float32).half()
+    return rows.dequantize()
+
+
 def run(st):
     case = st["case"]
     op = case["op"]
@@ -271,7 +279,7 @@ def run(st):
             return n.output, n.sum, g.x, g.weight
         if op == "norm_i8":
             n = ra.rms_norm_quantized(st["x"], st["w"], eps=_EPS, residual=st["residual"])
-            return n.output.dequantize(), n.sum
+            return _values(n.output), n.sum
         if op == "product":
             dt = _DT[case["dtype"]]
             return ra.quantized_linear(ra.QuantizedMatrix(st["xq"], st["xs"], dt),
