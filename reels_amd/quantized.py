@@ -68,11 +68,14 @@ def quantized_linear(x: QuantizedMatrix, weight: QuantizedMatrix,
     bias, residual = _contig(bias, dt, "bias"), _contig(residual, dt, "residual")
     y = torch.empty((M, N), dtype=dt, device=dev)
     L = _lib.lib()
-    nbytes = L.reels_hip_i8i8_workspace_bytes(M, K, N)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    px, pw = x.values.data_ptr(), weight.values.data_ptr()
+    ws, nbytes = None, 0
+    if K % 128 or (px | pw) & 15:  # zero-padded copies of the codes
+        nbytes = L.reels_hip_i8i8_workspace_bytes(M, K, N)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     with on_device(dev):
         _lib.check("reels_hip_i8i8_linear", L.reels_hip_i8i8_linear(
-            _ptr(x.values), _ptr(x.scales), _ptr(weight.values), _ptr(weight.scales), _ptr(bias),
+            px, _ptr(x.scales), pw, _ptr(weight.scales), _ptr(bias),
             _ptr(residual), _ACTIVATIONS[activation], _DTYPE_CODE[dt], M, K, N, _ptr(y), _ptr(ws),
             nbytes, _stream(dev)))
     return y
