@@ -52,7 +52,7 @@ __device__ __forceinline__ int find_entry(const Entry* table, int count, int64_t
 }
 
 __device__ __forceinline__ double block_sum(double v, double* slot) {
-  v = group_sum<64>(v);
+  v = group_reduce<64, false>(v);
   if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
   __syncthreads();
   v = slot[0];
@@ -61,28 +61,37 @@ __device__ __forceinline__ double block_sum(double v, double* slot) {
   return v;
 }
 
+// f(first element, how many exist) for this thread's vectors of a piece; the whole ones four at a time,
+// so that four loads are in flight
+template <int V, typename F> __device__ __forceinline__ void each_vec(int64_t n, F&& f) {
+  const int m = (int)n, full = m / (kThreads * V);
+#pragma unroll 4
+  for (int it = 0; it < full; ++it) f((it * kThreads + (int)threadIdx.x) * V, V);
+  const int i = (full * kThreads + (int)threadIdx.x) * V;
+  if (i < m) f(i, m - i < V ? m - i : V);
+}
+
 template <int ELT> __device__ __forceinline__ double piece_sum(const void* g, int64_t n) {
   constexpr int V = 16 / elt_bytes(ELT);
   double t = 0.0;
-  for (int64_t i = (int64_t)threadIdx.x * V; i < n; i += kThreads * V) {
+  each_vec<V>(n, [&](int i, int left) {
     float f[V];
-    load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), n - i < V ? (int)(n - i) : V, f);
+    load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), left, f);
 #pragma unroll
     for (int j = 0; j < V; ++j) t = fma((double)f[j], (double)f[j], t);
-  }
+  });
   return t;
 }
 
 template <int ELT> __device__ __forceinline__ void piece_scale(const void* g, void* o, int64_t n, float factor) {
   constexpr int V = 16 / elt_bytes(ELT);
-  for (int64_t i = (int64_t)threadIdx.x * V; i < n; i += kThreads * V) {
+  each_vec<V>(n, [&](int i, int left) {
     float f[V];
-    const int left = n - i < V ? (int)(n - i) : V;
     load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), left, f);
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] *= factor;
     store_vec<ELT, V>((uint8_t*)o + i * elt_bytes(ELT), left, f);
-  }
+  });
 }
 
 template <typename F> __device__ __forceinline__ void with_type(int t, F&& f) {

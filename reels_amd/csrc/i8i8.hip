@@ -459,27 +459,16 @@ int launch_small(const ProductArgs& a, int dtype, hipStream_t st) {
 }
 
 // rows of K codes at any address to rows of Kp (a multiple of 128), zeros past K; both operands in
-// one launch (rows past r0 belong to the second)
+// one launch (rows past r0 belong to the second), a wave per row
 __global__ __launch_bounds__(256) void product_pad_kernel(const int8_t* __restrict__ x, int64_t r0, const int8_t* __restrict__ w,
                                                           int64_t r1, int K, int Kp, int8_t* __restrict__ px,
                                                           int8_t* __restrict__ pw) {
-  const int64_t per = Kp / 16, total = (r0 + r1) * per, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    int64_t r = i / per;
-    const int c = (int)(i - r * per) * 16;
-    const int8_t* src = x;
-    int8_t* dst = px;
-    if (r >= r0) { r -= r0; src = w; dst = pw; }
-    src += r * K;
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (c + 16 <= K) {
-      v = load_any<u32x4>(src + c);
-    } else {
-#pragma unroll
-      for (int b = 0; b < 16; ++b)
-        if (c + b < K) v[b / 4] |= (uint32_t)(uint8_t)src[c + b] << (8 * (b % 4));
-    }
-    *reinterpret_cast<u32x4*>(dst + r * Kp + c) = v;
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < r0 + r1; i += (int64_t)gridDim.x * 4) {
+    const bool second = i >= r0;
+    const int64_t r = second ? i - r0 : i;
+    const int8_t* src = (second ? w : x) + r * K;
+    int8_t* dst = (second ? pw : px) + r * Kp;
+    for (int c = (threadIdx.x & 63) * 16; c < Kp; c += 1024) *reinterpret_cast<i32v4*>(dst + c) = load_codes(src + c, K - c);
   }
 }
 
@@ -565,7 +554,7 @@ extern "C" int reels_hip_i8i8_linear(const int8_t* x, const float* xs, const int
     const int Kp = (int)align_up((size_t)K, 128);
     int8_t* px = (int8_t*)align_up((size_t)workspace, 256);
     int8_t* pw = px + M * Kp;
-    const int64_t blocks = ceil_div((M + N) * (Kp / 16), 256);
+    const int64_t blocks = ceil_div(M + N, 4);
     { TraceScope _ts(st, "product_pad_kernel");
       product_pad_kernel<<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(x, M, w, N, (int)K, Kp, px, pw); }
     if (int rc = check_launch("product_pad_kernel")) return rc;

@@ -12,9 +12,9 @@
 //
 // All of it is bound by memory: each kernel reads its operands once and keeps the row in registers
 // between the reduction and the output. A row belongs to a group of TPR threads that hold NCH
-// 16-byte chunks each: TPR is the smallest of 16, 64, 256 and 1024 whose threads need at most four
-// chunks, so short rows (one head) share a wave and long ones have many loads in flight; rows past
-// 4096 chunks (32768 16-bit elements) run the loop form, which reads the row again from L2. Squares
+// 16-byte chunks each: TPR is the smallest of 16, 64 and 256 whose threads need at most four
+// chunks, or 1024 with two, so short rows (one head) share a wave and long ones have many loads in
+// flight; rows past 2048 chunks (16384 16-bit elements) run the loop form, which reads them again from L2. Squares
 // and products are summed in 64 bits (MI355X adds those at the rate of 32-bit ones), so rows of any
 // magnitude that the type holds have the norm that they should.
 #include "vec.h"
@@ -34,6 +34,7 @@ struct NormArgs {
   int8_t* q;
   float* scales;
   int64_t ld_x, ld_r, rows, cols;
+  double per_col;    // 1 / cols
   float eps;
   int w_f32;         // w holds f32 (else the row's type)
 };
@@ -41,7 +42,7 @@ struct NormArgs {
 // sum (or maximum) over the TPR threads of a row's group; slot: per-block LDS, one per wave
 template <int TPR, bool MAX> __device__ __forceinline__ double row_reduce(double v, double* slot) {
   constexpr int G = TPR < 64 ? TPR : 64;
-  v = MAX ? group_max<G>(v) : group_sum<G>(v);
+  v = group_reduce<G, MAX>(v);
   if constexpr (TPR > 64) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) slot[wave] = v;
@@ -49,7 +50,7 @@ template <int TPR, bool MAX> __device__ __forceinline__ double row_reduce(double
     const int first = wave / (TPR / 64) * (TPR / 64);
     v = slot[first];
 #pragma unroll
-    for (int i = 1; i < TPR / 64; ++i) v = MAX ? fmax(v, slot[first + i]) : v + slot[first + i];
+    for (int i = 1; i < TPR / 64; ++i) v = join<MAX>(v, slot[first + i]);
   }
   return v;
 }
@@ -65,174 +66,332 @@ template <int ELT, int V> __device__ __forceinline__ void load_weight(const void
   }
 }
 
-// the 127 steps of a row: |p| with every non-finite value as infinity, which the maximum keeps
+// What a row's codes take from it: the largest |s w| in 64 bits and its quotients' factors. even: every
+// weight is below 1e20 (and none is NaN).
+struct Quant {
+  double top, inv;  // codes are 127 p / top = p inv
+  float f1, f2;     // in f32: (s f1) w f2
+  bool zero, fast;
+  float scale;
+  __device__ __forceinline__ Quant(double t, double rstd, bool even) : top(t) {
+    const double size = top * rstd;  // the row's largest value
+    scale = (float)(size * (1.0 / 127.0));
+    const bool whole = __builtin_isfinite(scale);
+    if (!whole) scale = __builtin_nanf("");
+    else if (top == 0.0) scale = 1.0f;
+    zero = !whole || top == 0.0;
+    inv = 127.0 * rcp64(top);
+    f1 = (float)rstd;
+    f2 = (float)(127.0 * rcp64(size));
+    // In f32 the factors and the products that matter keep all their bits: a value (s rstd) that has
+    // lost some is below 2^-126, its product with an even weight below 1e-17, its code 0
+    fast = even && size > 1e-10 && size < 1e30 && rstd > 1e-30 && rstd < 1e30;
+  }
+};
+
+// the largest |s w| may be infinite: NaN counts as infinity, which the maximum keeps
 __device__ __forceinline__ double quant_abs(double p) {
   const double a = fabs(p);
   return a <= 1.7976931348623157e308 ? a : __builtin_inf();
 }
-// round_ties_even(127 p / top): the product with the reciprocal is within 2^-50 of the quotient, so
-// only values next to a border take the division
-__device__ __forceinline__ int quant_code(double p, double top, double inv) {
-  double t = p * inv, k = rint(t);
-  if (fabs(t - k) > 0.4999999999) k = rint(127.0 * p / top);
+// the largest |w| and |s w| of a chunk. wide: NaN stays (v_maximum3); the products in f32 where they
+// are exact, two 16-bit significands (the range is looked at by the caller), else in 64 bits
+template <bool EXACT32, int V>
+__device__ __forceinline__ void quant_top(const float (&s)[V], const float (&w)[V], double& top, float& wide) {
+  if constexpr (EXACT32) {
+    float t = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; j += 2) t = fmaxf(t, fmaxf(fabsf(s[j] * w[j]), fabsf(s[j + 1] * w[j + 1])));
+    top = fmax(top, (double)t);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = fmax(top, fabs((double)s[j] * (double)w[j]));
+  }
+#pragma unroll
+  for (int j = 0; j < V; j += 2)
+    wide = __builtin_elementwise_maximum(wide, __builtin_elementwise_maximum(fabsf(w[j]), fabsf(w[j + 1])));
+}
+
+// round_ties_even(127 p / top) of a product formed in 64 bits: p inv is within 2^-50 of the quotient,
+// so only values next to a border take the division
+__device__ __forceinline__ int quant_exact(float s, float w, const Quant& q) {
+  const double p = (double)s * (double)w, t = p * q.inv;
+  double k = rint(t);
+  if (fabs(t - k) > 0.4999999999) k = rint(127.0 * p / q.top);
   return (int)k;
 }
 
-template <int V> __device__ __forceinline__ void store_codes(int8_t* q, int left, const int (&c)[V]) {
-  struct Pack { int8_t e[V]; };
-  if (left >= V) {
-    Pack p;
+// The codes of a chunk, four to a word. In f32 the quotient has at most five roundings, 127 * 5 * 2^-24 = 3.8e-5: a chunk
+// with a value within 2^-14 of a border (6% of a wave's) is formed in 64 bits. Adding 1.5 * 2^23
+// rounds to a whole number, ties to even, and leaves it in the low byte.
+template <bool EXACT32, int V>
+__device__ __forceinline__ void quant_chunk(const float (&s)[V], const float (&w)[V], const Quant& q, uint32_t (&word)[V / 4]) {
+  float far = q.fast ? 0.0f : 1.0f;
+  uint32_t c[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) p.e[i] = (int8_t)c[i];
+  for (int j = 0; j < V; ++j) {
+    const float p = EXACT32 ? s[j] * w[j] : s[j] * q.f1 * w[j], f = EXACT32 ? (float)q.inv : q.f2;
+    const float m = fmaf(p, f, 12582912.0f);
+    far = fmaxf(far, fabsf(fmaf(p, f, -(m - 12582912.0f))));
+    c[j] = __float_as_uint(m);
+  }
+  if (far > 0.5f - 0x1p-14f) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[j] = (uint32_t)quant_exact(s[j], w[j], q);
+  }
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    const uint32_t lo = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x04000c0cu);
+    word[i] = q.zero ? 0u : lo | hi;
+  }
+}
+
+template <int V> __device__ __forceinline__ void store_codes(int8_t* q, int left, const uint32_t (&word)[V / 4]) {
+  struct Pack { int8_t e[V]; };
+  const Pack p = __builtin_bit_cast(Pack, word);
+  if (left >= V) {
     store_any(q, p);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < left) q[i] = (int8_t)c[i];
+      if (i < left) q[i] = p.e[i];
   }
 }
 
-template <int ELT, int TPR, int NCH, bool QUANT>
+// Where a thread's chunks of a row lie: chunk i at element col(i). Whole chunks are read without a
+// branch, from the row's first chunk where there is none (and zeroed), so that all loads of a row are
+// in flight together; the one partial chunk of a row whose length is no multiple of V, by elements.
+template <int ELT, int TPR, int NCH> struct Row {
+  static constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
+  int cols, lane, base;
+  bool live;  // a group past the last row takes part in the barriers
+  __device__ __forceinline__ Row(int64_t n, bool l) : cols((int)n), live(l) {
+    lane = threadIdx.x % TPR;
+    // the wave's first chunk, in a scalar register: chunks that no lane of the wave has are skipped
+    base = TPR > 64 ? __builtin_amdgcn_readfirstlane(lane & ~63) : 0;
+  }
+  __device__ __forceinline__ int col(int i) const { return (lane + TPR * i) * V; }
+  __device__ __forceinline__ bool some(int i) const { return (base + TPR * i) * V < cols; }
+  __device__ __forceinline__ bool full(int i) const { return live && col(i) + V <= cols; }
+  __device__ __forceinline__ bool part(int i) const { return live && col(i) < cols && col(i) + V > cols; }
+  __device__ __forceinline__ int left(int i) const { return cols - col(i); }
+  template <int E> __device__ __forceinline__ void load(const void* row, Chunk<E> (&d)[NCH]) const {
+    const uint8_t* p = (const uint8_t*)row;
+    if (cols >= V) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (some(i)) d[i].d = load_any<u32x4>((const typename Store<E>::raw*)(p + (int64_t)(full(i) ? col(i) : 0) * EB));
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+      if (!some(i) || !full(i)) d[i].zero();
+    if (cols % V != 0) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (part(i)) d[i].load(p + (int64_t)col(i) * EB, left(i));
+    }
+  }
+  // weights as f32, ones without any; f32 ones of a 16-bit row take two vectors a chunk
+  __device__ __forceinline__ void load_w(const void* w, int w_f32, float (&f)[NCH][V]) const {
+    if (w == nullptr) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[i][j] = 1.0f;
+      return;
+    }
+    if (cols >= V) {
+      if (w_f32) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+          if (some(i)) load_vec<REELS_HIP_F32, V>((const float*)w + (full(i) ? col(i) : 0), V, f[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+          if (some(i)) load_vec<ELT, V>((const uint8_t*)w + (int64_t)(full(i) ? col(i) : 0) * EB, V, f[i]);
+      }
+    }
+    if (cols % V != 0) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (part(i)) load_weight<ELT, V>(w, w_f32, col(i), left(i), f[i]);
+    }
+  }
+  __device__ __forceinline__ void store(void* row, int i, const Chunk<ELT>& d) const {
+    uint8_t* p = (uint8_t*)row + (int64_t)col(i) * EB;
+    if (full(i)) store_any((typename Store<ELT>::raw*)p, d.d);
+    else if (part(i)) d.store(p, left(i));
+  }
+};
+
+// MODE 0: y; 1: int8 rows; 2: the same with 16-bit values and weights (or none)
+template <int ELT, int TPR, int NCH, int MODE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormArgs a) {
-  constexpr int V = 16 / elt_bytes(ELT), EB = elt_bytes(ELT), NT = TPR < 256 ? 256 : TPR;
+  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), NT = TPR < 256 ? 256 : TPR;
+  constexpr bool QUANT = MODE > 0, EXACT32 = MODE == 2;
   __shared__ double slots[2][NT / 64];
-  const int lane = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
-  const bool live = row < a.rows;  // a group past the end takes part in the barriers
-  float s[NCH][V];
+  const int64_t row0 = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const Row<ELT, TPR, NCH> at(a.cols, row0 < a.rows);
+  const int64_t row = at.live ? row0 : a.rows - 1;
+  Chunk<ELT> s[NCH], r[NCH];
+  float w[NCH][V];
+  at.load((const uint8_t*)a.x + row * a.ld_x * EB, s);
+  if (a.res != nullptr) at.load((const uint8_t*)a.res + row * a.ld_r * EB, r);
+  if constexpr (!QUANT) at.load_w(a.w, a.w_f32, w);
   double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    const int64_t c = (int64_t)(lane + TPR * i) * V;
-    const int left = live && c < a.cols ? (a.cols - c < V ? (int)(a.cols - c) : V) : 0;
-    if (left <= 0) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[i][j] = 0.0f;
-      continue;
-    }
-    load_vec<ELT, V>((const uint8_t*)a.x + (row * a.ld_x + c) * EB, left, s[i]);
+    if (!at.some(i)) continue;
     if (a.res != nullptr) {
-      float r[V];
-      load_vec<ELT, V>((const uint8_t*)a.res + (row * a.ld_r + c) * EB, left, r);
+      float f[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[i][j] = Store<ELT>::get(Store<ELT>::put(s[i][j] + r[j]));
+      for (int j = 0; j < V; ++j) f[j] = s[i].get(j) + r[i].get(j);
+      s[i].pack(f);
+      at.store((uint8_t*)a.sum + row * a.cols * EB, i, s[i]);
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) ss = fma((double)s[i].get(j), (double)s[i].get(j), ss);
+    s[i].hold();
   }
-#pragma unroll
-  for (int i = 0; i < NCH; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) ss = fma((double)s[i][j], (double)s[i][j], ss);
+  if constexpr (QUANT) at.load_w(a.w, a.w_f32, w);
   ss = row_reduce<TPR, false>(ss, slots[0]);
-  const double rstd = 1.0 / sqrt(ss / (double)a.cols + (double)a.eps);
-  float w[NCH][V];
-  double top = 0.0;
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int64_t c = (int64_t)(lane + TPR * i) * V;
-    const int left = live && c < a.cols ? (a.cols - c < V ? (int)(a.cols - c) : V) : 0;
-    if (left <= 0) continue;
-    if (a.res != nullptr) store_vec<ELT, V>((uint8_t*)a.sum + (row * a.cols + c) * EB, left, s[i]);
-    load_weight<ELT, V>(a.w, a.w_f32, c, left, w[i]);
-    if constexpr (QUANT) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) top = fmax(top, quant_abs((double)s[i][j] * (double)w[i][j]));
-    } else {
-      const float rs = (float)rstd;
-      float y[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = s[i][j] * rs * w[i][j];
-      store_vec<ELT, V>((uint8_t*)a.y + (row * a.cols + c) * EB, left, y);
-    }
-  }
-  if constexpr (QUANT) {
-    top = row_reduce<TPR, true>(top, slots[1]);
-    float scale = (float)(top * rstd / 127.0);
-    const bool whole = __builtin_isfinite(scale);
-    if (!whole) scale = __builtin_nanf("");
-    if (top == 0.0 && whole) scale = 1.0f;
-    if (live && lane == 0) a.scales[row] = scale;
-    const bool zero = !whole || top == 0.0;
-    const double inv = 127.0 / top;
+  const double rstd = rsqrt64(fma(ss, a.per_col, (double)a.eps));
+  if constexpr (!QUANT) {
+    const float rs = (float)rstd;
+    if (at.live && at.lane == 0) a.rstd[row] = rs;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int64_t c = (int64_t)(lane + TPR * i) * V;
-      const int left = live && c < a.cols ? (a.cols - c < V ? (int)(a.cols - c) : V) : 0;
-      if (left <= 0) continue;
-      int code[V];
+      if (!at.some(i)) continue;
+      float y[V];
+      Chunk<ELT> o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) code[j] = zero ? 0 : quant_code((double)s[i][j] * (double)w[i][j], top, inv);
-      store_codes<V>(a.q + row * a.cols + c, left, code);
+      for (int j = 0; j < V; ++j) y[j] = s[i].get(j) * rs * w[i][j];
+      o.pack(y);
+      at.store((uint8_t*)a.y + row * a.cols * EB, i, o);
     }
-  } else if (live && lane == 0) {
-    a.rstd[row] = (float)rstd;
+  } else {
+    double top = 0.0;
+    float wide = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (!at.some(i)) continue;
+      if (at.full(i) || at.part(i)) {
+        float f[V];
+        s[i].unpack(f);
+        quant_top<EXACT32, V>(f, w[i], top, wide);
+      }
+      s[i].hold();
+    }
+    top = row_reduce<TPR, true>(wide <= 1e20f ? top : __builtin_inf(), slots[1]);
+    bool even = top < __builtin_inf();
+    if (EXACT32 && !(top > 1e-30 && top < 1e30)) even = false;  // f32 products out of its range
+    if (!even) {  // once more in 64 bits, with NaN seen (a row's threads take this together)
+      top = 0.0;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        if (!(at.full(i) || at.part(i))) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < at.left(i)) top = fmax(top, quant_abs((double)s[i].get(j) * (double)w[i][j]));
+      }
+      top = row_reduce<TPR, true>(top, slots[0]);
+    }
+    const Quant q(top, rstd, even);
+    if (at.live && at.lane == 0) a.scales[row] = q.scale;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (!(at.full(i) || at.part(i))) continue;
+      float f[V];
+      uint32_t word[V / 4];
+      s[i].unpack(f);
+      quant_chunk<EXACT32, V>(f, w[i], q, word);
+      store_codes<V>(a.q + row * a.cols + at.col(i), at.left(i), word);
+    }
+  }
+}
+
+// s of a chunk: x, or x + residual rounded to the type
+template <int ELT> __device__ __forceinline__ void load_sum(const NormArgs& a, int64_t row, int64_t c, int left, Chunk<ELT>& s) {
+  constexpr int EB = elt_bytes(ELT), V = Chunk<ELT>::V;
+  s.load((const uint8_t*)a.x + (row * a.ld_x + c) * EB, left);
+  if (a.res != nullptr) {
+    Chunk<ELT> r;
+    r.load((const uint8_t*)a.res + (row * a.ld_r + c) * EB, left);
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = s.get(j) + r.get(j);
+    s.pack(f);
   }
 }
 
 // rows past the register form: one workgroup per row, the row read again for its output
 template <int ELT, bool QUANT>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs a) {
-  constexpr int V = 16 / elt_bytes(ELT), EB = elt_bytes(ELT);
+  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
   __shared__ double slots[2][kLongThreads / 64];
   const int64_t row = blockIdx.x;
   double ss = 0.0, top = 0.0;
-  auto load_sum = [&](int64_t c, int left, float (&s)[V]) {
-    load_vec<ELT, V>((const uint8_t*)a.x + (row * a.ld_x + c) * EB, left, s);
-    if (a.res != nullptr) {
-      float r[V];
-      load_vec<ELT, V>((const uint8_t*)a.res + (row * a.ld_r + c) * EB, left, r);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[j] = Store<ELT>::get(Store<ELT>::put(s[j] + r[j]));
-    }
-  };
+  float wide = 0.0f;
   for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += kLongThreads * V) {
     const int left = a.cols - c < V ? (int)(a.cols - c) : V;
-    float s[V], w[V];
-    load_sum(c, left, s);
+    Chunk<ELT> s;
+    load_sum<ELT>(a, row, c, left, s);
 #pragma unroll
-    for (int j = 0; j < V; ++j) ss = fma((double)s[j], (double)s[j], ss);
+    for (int j = 0; j < V; ++j) ss = fma((double)s.get(j), (double)s.get(j), ss);
     if constexpr (QUANT) {
+      float w[V];
       load_weight<ELT, V>(a.w, a.w_f32, c, left, w);
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < left) top = fmax(top, quant_abs((double)s[j] * (double)w[j]));
+      float f[V];
+      s.unpack(f);
+      quant_top<false, V>(f, w, top, wide);
     }
   }
   ss = row_reduce<kLongThreads, false>(ss, slots[0]);
-  const double rstd = 1.0 / sqrt(ss / (double)a.cols + (double)a.eps);
-  float scale = 1.0f;
-  bool zero = false;
-  double inv = 0.0;
+  const double rstd = rsqrt64(fma(ss, a.per_col, (double)a.eps));
+  bool even = true;
   if constexpr (QUANT) {
-    top = row_reduce<kLongThreads, true>(top, slots[1]);
-    scale = (float)(top * rstd / 127.0);
-    const bool whole = __builtin_isfinite(scale);
-    if (!whole) scale = __builtin_nanf("");
-    if (top == 0.0 && whole) scale = 1.0f;
-    zero = !whole || top == 0.0;
-    inv = 127.0 / top;
-    if (threadIdx.x == 0) a.scales[row] = scale;
-  } else if (threadIdx.x == 0) {
-    a.rstd[row] = (float)rstd;
+    top = row_reduce<kLongThreads, true>(wide <= 1e20f ? top : __builtin_inf(), slots[1]);
+    even = top < __builtin_inf();
+    if (!even) {
+      top = 0.0;
+      for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += kLongThreads * V) {
+        const int left = a.cols - c < V ? (int)(a.cols - c) : V;
+        Chunk<ELT> s;
+        float w[V];
+        load_sum<ELT>(a, row, c, left, s);
+        load_weight<ELT, V>(a.w, a.w_f32, c, left, w);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < left) top = fmax(top, quant_abs((double)s.get(j) * (double)w[j]));
+      }
+      top = row_reduce<kLongThreads, true>(top, slots[0]);
+    }
+  }
+  const Quant q(top, rstd, even);
+  if (threadIdx.x == 0) {
+    if constexpr (QUANT) a.scales[row] = q.scale;
+    else a.rstd[row] = (float)rstd;
   }
   // the sum is written here, after every read of x and the residual's first pass, chunk by chunk by
   // the thread that read it, so it may take the place of x or of the residual
   for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += kLongThreads * V) {
     const int left = a.cols - c < V ? (int)(a.cols - c) : V;
-    float s[V], w[V];
-    load_sum(c, left, s);
+    Chunk<ELT> s;
+    float w[V], f[V];
+    load_sum<ELT>(a, row, c, left, s);
     load_weight<ELT, V>(a.w, a.w_f32, c, left, w);
-    if (a.res != nullptr) store_vec<ELT, V>((uint8_t*)a.sum + (row * a.cols + c) * EB, left, s);
+    s.unpack(f);
+    if (a.res != nullptr) s.store((uint8_t*)a.sum + (row * a.cols + c) * EB, left);
     if constexpr (QUANT) {
-      int code[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) code[j] = zero ? 0 : quant_code((double)s[j] * (double)w[j], top, inv);
-      store_codes<V>(a.q + row * a.cols + c, left, code);
+      uint32_t word[V / 4];
+      quant_chunk<false, V>(f, w, q, word);
+      store_codes<V>(a.q + row * a.cols + c, left, word);
     } else {
       const float rs = (float)rstd;
-      float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = s[j] * rs * w[j];
-      store_vec<ELT, V>((uint8_t*)a.y + (row * a.cols + c) * EB, left, y);
+      for (int j = 0; j < V; ++j) f[j] = f[j] * rs * w[j];
+      store_vec<ELT, V>((uint8_t*)a.y + (row * a.cols + c) * EB, left, f);
     }
   }
 }
@@ -247,6 +406,7 @@ struct NormBwdArgs {
   void* dx;
   float* part;       // [workgroups][cols] partial dw, or nullptr
   int64_t rows, cols;
+  double per_col;
   int w_f32;
 };
 
@@ -268,55 +428,44 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd_kernel(NormBwd
   }
   int turn = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB, turn ^= 1) {
-    const int64_t row = r0 + group;
-    const bool live = row < a.rows;
-    const float rstd = live ? a.rstd[row] : 0.0f;
-    float s[NCH][V], g[NCH][V];
+    const Row<ELT, TPR, NCH> at(a.cols, r0 + group < a.rows);
+    const int64_t row = at.live ? r0 + group : a.rows - 1, begin = row * a.cols * EB;
+    const float rstd = at.live ? a.rstd[row] : 0.0f;
+    Chunk<ELT> s[NCH], dy[NCH], ds[NCH];
+    float w[NCH][V];
+    at.load((const uint8_t*)a.s + begin, s);
+    at.load((const uint8_t*)a.dy + begin, dy);
+    if (a.dsum != nullptr) at.load((const uint8_t*)a.dsum + begin, ds);
+    at.load_w(a.w, a.w_f32, w);
     double gs = 0.0;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int64_t c = (int64_t)(lane + TPR * i) * V;
-      const int left = live && c < a.cols ? (a.cols - c < V ? (int)(a.cols - c) : V) : 0;
-      if (left <= 0) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[i][j] = g[i][j] = 0.0f;
-        continue;
-      }
-      load_vec<ELT, V>((const uint8_t*)a.s + (row * a.cols + c) * EB, left, s[i]);
-      load_vec<ELT, V>((const uint8_t*)a.dy + (row * a.cols + c) * EB, left, g[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int64_t c = (int64_t)(lane + TPR * i) * V;
-      const int left = live && c < a.cols ? (a.cols - c < V ? (int)(a.cols - c) : V) : 0;
-      if (left <= 0) continue;
-      float w[V];
-      load_weight<ELT, V>(a.w, a.w_f32, c, left, w);
+      if (!at.some(i) || !(at.full(i) || at.part(i))) continue;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if constexpr (DW) dw[i][j] += g[i][j] * (s[i][j] * rstd);
-        g[i][j] *= w[j];
-        gs = fma((double)g[i][j], (double)s[i][j], gs);
+        const float sv = s[i].get(j), d = dy[i].get(j);
+        if constexpr (DW) dw[i][j] += d * (sv * rstd);
+        gs = fma((double)(d * w[i][j]), (double)sv, gs);
       }
+      s[i].hold();
+      dy[i].hold();
     }
     // two slots in turn: a wave may enter the next row's reduction while another still reads this one's
     gs = row_reduce<TPR, false>(gs, slots[turn]);
-    const float k = (float)(gs / (double)a.cols * (double)rstd * (double)rstd);
+    const float k = (float)(gs * a.per_col * (double)rstd * (double)rstd);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int64_t c = (int64_t)(lane + TPR * i) * V;
-      const int left = live && c < a.cols ? (a.cols - c < V ? (int)(a.cols - c) : V) : 0;
-      if (left <= 0) continue;
+      if (!at.some(i)) continue;
       float d[V];
+      Chunk<ELT> o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = rstd * (g[i][j] - s[i][j] * k);
+      for (int j = 0; j < V; ++j) d[j] = rstd * (dy[i].get(j) * w[i][j] - s[i].get(j) * k);
       if (a.dsum != nullptr) {
-        float t[V];
-        load_vec<ELT, V>((const uint8_t*)a.dsum + (row * a.cols + c) * EB, left, t);
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] += t[j];
+        for (int j = 0; j < V; ++j) d[j] += ds[i].get(j);
       }
-      store_vec<ELT, V>((uint8_t*)a.dx + (row * a.cols + c) * EB, left, d);
+      o.pack(d);
+      at.store((uint8_t*)a.dx + begin, i, o);
     }
   }
   if constexpr (DW) {
@@ -368,7 +517,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_long_kernel(NormBwdArgs
       if (j < left) gs = fma((double)g[j], (double)s[j], gs);
   }
   gs = row_reduce<kLongThreads, false>(gs, slots);
-  const float k = (float)(gs / (double)a.cols * (double)rstd * (double)rstd);
+  const float k = (float)(gs * a.per_col * (double)rstd * (double)rstd);
   for (int64_t c = (int64_t)threadIdx.x * V; c < a.cols; c += kLongThreads * V) {
     const int left = a.cols - c < V ? (int)(a.cols - c) : V;
     float s[V], g[V], d[V];
@@ -401,20 +550,23 @@ __global__ __launch_bounds__(256) void norm_dw_long_kernel(NormBwdArgs a) {
   a.part[(int64_t)blockIdx.y * a.cols + c] = t;
 }
 
-// dw[c] = sum over the partial rows in order of 16 slices: 64 columns x 16 slices per workgroup
+// dw[c] = sum over the partial rows: 32 columns x 32 slices per workgroup, slice y adds the rows y,
+// y + 32, ... and the slices follow in order
 __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int n, int64_t cols,
                                                        float* __restrict__ dw) {
-  __shared__ float acc[16][64];
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + x;
+  __shared__ float acc[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + x;
   float t = 0.0f;
-  if (c < cols)
-    for (int r = y; r < n; r += 16) t += part[(int64_t)r * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int r = y; r < n; r += 32) t += part[(int64_t)r * cols + c];
+  }
   acc[y][x] = t;
   __syncthreads();
   if (y == 0 && c < cols) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) t += acc[i][x];
+    for (int i = 1; i < 32; ++i) t += acc[i][x];
     dw[c] = t;
   }
 }
@@ -423,8 +575,9 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
 struct Form { int tpr, nch; };  // tpr 0: the loop form
 Form norm_form(int elt, int64_t cols) {
   const int64_t chunks = ceil_div(cols, 16 / elt_bytes(elt));
-  for (int tpr : {16, 64, 256, 1024})
+  for (int tpr : {16, 64, 256})
     if (chunks <= 4 * tpr) return {tpr, (int)ceil_div(chunks, tpr)};
+  if (chunks <= 2048) return {1024, 2};
   return {0, 0};
 }
 
@@ -442,7 +595,7 @@ template <typename F> void with_form(Form f, F&& g) {
     case 16: nch(Int<16>{}); break;
     case 64: nch(Int<64>{}); break;
     case 256: nch(Int<256>{}); break;
-    default: nch(Int<1024>{}); break;
+    default: g(Int<1024>{}, Int<2>{}); break;
   }
 }
 
@@ -464,6 +617,7 @@ int norm_forward(const char* fn, const char* label, bool quant, NormArgs a, int 
   if (a.x == nullptr || (a.res != nullptr && a.sum == nullptr) || (quant ? a.q == nullptr || a.scales == nullptr : a.y == nullptr || a.rstd == nullptr))
     return fail(REELS_HIP_EINVAL, std::string(fn) + ": NULL operand");
   a.w_f32 = w_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32;
+  a.per_col = 1.0 / (double)a.cols;
   const Form f = norm_form(dtype, a.cols);
   { TraceScope _ts(st, label);
     with_any_elt(dtype, [&](auto e) {
@@ -476,17 +630,19 @@ int norm_forward(const char* fn, const char* label, bool quant, NormArgs a, int 
       with_form(f, [&](auto tpr, auto nch) {
         constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = T < 256 ? 256 : T;
         const unsigned grid = (unsigned)ceil_div(a.rows, NT / T);
-        if (quant) norm_kernel<E, T, C, true><<<grid, NT, 0, st>>>(a);
-        else norm_kernel<E, T, C, false><<<grid, NT, 0, st>>>(a);
+        if (!quant) norm_kernel<E, T, C, 0><<<grid, NT, 0, st>>>(a);
+        else if (E == REELS_HIP_F32 || a.w_f32) norm_kernel<E, T, C, 1><<<grid, NT, 0, st>>>(a);
+        else if constexpr (E != REELS_HIP_F32) norm_kernel<E, T, C, 2><<<grid, NT, 0, st>>>(a);
       });
     }); }
   return check_launch(label);
 }
 
-// workgroups of the backward with dw (each writes one partial row): enough to fill the GPU
+// workgroups of the backward with dw (each writes one partial row): enough to fill the GPU, and at
+// least two rows for each group of threads, so that the partial rows stay a small part of the traffic
 int64_t norm_parts(int64_t rows, Form f) {
   const int64_t rpb = f.tpr == 0 ? 1 : (f.tpr < 256 ? 256 / f.tpr : 1);
-  const int64_t want = f.tpr == 0 ? 64 : (f.tpr <= 256 ? 1024 : 256), need = ceil_div(rows, rpb);
+  const int64_t want = f.tpr == 0 ? 64 : (f.tpr <= 256 ? 1024 : 256), need = ceil_div(rows, 2 * rpb);
   return need < want ? need : want;
 }
 
@@ -498,7 +654,7 @@ extern "C" int reels_hip_rms_norm(const void* x, int64_t ld_x, const void* resid
                                   float* rstd, void* stream) {
   using namespace reels;
   return norm_forward("reels_hip_rms_norm", "norm_kernel", false,
-                      NormArgs{x, residual, weight, sum, y, rstd, nullptr, nullptr, ld_x, ld_r, rows, cols, eps, 0}, dtype,
+                      NormArgs{x, residual, weight, sum, y, rstd, nullptr, nullptr, ld_x, ld_r, rows, cols, 0.0, eps, 0}, dtype,
                       w_dtype, (hipStream_t)stream);
 }
 
@@ -507,7 +663,7 @@ extern "C" int reels_hip_rms_norm_i8(const void* x, int64_t ld_x, const void* re
                                      float* scales, void* stream) {
   using namespace reels;
   return norm_forward("reels_hip_rms_norm_i8", "norm_kernel<int8>", true,
-                      NormArgs{x, residual, weight, sum, nullptr, nullptr, q, scales, ld_x, ld_r, rows, cols, eps, 0}, dtype,
+                      NormArgs{x, residual, weight, sum, nullptr, nullptr, q, scales, ld_x, ld_r, rows, cols, 0.0, eps, 0}, dtype,
                       w_dtype, (hipStream_t)stream);
 }
 
@@ -536,7 +692,7 @@ extern "C" int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void*
   if (rows > 0 && (dy == nullptr || s == nullptr || rstd == nullptr || dx == nullptr))
     return fail(REELS_HIP_EINVAL, std::string(fn) + ": NULL operand");
   if (rows == 0 && dw == nullptr) return REELS_HIP_OK;
-  NormBwdArgs a{dy, s, dsum, weight, rstd, dx, (float*)workspace, rows, cols, w_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32};
+  NormBwdArgs a{dy, s, dsum, weight, rstd, dx, (float*)workspace, rows, cols, 1.0 / (double)cols, w_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32};
   const Form f = norm_form(dtype, cols);
   const int64_t parts = rows == 0 ? 0 : norm_parts(rows, f);
   if (rows > 0) {
@@ -558,6 +714,6 @@ extern "C" int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void*
   if (int rc = check_launch("norm_bwd_kernel")) return rc;
   if (dw == nullptr) return REELS_HIP_OK;
   { TraceScope _ts(st, "norm_dw_kernel");
-    norm_dw_kernel<<<(unsigned)ceil_div(cols, 64), 1024, 0, st>>>((const float*)workspace, (int)parts, cols, dw); }
+    norm_dw_kernel<<<(unsigned)ceil_div(cols, 32), 1024, 0, st>>>((const float*)workspace, (int)parts, cols, dw); }
   return check_launch("norm_dw_kernel");
 }

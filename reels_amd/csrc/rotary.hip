@@ -151,9 +151,11 @@ extern "C" int reels_hip_rotary(const void* q, int64_t ld_q, const void* k, int6
   a.tokens = B * S;
   a.S = (int)S; a.D = (int)D; a.P = (int)P; a.axes = axes; a.inverse = inverse != 0;
   a.heads[0] = (int)Hq; a.heads[1] = (int)Hk;
-  // tokens of a workgroup: about 2048 items of 16 bytes, so that the angles are a small part of its work
+  // tokens of a workgroup: about 32 KiB, so that the angles are a small part of its work, but no more
+  // than leaves 2048 workgroups (1560 tokens of 6 KiB: 11.2 us in workgroups of five)
   const int64_t token_bytes = (Hq + Hk) * D * elt_bytes(dtype);
   int64_t tb = 32768 / token_bytes;
+  if (tb > a.tokens / 2048) tb = a.tokens / 2048;
   a.tb = (int)(tb < 1 ? 1 : tb > 16 ? 16 : tb);
   const unsigned grid = (unsigned)ceil_div(a.tokens, a.tb);
   const size_t lds = (size_t)a.tb * P * sizeof(float2);

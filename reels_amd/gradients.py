@@ -6,12 +6,13 @@ from __future__ import annotations
 
 import math
 from array import array
+from operator import attrgetter
 from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
-from .layers import _DTYPE_CODE, _need_device, _ptr, _stream, on_device
+from .layers import _DTYPE_CODE, _launch, _need_device, _stream
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -26,80 +27,92 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _tensors(grads, name):
-    if not all(isinstance(g, torch.Tensor) for g in grads):
+# A call's host time is that of these loops, 25 to 50 ns a tensor for each property that is read (800
+# tensors and their outputs: 0.74 ms with a statement for each check, 0.22 ms alone to compare their
+# shapes), so every property is read once, by one map over the list.
+_T = torch.Tensor
+_dtype = attrgetter("dtype")
+
+
+def _tensors(ts, name):
+    """(types, sizes, whether all are contiguous) of a list of tensors on one device."""
+    if not all(issubclass(c, _T) for c in set(map(type, ts))):
         raise TypeError(f"{name} must be tensors")
-    for g in grads:
-        if g.dtype not in _DTYPE_CODE:
-            raise TypeError(f"{name} must be float32, bfloat16 or float16, got {g.dtype}")
-        _need_device(g, name)
-    if len({g.device for g in grads}) > 1:
+    types = list(map(_dtype, ts))
+    for d in set(types):
+        if d not in _DTYPE_CODE:
+            raise TypeError(f"{name} must be float32, bfloat16 or float16, got {d}")
+    devices = set(map(_T.get_device, ts))
+    if -1 in devices:
+        for t in ts:
+            _need_device(t, name)
+    if len(devices) > 1:
         raise ValueError(f"{name} lie on several devices")
+    return types, array("q", map(_T.numel, ts)), all(map(_T.is_contiguous, ts))
 
 
 def _pointers(ts):
-    return array("q", [t.data_ptr() for t in ts])
+    return array("q", map(_T.data_ptr, ts))
 
 
-def _call(grads, max_norm, outs):
-    _tensors(grads, "gradients")
-    if not all(map(_dense, grads)):
+def _call(grads, checked, max_norm, out):
+    types, sizes, contiguous = checked
+    if not contiguous and not all(map(_dense, grads)):
         raise ValueError("gradients must be dense")
-    dev = grads[0].device
-    n = len(grads)
-    L = _lib.lib()
-    ptrs, sizes = _pointers(grads), array("q", [g.numel() for g in grads])
-    types = array("i", [_DTYPE_CODE[g.dtype] for g in grads])
+    dev, n = grads[0].device, len(grads)
+    ptrs, codes = _pointers(grads), array("i", map(_DTYPE_CODE.__getitem__, types))
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = L.reels_hip_grad_workspace_bytes(n)
+    nbytes = _lib.lib().reels_hip_grad_workspace_bytes(n)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-
-    def at(a):
-        return a.buffer_info()[0]
-
-    with on_device(dev):
-        if max_norm is None:
-            _lib.check("reels_hip_grad_norm", L.reels_hip_grad_norm(
-                at(ptrs), at(sizes), at(types), n, _ptr(norm), _ptr(ws), nbytes, _stream(dev)))
-        else:
-            to = ptrs if outs is grads else _pointers(outs)
-            _lib.check("reels_hip_clip_gradients", L.reels_hip_clip_gradients(
-                at(ptrs), at(to), at(sizes), at(types), n, float(max_norm), _ptr(norm), _ptr(ws),
-                nbytes, _stream(dev)))
+    of, to = ptrs.buffer_info()[0], (sizes.buffer_info()[0], codes.buffer_info()[0], n)
+    end = (norm.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
+    if max_norm is None:
+        _launch("reels_hip_grad_norm", dev, of, *to, *end)
+    else:
+        outs = ptrs if out is None else _pointers(out)
+        _launch("reels_hip_clip_gradients", dev, of, outs.buffer_info()[0], *to, max_norm, *end)
     return norm
+
+
+def _without_none(ts):
+    return [t for t in ts if t is not None]
 
 
 def gradient_norm(grads: Sequence[Optional[torch.Tensor]]) -> torch.Tensor:
     """sqrt of the sum of squares of all elements of all tensors (None entries are skipped), float32
     on their device; the sum runs in 64 bits."""
-    grads = [g for g in grads if g is not None]
+    grads = _without_none(grads)
     if not grads:
         raise ValueError("no gradients")
-    return _call(grads, None, None)
+    return _call(grads, _tensors(grads, "gradients"), None, None)
 
 
 def clip_gradients(grads: Sequence[Optional[torch.Tensor]], max_norm: float,
                    out: Optional[Sequence[Optional[torch.Tensor]]] = None) -> torch.Tensor:
     """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)), norm their ``gradient_norm``,
     which it returns (without waiting for it). In place, or into ``out``: tensors of the gradients'
-    shapes, strides and types, such as the pieces of an optimizer's buffer. None entries are skipped
+    sizes and types (and, where they are not contiguous, shapes and strides), such as the pieces of an
+    optimizer's buffer. None entries are skipped
     in both. Gradients whose norm is not finite are left (or copied) as they are. A gradient that
     occurs twice, and outputs that overlap, raise."""
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError("max_norm must not be negative or NaN")
+    grads = list(grads)
     if out is not None:
-        if len(out) != len(grads) or any((g is None) != (o is None) for g, o in zip(grads, out)):
+        out = list(out)
+        if len(out) != len(grads) or [o is None for o in out] != [g is None for g in grads]:
             raise ValueError("out must match the gradients one by one")
-        out = [o for o in out if o is not None]
-    grads = [g for g in grads if g is not None]
+        out = _without_none(out)
+    grads = _without_none(grads)
     if not grads:
         raise ValueError("no gradients")
+    checked = _tensors(grads, "gradients")
     if out is not None:
-        _tensors(out, "out")
-        for g, o in zip(grads, out):
-            if o.shape != g.shape or o.dtype != g.dtype or o.device != g.device:
-                raise ValueError(f"out must match its gradient: {tuple(g.shape)} {g.dtype} on {g.device}, "
-                                 f"got {tuple(o.shape)} {o.dtype} on {o.device}")
-            if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                raise ValueError("out must have its gradient's strides")
-    return _call(grads, max_norm, grads if out is None else out)
+        types, sizes, contiguous = _tensors(out, "out")
+        if types != checked[0] or sizes != checked[1] or out[0].device != grads[0].device:
+            raise ValueError("out must have its gradients' sizes and types, on their device")
+        if not (contiguous and checked[2]) and any(
+                (o.shape != g.shape or o.stride() != g.stride())
+                and not (o.is_contiguous() and g.is_contiguous()) for o, g in zip(out, grads)):
+            raise ValueError("out must have its gradients' strides")
+    return _call(grads, checked, max_norm, out)

@@ -43,23 +43,20 @@ def _stream(device: torch.device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *_):
-        return False
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-_HERE = _Here()
-
-
-def on_device(device: torch.device):
-    """The device as the current one for a launch (a stream belongs to its device); nothing where it
-    is current already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+def _launch(fn: str, device: torch.device, *args) -> None:
+    """Calls a C entry point with the device as the current one (a stream belongs to its device) and
+    raises for a negative status."""
+    entry = getattr(_lib.lib(), fn)
+    if device.index is None or device.index == _current_device():
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args)
+    if rc != 0:
+        _lib.check(fn, rc)
 
 
 def _need_device(t: torch.Tensor, name: str) -> None:

@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .layers import _DTYPE_CODE, QuantizedMatrix, _act_dtype, _contig, _ptr, _stream, on_device
+from .layers import _DTYPE_CODE, QuantizedMatrix, _act_dtype, _contig, _launch, _ptr, _stream
 
 
 class RMSNormResult(NamedTuple):
@@ -34,9 +34,15 @@ class RMSNormGradients(NamedTuple):
 
 def _rows(t: torch.Tensor, C: int):
     """(tensor, row stride): a matrix whose rows are contiguous is taken as it lies."""
+    if t.is_contiguous():
+        return t, C
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= C:
         return t, t.stride(0)
     return t.contiguous(), C
+
+
+def _like(x, xr):
+    return torch.empty_like(xr) if xr.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _operands(x, weight, residual, eps):
@@ -79,20 +85,18 @@ def _forward(x, weight, eps, residual, quantized):
     res, ld_r, s = None, C, x
     if residual is not None:
         res, ld_r = _rows(residual, C)
-        s = torch.empty(x.shape, dtype=dt, device=dev)
+        s = _like(x, xr)
     if quantized:
         fn = "reels_hip_rms_norm_i8"
         out = torch.empty((M, C), dtype=torch.int8, device=dev)
         per_row = torch.empty((M,), dtype=torch.float32, device=dev)
     else:
         fn = "reels_hip_rms_norm"
-        out = torch.empty(x.shape, dtype=dt, device=dev)
+        out = _like(x, xr)
         per_row = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    with on_device(dev):
-        _lib.check(fn, getattr(_lib.lib(), fn)(
-            _ptr(xr), ld_x, _ptr(res), ld_r, _ptr(weight),
-            _DTYPE_CODE[dt if weight is None else weight.dtype], _DTYPE_CODE[dt], M, C, float(eps),
-            None if res is None else _ptr(s), _ptr(out), _ptr(per_row), _stream(dev)))
+    _launch(fn, dev, _ptr(xr), ld_x, _ptr(res), ld_r, _ptr(weight),
+            _DTYPE_CODE[dt if weight is None else weight.dtype], _DTYPE_CODE[dt], M, C, eps,
+            None if res is None else s.data_ptr(), out.data_ptr(), per_row.data_ptr(), _stream(dev))
     return out, s, per_row
 
 
@@ -138,18 +142,15 @@ def rms_norm_backward(dy: torch.Tensor, s: torch.Tensor, weight: Optional[torch.
     dy, dsum, s = _contig(dy, dt, "dy"), _contig(dsum, dt, "dsum"), s.contiguous()
     rstd = _contig(rstd, torch.float32, "rstd")
     dev, M = s.device, s.numel() // C
-    dx = torch.empty(s.shape, dtype=dt, device=dev)
+    dx = torch.empty_like(s)
     dw, ws, nbytes = None, None, 0
-    L = _lib.lib()
     if want_dweight and weight is not None:
         dw = torch.empty((C,), dtype=torch.float32, device=dev)
-        nbytes = L.reels_hip_rms_norm_workspace_bytes(M, C)
+        nbytes = _lib.lib().reels_hip_rms_norm_workspace_bytes(M, C)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    with on_device(dev):
-        _lib.check("reels_hip_rms_norm_bwd", L.reels_hip_rms_norm_bwd(
-            _ptr(dy), _ptr(s), _ptr(dsum), _ptr(weight),
+    _launch("reels_hip_rms_norm_bwd", dev, _ptr(dy), _ptr(s), _ptr(dsum), _ptr(weight),
             _DTYPE_CODE[dt if weight is None else weight.dtype], _ptr(rstd), _DTYPE_CODE[dt], M, C,
-            _ptr(dx), _ptr(dw), _ptr(ws), nbytes, _stream(dev)))
+            _ptr(dx), _ptr(dw), _ptr(ws), nbytes, _stream(dev))
     return RMSNormGradients(dx, dw)
 
 

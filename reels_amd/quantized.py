@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from .layers import (_DTYPE_CODE, QuantizedMatrix, _act_dtype, _check_codes, _check_shape, _contig,
-                     _need_device, _on_activation_device, _ptr, _stream, on_device)
+                     _launch, _need_device, _on_activation_device, _ptr, _stream)
 
 _ACTIVATIONS = {None: _lib.ACT_NONE, "gelu_tanh": _lib.ACT_GELU_TANH}
 
@@ -28,10 +28,8 @@ def quantize_rows(x: torch.Tensor) -> QuantizedMatrix:
     M, K = x.shape
     values = torch.empty((M, K), dtype=torch.int8, device=x.device)
     scales = torch.empty((M,), dtype=torch.float32, device=x.device)
-    with on_device(x.device):
-        _lib.check("reels_hip_i8_pack", _lib.lib().reels_hip_i8_pack(
-            _ptr(x), _DTYPE_CODE[dt], M, K, max(x.stride(0), K), _ptr(values), _ptr(scales), None,
-            _stream(x.device)))
+    _launch("reels_hip_i8_pack", x.device, _ptr(x), _DTYPE_CODE[dt], M, K, max(x.stride(0), K),
+            _ptr(values), _ptr(scales), None, _stream(x.device))
     return QuantizedMatrix(values, scales, dt)
 
 
@@ -67,15 +65,12 @@ def quantized_linear(x: QuantizedMatrix, weight: QuantizedMatrix,
             raise ValueError(f"{n} is on {t.device}, the rows on {dev}")
     bias, residual = _contig(bias, dt, "bias"), _contig(residual, dt, "residual")
     y = torch.empty((M, N), dtype=dt, device=dev)
-    L = _lib.lib()
     px, pw = x.values.data_ptr(), weight.values.data_ptr()
     ws, nbytes = None, 0
     if K % 128 or (px | pw) & 15:  # zero-padded copies of the codes
-        nbytes = L.reels_hip_i8i8_workspace_bytes(M, K, N)
+        nbytes = _lib.lib().reels_hip_i8i8_workspace_bytes(M, K, N)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    with on_device(dev):
-        _lib.check("reels_hip_i8i8_linear", L.reels_hip_i8i8_linear(
-            px, _ptr(x.scales), pw, _ptr(weight.scales), _ptr(bias),
+    _launch("reels_hip_i8i8_linear", dev, px, _ptr(x.scales), pw, _ptr(weight.scales), _ptr(bias),
             _ptr(residual), _ACTIVATIONS[activation], _DTYPE_CODE[dt], M, K, N, _ptr(y), _ptr(ws),
-            nbytes, _stream(dev)))
+            nbytes, _stream(dev))
     return y

@@ -15,7 +15,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .layers import _DTYPE_CODE, _act_dtype, _ptr, _stream, on_device
+from .layers import _DTYPE_CODE, _act_dtype, _launch, _ptr, _stream
 
 _POS = {torch.float32: _lib.F32, torch.int32: _lib.I32}
 
@@ -35,8 +35,11 @@ def grid_positions(frames: int, height: int, width: int, device=None) -> torch.T
     return torch.stack(torch.meshgrid(t, h, w, indexing="ij"), dim=-1).reshape(-1, 3)
 
 
-@functools.lru_cache(maxsize=64)
-def _pairs(axes: Tuple[int, ...]):
+@functools.lru_cache(maxsize=256)
+def _pairs(axes: Tuple[int, ...], D: int):
+    """The C array of the axes' pairs, checked against the head dim."""
+    if not 1 <= len(axes) <= 4 or min(axes) < 0 or 2 * sum(axes) > D:
+        raise ValueError(f"axes must be one to four numbers of pairs, together at most {D // 2}, got {axes}")
     return (ctypes.c_int32 * len(axes))(*axes)
 
 
@@ -53,6 +56,10 @@ def _tokens(t: torch.Tensor):
     return t.contiguous(), H * D
 
 
+def _like(t, taken):
+    return torch.empty_like(taken) if taken.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _rotate(q, k, positions, axes, theta, interleaved, inverse):
     dt = _act_dtype(q, "q")
     if q.dim() != 4:
@@ -60,40 +67,34 @@ def _rotate(q, k, positions, axes, theta, interleaved, inverse):
     B, S, Hq, D = q.shape
     Hk = 0
     if k is not None:
-        if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D:
+        if k.dim() != 4 or k.shape != (B, S, k.shape[2], D):
             raise ValueError(f"k must be [{B}][{S}][heads][{D}], got {tuple(k.shape)}")
         if k.dtype != dt or k.device != q.device:
             raise TypeError(f"k must be {dt} on {q.device}, got {k.dtype} on {k.device}")
         Hk = k.shape[2]
     if D < 2 or D % 2 or D > 512:
         raise ValueError(f"head_dim must be even and at most 512, got {D}")
-    axes = tuple(int(n) for n in axes)
-    if not 1 <= len(axes) <= 4 or min(axes) < 0 or 2 * sum(axes) > D:
-        raise ValueError(f"axes must be one to four numbers of pairs, together at most {D // 2}, got {axes}")
-    if not (math.isfinite(theta) and theta > 0):
+    axes = tuple(axes)
+    pairs, n = _pairs(axes, D), len(axes)
+    if not 0 < theta < math.inf:
         raise ValueError("theta must be finite and positive")
     if positions.dtype not in _POS:
         raise TypeError(f"positions must be int32 or float32, got {positions.dtype}")
     if positions.device != q.device:
         raise ValueError(f"positions are on {positions.device}, q on {q.device}")
-    p = positions
-    if p.dim() == 2:
-        p = p[None]
-    if p.dim() != 3 or p.shape[0] not in (1, B) or tuple(p.shape[1:]) != (S, len(axes)):
-        raise ValueError(f"positions must be [{S}][{len(axes)}] or [{B}][{S}][{len(axes)}], got "
-                         f"{tuple(positions.shape)}")
-    p = p.contiguous()
+    ps = positions.shape
+    if not (ps == (S, n) or ps == (1, S, n) or ps == (B, S, n)):
+        raise ValueError(f"positions must be [{S}][{n}] or [{B}][{S}][{n}], got {tuple(ps)}")
+    p = positions.contiguous()
     qr, ld_q = _tokens(q)
-    yq = torch.empty(q.shape, dtype=dt, device=q.device)
+    yq = _like(q, qr)
     kr, ld_k, yk = None, 0, None
     if k is not None:
         kr, ld_k = _tokens(k)
-        yk = torch.empty(k.shape, dtype=dt, device=q.device)
-    with on_device(q.device):
-        _lib.check("reels_hip_rotary", _lib.lib().reels_hip_rotary(
-            _ptr(qr), ld_q, _ptr(kr), ld_k, _ptr(p), _POS[p.dtype], p.shape[0], _DTYPE_CODE[dt], B,
-            S, Hq, Hk, D, _pairs(axes), len(axes), float(theta), int(bool(interleaved)), inverse,
-            _ptr(yq), _ptr(yk), _stream(q.device)))
+        yk = _like(k, kr)
+    _launch("reels_hip_rotary", q.device, _ptr(qr), ld_q, _ptr(kr), ld_k, _ptr(p), _POS[p.dtype],
+            1 if len(ps) == 2 else ps[0], _DTYPE_CODE[dt], B, S, Hq, Hk, D, pairs, n, theta,
+            int(bool(interleaved)), inverse, _ptr(yq), _ptr(yk), _stream(q.device))
     return yq, yk
 
 

@@ -175,6 +175,27 @@ def test_values_outside_the_ordinary(dev, C):
     assert torch.isnan(q.output.scales).all()
 
 
+@pytest.mark.parametrize("C", [40, 3000, 40000])
+def test_quantized_with_wide_weights(dev, C):
+    """Weights and rows whose products pass the f32 range on either side still give the codes of the
+    64-bit quotients."""
+    g = torch.Generator(device=dev).manual_seed(C)
+    x = torch.randn(6, C, generator=g, device=dev)
+    x[1] *= 1e-36
+    x[2] *= 1e30
+    x[3] *= 10.0 ** torch.randint(-30, 1, (C,), generator=g, device=dev).float()
+    for w in (torch.full((C,), 3e25, device=dev), 10.0 ** torch.randint(-30, 31, (C,), generator=g, device=dev).float(),
+              torch.full((C,), 1e-25, device=dev)):
+        for eps in (0.0, 1e-6):
+            q = rms_norm_quantized(x, w, eps).output
+            p = x.double() * w.double()
+            top = p.abs().amax(-1, keepdim=True)
+            rstd = 1.0 / torch.sqrt(x.double().square().mean(-1) + float(torch.tensor(eps)))
+            fits = (top[:, 0] * rstd / 127).float().isfinite()
+            assert torch.equal(q.values[fits].double(), torch.round(127.0 * p / top)[fits])
+            assert torch.isnan(q.scales[~fits]).all() and torch.isfinite(q.scales[fits]).all()
+
+
 def test_ties_go_to_even(dev):
     # 127 p / top is a half exactly where p is half the row's largest
     x = torch.tensor([[2.0, 1.0, -1.0, 0.5, 2.0, -2.0, 0.0, 0.0]], device=dev, dtype=torch.bfloat16)
