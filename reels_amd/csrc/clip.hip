@@ -6,7 +6,7 @@
 // Bound by memory: the gradients are read for the norm and again for the scaled copy, which needs
 // the finished norm. The tensors (their pointers, sizes and types) travel in kernel arguments to a
 // table in the workspace, 96 at a time, so a call records into a graph and the host keeps nothing.
-// The work is cut into pieces of 16384 elements; every workgroup takes a run of consecutive pieces.
+// The work is cut into pieces of 16384 elements, dealt to the workgroups in turn.
 // Squares are summed in 64 bits, one partial per workgroup, and every workgroup of the second pass
 // adds the partials in the same order: the result does not depend on the run.
 #include "vec.h"
@@ -40,16 +40,33 @@ __global__ __launch_bounds__(128) void grad_table_kernel(Batch b, Entry* table, 
 __device__ __forceinline__ int64_t entry_size(const Entry& e) { return e.n >> 2; }
 __device__ __forceinline__ int entry_type(const Entry& e) { return (int)(e.n & 3); }
 
-// index of the tensor that holds a piece
-__device__ __forceinline__ int find_entry(const Entry* table, int count, int64_t piece) {
-  int lo = 0, hi = count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (table[mid].first <= piece) lo = mid;
-    else hi = mid - 1;
+// Index of the tensor that holds a piece: in LDS, where a workgroup keeps the tensors' first pieces if
+// they fit, else in the table
+constexpr int kCached = 1024;
+struct Finder {
+  const Entry* table;
+  int64_t* cache;
+  int count;
+  __device__ __forceinline__ Finder(const Entry* t, int n, int64_t* c) : table(t), cache(c), count(n) {
+    if (n > kCached) return;
+    for (int i = threadIdx.x; i < n; i += kThreads) c[i] = t[i].first;
+    __syncthreads();
   }
-  return lo;
-}
+  template <typename F> __device__ __forceinline__ int search(int64_t piece, F&& first) const {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first(mid) <= piece) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+  __device__ __forceinline__ int find(int64_t piece) const {
+    const Entry* t = table;
+    const int64_t* c = cache;
+    return count <= kCached ? search(piece, [c](int i) { return c[i]; }) : search(piece, [t](int i) { return t[i].first; });
+  }
+};
 
 __device__ __forceinline__ double block_sum(double v, double* slot) {
   v = group_reduce<64, false>(v);
@@ -61,36 +78,56 @@ __device__ __forceinline__ double block_sum(double v, double* slot) {
   return v;
 }
 
-// f(first element, how many exist) for this thread's vectors of a piece; the whole ones four at a time,
-// so that four loads are in flight
-template <int V, typename F> __device__ __forceinline__ void each_vec(int64_t n, F&& f) {
-  const int m = (int)n, full = m / (kThreads * V);
-#pragma unroll 4
-  for (int it = 0; it < full; ++it) f((it * kThreads + (int)threadIdx.x) * V, V);
-  const int i = (full * kThreads + (int)threadIdx.x) * V;
-  if (i < m) f(i, m - i < V ? m - i : V);
+// 16 bytes at a global address at any multiple of the element: the tensors' pointers come from memory,
+// where the compiler cannot see that they are global and would take flat accesses
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef __attribute__((address_space(1))) u32x4_any* global16;
+__device__ __forceinline__ u32x4 load_global(const uint8_t* p) { return *(global16)(uintptr_t)p; }
+__device__ __forceinline__ void store_global(uint8_t* p, const u32x4& v) { *(global16)(uintptr_t)p = v; }
+
+// f(chunk, byte offset, how many exist) for this thread's chunks of a piece of n elements, eight loads in flight
+template <int ELT, typename F> __device__ __forceinline__ void each_chunk(const uint8_t* g, int n, F&& f) {
+  constexpr int V = Chunk<ELT>::V, U = 8, STEP = kThreads * 16;
+  const int full = n / (kThreads * V);
+  int it = 0, at = (int)threadIdx.x * 16;
+  for (; it + U <= full; it += U, at += U * STEP) {
+    Chunk<ELT> c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) c[u].d = load_global(g + at + u * STEP);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(c[u], at + u * STEP, V);
+  }
+  for (; it < full; ++it, at += STEP) {
+    Chunk<ELT> c;
+    c.d = load_global(g + at);
+    f(c, at, V);
+  }
+  const int left = n - at / elt_bytes(ELT);
+  if (left <= 0) return;
+  Chunk<ELT> c;
+  c.load(g + at, left < V ? left : V);
+  f(c, at, left < V ? left : V);
 }
 
-template <int ELT> __device__ __forceinline__ double piece_sum(const void* g, int64_t n) {
-  constexpr int V = 16 / elt_bytes(ELT);
+template <int ELT> __device__ __forceinline__ double piece_sum(const uint8_t* g, int n) {
   double t = 0.0;
-  each_vec<V>(n, [&](int i, int left) {
-    float f[V];
-    load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), left, f);
+  each_chunk<ELT>(g, n, [&](const Chunk<ELT>& c, int, int) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) t = fma((double)f[j], (double)f[j], t);
+    for (int j = 0; j < Chunk<ELT>::V; ++j) t = fma((double)c.get(j), (double)c.get(j), t);
   });
   return t;
 }
 
-template <int ELT> __device__ __forceinline__ void piece_scale(const void* g, void* o, int64_t n, float factor) {
-  constexpr int V = 16 / elt_bytes(ELT);
-  each_vec<V>(n, [&](int i, int left) {
+template <int ELT> __device__ __forceinline__ void piece_scale(const uint8_t* g, uint8_t* o, int n, float factor) {
+  constexpr int V = Chunk<ELT>::V;
+  each_chunk<ELT>(g, n, [&](const Chunk<ELT>& c, int at, int left) {
     float f[V];
-    load_vec<ELT, V>((const uint8_t*)g + i * elt_bytes(ELT), left, f);
+    Chunk<ELT> d;
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] *= factor;
-    store_vec<ELT, V>((uint8_t*)o + i * elt_bytes(ELT), left, f);
+    for (int j = 0; j < V; ++j) f[j] = c.get(j) * factor;
+    d.pack(f);
+    if (left == V) store_global(o + at, d.d);
+    else d.store(o + at, left);
   });
 }
 
@@ -100,26 +137,28 @@ template <typename F> __device__ __forceinline__ void with_type(int t, F&& f) {
   else f(std::integral_constant<int, REELS_HIP_BF16>{});
 }
 
-// f(entry, element offset, elements) for every piece of this workgroup
-template <typename F> __device__ __forceinline__ void each_piece(const Entry* table, int count, int64_t pieces, F&& f) {
-  const int64_t p0 = pieces * blockIdx.x / gridDim.x, p1 = pieces * (blockIdx.x + 1) / gridDim.x;
-  if (p0 >= p1) return;
-  int at = find_entry(table, count, p0);
-  for (int64_t p = p0; p < p1; ++p) {
-    while (at + 1 < count && table[at + 1].first <= p) ++at;
-    const Entry e = table[at];
-    const int64_t off = (p - e.first) * kPiece, n = entry_size(e) - off;
-    f(e, off, n < kPiece ? n : kPiece);
+// f(entry, element offset, elements) for every piece of this workgroup: neighbouring workgroups take
+// neighbouring pieces (each its own run of pieces put all of them on the same memory channels at a
+// time: 524 MB summed in 131 us). The second pass goes backwards, from what the first has left in cache.
+template <bool BACK, typename F> __device__ __forceinline__ void each_piece(const Finder& at, int64_t pieces, F&& f) {
+  const int64_t n = (pieces - blockIdx.x + gridDim.x - 1) / gridDim.x;
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t p = blockIdx.x + (BACK ? n - 1 - i : i) * gridDim.x;
+    const Entry e = at.table[at.find(p)];
+    const int64_t off = (p - e.first) * kPiece, left = entry_size(e) - off;
+    f(e, off, left < kPiece ? left : kPiece);
   }
 }
 
 __global__ __launch_bounds__(kThreads) void grad_sum_kernel(const Entry* table, int count, int64_t pieces, double* part) {
   __shared__ double slot[kThreads / 64];
+  __shared__ int64_t cache[kCached];
+  const Finder at(table, count, cache);
   double t = 0.0;
-  each_piece(table, count, pieces, [&](const Entry& e, int64_t off, int64_t n) {
+  each_piece<false>(at, pieces, [&](const Entry& e, int64_t off, int64_t n) {
     with_type(entry_type(e), [&](auto ty) {
       constexpr int E = decltype(ty)::value;
-      t += piece_sum<E>((const uint8_t*)e.g + off * elt_bytes(E), n);
+      t += piece_sum<E>((const uint8_t*)e.g + off * elt_bytes(E), (int)n);
     });
   });
   t = block_sum(t, slot);
@@ -141,17 +180,19 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const double* part,
 __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const Entry* table, int count, int64_t pieces,
                                                               const double* part, int n, float max_norm, float* norm) {
   __shared__ double slot[kThreads / 64];
+  __shared__ int64_t cache[kCached];
+  const Finder at(table, count, cache);
   const double t = total_norm(part, n, slot);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)t;
   // gradients whose norm is not finite are left as they are: a factor of 0 or NaN would hide which
   // of them it came from
   const double f = (double)max_norm / (t + 1e-6);
   const float factor = __builtin_isfinite(t) && f < 1.0 ? (float)f : 1.0f;
-  each_piece(table, count, pieces, [&](const Entry& e, int64_t off, int64_t m) {
+  each_piece<true>(at, pieces, [&](const Entry& e, int64_t off, int64_t m) {
     if (factor == 1.0f && e.g == e.o) return;  // in place and nothing to clip
     with_type(entry_type(e), [&](auto ty) {
       constexpr int E = decltype(ty)::value;
-      piece_scale<E>((const uint8_t*)e.g + off * elt_bytes(E), (uint8_t*)e.o + off * elt_bytes(E), m, factor);
+      piece_scale<E>((const uint8_t*)e.g + off * elt_bytes(E), (uint8_t*)e.o + off * elt_bytes(E), (int)m, factor);
     });
   });
 }
