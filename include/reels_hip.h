@@ -393,7 +393,7 @@ int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void* dsum, cons
  * The sums are exact whole numbers (K < 131072), the rest runs in f32 and rounds once, so a row of
  * y does not depend on M nor on its place. Any alignment. workspace:
  * reels_hip_i8i8_workspace_bytes(M, K, N) bytes (0 for up to 16 tokens), for zero-padded copies of
- * the codes; not used, and may be NULL, where K is a multiple of 128 and x and w are 16-byte aligned.
+ * the codes; not used, and may be NULL, where K is a multiple of 4 and x and w are 4-byte aligned.
  */
 size_t reels_hip_i8i8_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int reels_hip_i8i8_linear(const int8_t* x, const float* xs, const int8_t* w, const float* ws,

@@ -201,6 +201,18 @@ size_t table_bytes(int64_t count) { return align_up((size_t)count * sizeof(Entry
 
 // two ranges overlap, one of them an output, unless they are a tensor and its own output
 bool outputs_overlap(const void* const* g, void* const* o, const int64_t* n, const int32_t* ty, int64_t count) {
+  // outputs that follow each other in memory (pieces of one buffer), every gradient outside them: no sort
+  uintptr_t lo = 0, hi = 0;
+  bool rising = true;
+  for (int64_t i = 0; i < count && rising; ++i) {
+    if (n[i] == 0) continue;
+    rising = (uintptr_t)o[i] >= hi;
+    if (lo == 0) lo = (uintptr_t)o[i];
+    hi = (uintptr_t)o[i] + (uintptr_t)n[i] * elt_bytes(ty[i]);
+  }
+  for (int64_t i = 0; i < count && rising; ++i)
+    rising = n[i] == 0 || g[i] == o[i] || (uintptr_t)g[i] >= hi || (uintptr_t)g[i] + (uintptr_t)n[i] * elt_bytes(ty[i]) <= lo;
+  if (rising) return false;
   struct Span { uintptr_t a, b; bool out; };
   std::vector<Span> v;
   v.reserve((size_t)count * 2);

@@ -34,11 +34,32 @@ struct ProductArgs {
 // read stage kt, so the weight copy of step kt + 2 goes into it right away, and the activation copy
 // of step kt + 2 into the stage of step kt - 1 already during the first half of step kt. Per step a
 // wave reads TJ + 4 fragments for 4 TJ MFMAs, twice. Rows past the edges read as zeros (the buffer's
-// bounds); K is a multiple of 128 here, other K run on zero-padded copies.
+// bounds). K and the rows' addresses are multiples of 4 here, which the copies need; others run on
+// padded copies.
 template <int TJ> struct Tile {
   static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 128;
   static constexpr int ACT = BM * BK, WB = BN * BK, LDS = 3 * ACT + 2 * WB;
 };
+
+// Zeros for the activations' bytes from `keep` on in a tile of 128-byte rows: where K is no multiple of
+// 128 the last step's rows end in the next row's codes, and zeros on one side take them out of the sum
+template <int ROWS, int NT> __device__ __forceinline__ void clear_tail(uint8_t* tile, int keep) {
+  for (int i = threadIdx.x; i < ROWS * 8; i += NT) {
+    const int row = i >> 3, c = i & 7, lo = keep - c * 16;  // lo: bytes of chunk c that stay
+    if (lo >= 16) continue;
+    i32v4* p = reinterpret_cast<i32v4*>(tile + row * 128 + ((c ^ (row & 7)) << 4));
+    i32v4 v = *p;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int b = lo - 4 * q;
+      v[q] = b >= 4 ? v[q] : b <= 0 ? 0 : v[q] & ((1 << (8 * b)) - 1);
+    }
+    *p = v;
+  }
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 template <int ELT, int TJ>
 __global__ __launch_bounds__(Tile<TJ>::NT) void product_tile_kernel(ProductArgs a, int tiles_n, int tiles_m) {
@@ -54,7 +75,7 @@ __global__ __launch_bounds__(Tile<TJ>::NT) void product_tile_kernel(ProductArgs 
   const int group = 4 * tiles_n, g = logical / group, first = g * 4;
   const int gm = tiles_m - first < 4 ? tiles_m - first : 4, within = logical - g * group;
   const int64_t m0 = (int64_t)(first + within % gm) * T::BM, n0 = (int64_t)(within / gm) * T::BN;
-  const int nk = (int)(a.K / T::BK), K = (int)a.K;
+  const int K = (int)a.K, nk = (K + T::BK - 1) / T::BK, tail = K % T::BK;
   const int rows = (int)(a.M - m0 < T::BM ? a.M - m0 : T::BM), cols = (int)(a.N - n0 < T::BN ? a.N - n0 : T::BN);
   const i32x4 rx = buffer_rsrc(a.x + m0 * a.K, (uint32_t)rows * K), rw = buffer_rsrc(a.w + n0 * a.K, (uint32_t)cols * K);
   const i32x4 rnone = buffer_rsrc(a.x, 0u);  // zero records: a copy through it reads nothing
@@ -97,6 +118,7 @@ __global__ __launch_bounds__(Tile<TJ>::NT) void product_tile_kernel(ProductArgs 
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
+  if (nk == 1 && tail != 0) clear_tail<T::BM, T::NT>(abase(0), tail);
   read_w(wbase(0), 0, w0);
 #pragma unroll
   for (int j = 0; j < TJ; ++j) x[j] = read_x(abase(0), 0, j);
@@ -128,6 +150,9 @@ __global__ __launch_bounds__(Tile<TJ>::NT) void product_tile_kernel(ProductArgs 
     __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4): step kt + 1 has landed
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    if constexpr (LAST) {
+      if (tail != 0) clear_tail<T::BM, T::NT>(abase(kt + 1), tail);
+    }
     if (TJ == 8 && w >= 4) __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
     const uint8_t* san = abase(kt + 1);
@@ -269,7 +294,7 @@ __global__ __launch_bounds__(small::NT) void product_small_kernel(ProductArgs a,
   const int xcd = blockIdx.x & 7, nt = gridDim.x;
   const int logical = xcd * (nt >> 3) + (xcd < (nt & 7) ? xcd : nt & 7) + (blockIdx.x >> 3);
   const int64_t m0 = (int64_t)(logical % tiles_m) * BT, n0 = (int64_t)(logical / tiles_m) * BT;
-  const int K = (int)a.K, nk = K / BK;
+  const int K = (int)a.K, nk = (K + BK - 1) / BK, tail = K % BK;
   const int rows = (int)(a.M - m0 < BT ? a.M - m0 : BT), cols = (int)(a.N - n0 < BT ? a.N - n0 : BT);
   const i32x4 rx = buffer_rsrc(a.x + m0 * a.K, (uint32_t)rows * K), rw = buffer_rsrc(a.w + n0 * a.K, (uint32_t)cols * K);
   const int crow = w * 8 + (lane >> 3);  // a wave copies rows 8 w .. 8 w + 7 of each tile
@@ -291,6 +316,7 @@ __global__ __launch_bounds__(small::NT) void product_small_kernel(ProductArgs a,
     __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4): step kt has landed, the two after it may fly
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    if (kt == nk - 1 && tail != 0) clear_tail<BT, NT>(smem + (kt & (RING - 1)) * STAGE, tail);
     const uint8_t* s = smem + (kt & (RING - 1)) * STAGE + l16 * 128 + off;
     i32v4 xf[2], wf[2];
 #pragma unroll
@@ -339,10 +365,16 @@ __global__ __launch_bounds__(small::NT) void product_small_kernel(ProductArgs a,
 // waves are within 4% of that at one token of 5120, 2 to 14% slower at 13824 outputs.
 constexpr int kFewTokens = 16, kFewWaves = 8, kFewUnroll = 4;
 
-// 16 codes at p, the first `left` of which exist
-__device__ __forceinline__ i32v4 load_codes(const int8_t* p, int left) {
+// 16 codes at p, the first `left` of which belong to its row of K, zeros for the others: a part of 16
+// is the row's last 16 codes shifted down (a loop over bytes waits for each)
+__device__ __forceinline__ i32v4 load_codes(const int8_t* p, int left, int K) {
   if (left >= 16) return load_any<i32v4>(p);
   i32v4 v = {0, 0, 0, 0};
+  if (left <= 0) return v;
+  if (K >= 16) {
+    const unsigned __int128 u = load_any<unsigned __int128>(p + left - 16) >> (8 * (16 - left));
+    return __builtin_bit_cast(i32v4, u);
+  }
   for (int b = 0; b < left; ++b) {
     const int byte = (int)((uint32_t)(uint8_t)p[b] << (8 * (b % 4)));
 #pragma unroll
@@ -379,8 +411,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(ProductArgs
   // what is left of K in pieces of 64, codes past it as zeros
   const int piece = (lines * 2 + w) * 64;
   if (w < 2 && piece < K)
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_codes(wr + piece, (int)K - piece - lq * 16),
-                                                load_codes(xr + piece, (int)K - piece - lq * 16), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_codes(wr + piece, (int)K - piece - lq * 16, (int)K),
+                                                load_codes(xr + piece, (int)K - piece - lq * 16, (int)K), acc, 0, 0, 0);
   part[w][lane] = acc;
   __syncthreads();
   if (w > 0) return;
@@ -428,8 +460,8 @@ __global__ __launch_bounds__(64) void product_dot_kernel(ProductArgs a) {
   i32v4 wf[U], xf[U];  // fewer than U KiB are left, the last piece of a lane perhaps in part
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    wf[u] = load_codes(wr + k + u * 1024, K - k - u * 1024);
-    xf[u] = load_codes(a.x + k + u * 1024, K - k - u * 1024);
+    wf[u] = load_codes(wr + k + u * 1024, K - k - u * 1024, K);
+    xf[u] = load_codes(a.x + k + u * 1024, K - k - u * 1024, K);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) dot(wf[u], xf[u]);
@@ -468,7 +500,7 @@ __global__ __launch_bounds__(256) void product_pad_kernel(const int8_t* __restri
     const int64_t r = second ? i - r0 : i;
     const int8_t* src = (second ? w : x) + r * K;
     int8_t* dst = (second ? pw : px) + r * Kp;
-    for (int c = (threadIdx.x & 63) * 16; c < Kp; c += 1024) *reinterpret_cast<i32v4*>(dst + c) = load_codes(src + c, K - c);
+    for (int c = (threadIdx.x & 63) * 16; c < Kp; c += 1024) *reinterpret_cast<i32v4*>(dst + c) = load_codes(src + c, K - c, K);
   }
 }
 
@@ -493,7 +525,8 @@ template <int TJ> int launch_tiles(const ProductArgs& a, int dtype, hipStream_t 
   return check_launch("product_tile_kernel");
 }
 
-bool whole_rows(const void* x, const void* w, int64_t K) { return K % 128 == 0 && aligned16(x) && aligned16(w); }
+// rows that the copies to LDS can take as they lie
+bool whole_rows(const void* x, const void* w, int64_t K) { return K % 4 == 0 && ((uintptr_t)x & 3) == 0 && ((uintptr_t)w & 3) == 0; }
 
 // The tiled form with the least estimated time, in microseconds. A workgroup's step of 128 codes
 // takes about as long whatever the size: 64 x 64 tiles 0.27 us with one workgroup on a CU and 0.55
@@ -503,7 +536,7 @@ bool whole_rows(const void* x, const void* w, int64_t K) { return K % 128 == 0 &
 // 10240 47.8 / 38.9 / 48.3, 1560 x 1536 -> 8960 44.8 / 33.9 / 27.4, 2048 x 5120 -> 5120 119 / 70.0 /
 // 53.7, 32760 x 5120 -> 5120 - / 928 / 670.
 int tile_of(int64_t M, int64_t N, int64_t K) {
-  const double steps = (double)(K / 128);
+  const double steps = (double)ceil_div(K, 128);
   auto two = [](int64_t blocks, double one, double both) {  // two workgroups fit a CU
     const int64_t full = blocks / 512, rest = blocks % 512;
     return (double)full * both + (rest == 0 ? 0.0 : rest <= 256 ? one : both);

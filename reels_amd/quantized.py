@@ -67,7 +67,7 @@ def quantized_linear(x: QuantizedMatrix, weight: QuantizedMatrix,
     y = torch.empty((M, N), dtype=dt, device=dev)
     px, pw = x.values.data_ptr(), weight.values.data_ptr()
     ws, nbytes = None, 0
-    if K % 128 or (px | pw) & 15:  # zero-padded copies of the codes
+    if (K | px | pw) & 3:  # zero-padded copies of the codes
         nbytes = _lib.lib().reels_hip_i8i8_workspace_bytes(M, K, N)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     _launch("reels_hip_i8i8_linear", dev, px, _ptr(x.scales), pw, _ptr(weight.scales), _ptr(bias),

@@ -59,7 +59,7 @@ def test_product_c_refusals():
     assert prod(dt=3) == -2
     assert prod(act=2) == -1 and "activation" in _err()
     assert prod(M=-1) == -1 and prod(K=0) == -1 and prod(N=0) == -1 and prod(K=1 << 17) == -1
-    assert prod(work=None) == -3 and prod(n=0) == -3
+    assert prod(work=None, K=63) == -3 and prod(n=0, K=63) == -3
     for name in ("x", "xs", "w", "ws", "y"):
         assert prod(**{name: None}) == -1 and "NULL" in _err()
     assert prod(M=0, x=None, y=None) == 0
