@@ -13,8 +13,9 @@
 // All of it is bound by memory: each kernel reads its operands once and keeps the row in registers
 // between the reduction and the output. A row belongs to a group of TPR threads that hold NCH
 // 16-byte chunks each: TPR is the smallest of 16, 64 and 256 whose threads need at most four
-// chunks, or 1024 with two, so short rows (one head) share a wave and long ones have many loads in
-// flight; rows past 2048 chunks (16384 16-bit elements) run the loop form, which reads them again from L2. Squares
+// chunks, or 512 (f32: or 1024) with three or four, so short rows (one head) share a wave and long
+// ones have many loads in flight; rows past 16384 elements run the loop form, which reads them again
+// from L2. Squares
 // and products are summed in 64 bits (MI355X adds those at the rate of 32-bit ones), so rows of any
 // magnitude that the type holds have the norm that they should.
 #include "vec.h"
@@ -159,9 +160,10 @@ template <int V> __device__ __forceinline__ void store_codes(int8_t* q, int left
   }
 }
 
-// Where a thread's chunks of a row lie: chunk i at element col(i). Whole chunks are read without a
-// branch, from the row's first chunk where there is none (and zeroed), so that all loads of a row are
-// in flight together; the one partial chunk of a row whose length is no multiple of V, by elements.
+// Where a thread's chunks of a row lie: chunk i at element col(i). Chunks are read without a branch, so
+// that all loads of a row are in flight together: a thread without a chunk reads the row's first one
+// (and zeroes it), and where the row's length is no multiple of V its last V elements stand for the
+// partial chunk, shifted down. Rows shorter than V are read by elements.
 template <int ELT, int TPR, int NCH> struct Row {
   static constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
   int cols, lane, base;
@@ -178,21 +180,30 @@ template <int ELT, int TPR, int NCH> struct Row {
   __device__ __forceinline__ int left(int i) const { return cols - col(i); }
   template <int E> __device__ __forceinline__ void load(const void* row, Chunk<E> (&d)[NCH]) const {
     const uint8_t* p = (const uint8_t*)row;
-    if (cols >= V) {
+    if (cols < V) {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
-        if (some(i)) d[i].d = load_any<u32x4>((const typename Store<E>::raw*)(p + (int64_t)(full(i) ? col(i) : 0) * EB));
+      for (int i = 0; i < NCH; ++i) {
+        d[i].zero();
+        if (part(i)) d[i].load(p + (int64_t)col(i) * EB, left(i));
+      }
+      return;
     }
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
-      if (!some(i) || !full(i)) d[i].zero();
+    for (int i = 0; i < NCH; ++i) {
+      const int at = full(i) ? col(i) : part(i) ? cols - V : 0;
+      if (some(i)) d[i].d = load_any<u32x4>((const typename Store<E>::raw*)(p + (int64_t)at * EB));
+    }
     if (cols % V != 0) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
-        if (part(i)) d[i].load(p + (int64_t)col(i) * EB, left(i));
+        if (some(i) && part(i))
+          d[i].d = __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, d[i].d) >> (8 * EB * (V - left(i))));
     }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+      if (!some(i) || !(full(i) || part(i))) d[i].zero();
   }
-  // weights as f32, ones without any; f32 ones of a 16-bit row take two vectors a chunk
+  // weights as f32, ones without any, by the same places
   __device__ __forceinline__ void load_w(const void* w, int w_f32, float (&f)[NCH][V]) const {
     if (w == nullptr) {
 #pragma unroll
@@ -201,21 +212,31 @@ template <int ELT, int TPR, int NCH> struct Row {
         for (int j = 0; j < V; ++j) f[i][j] = 1.0f;
       return;
     }
-    if (cols >= V) {
-      if (w_f32) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-          if (some(i)) load_vec<REELS_HIP_F32, V>((const float*)w + (full(i) ? col(i) : 0), V, f[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-          if (some(i)) load_vec<ELT, V>((const uint8_t*)w + (int64_t)(full(i) ? col(i) : 0) * EB, V, f[i]);
-      }
-    }
-    if (cols % V != 0) {
+    if (cols < V) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
         if (part(i)) load_weight<ELT, V>(w, w_f32, col(i), left(i), f[i]);
+      return;
+    }
+    if (w_f32) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (some(i)) load_vec<REELS_HIP_F32, V>((const float*)w + (full(i) ? col(i) : part(i) ? cols - V : 0), V, f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (some(i)) load_vec<ELT, V>((const uint8_t*)w + (int64_t)(full(i) ? col(i) : part(i) ? cols - V : 0) * EB, V, f[i]);
+    }
+    if (cols % V != 0) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        if (!some(i)) continue;
+        const int by = part(i) ? V - left(i) : 0;  // down by so many elements, in steps of 4, 2 and 1
+#pragma unroll
+        for (int sh = V / 2; sh > 0; sh /= 2)
+#pragma unroll
+          for (int j = 0; j < V; ++j) f[i][j] = (by & sh) ? (j + sh < V ? f[i][j + sh] : 0.0f) : f[i][j];
+      }
     }
   }
   __device__ __forceinline__ void store(void* row, int i, const Chunk<ELT>& d) const {
@@ -413,8 +434,14 @@ struct NormBwdArgs {
 // A workgroup walks the rows b, b + gridDim, ... (times the rows it holds at once): with dw each
 // thread keeps the sums of its own columns in registers over all its rows, and the groups of a
 // workgroup add theirs in LDS in group order, one partial row per workgroup.
+// Waves a SIMD has to hold, by the registers that a row's three operands, weights and sums of dw take
+constexpr int bwd_waves(int tpr, int nch, bool dw) {
+  if (tpr == 1024) return 4;
+  return dw ? (nch == 1 ? 7 : nch == 2 ? 4 : nch == 3 ? 3 : 2) : (nch == 1 ? 7 : nch == 2 ? 5 : nch == 3 ? 4 : 3);
+}
+
 template <int ELT, int TPR, int NCH, bool DW>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd_kernel(NormBwdArgs a) {
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, bwd_waves(TPR, NCH, DW)) void norm_bwd_kernel(NormBwdArgs a) {
   constexpr int V = 16 / elt_bytes(ELT), EB = elt_bytes(ELT), NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
   __shared__ double slots[2][NT / 64];
   __shared__ float acc[DW && RPB > 1 ? RPB * TPR * NCH * V : 1];
@@ -577,12 +604,13 @@ Form norm_form(int elt, int64_t cols) {
   const int64_t chunks = ceil_div(cols, 16 / elt_bytes(elt));
   for (int tpr : {16, 64, 256})
     if (chunks <= 4 * tpr) return {tpr, (int)ceil_div(chunks, tpr)};
-  if (chunks <= 2048) return {1024, 2};
+  if (chunks <= 2048) return {512, chunks <= 1536 ? 3 : 4};
+  if (elt == REELS_HIP_F32 && chunks <= 4096) return {1024, chunks <= 3072 ? 3 : 4};  // half the values a chunk
   return {0, 0};
 }
 
 template <int N> using Int = std::integral_constant<int, N>;
-template <typename F> void with_form(Form f, F&& g) {
+template <int ELT, typename F> void with_form(Form f, F&& g) {
   auto nch = [&](auto tpr) {
     switch (f.nch) {
       case 1: g(tpr, Int<1>{}); break;
@@ -595,7 +623,16 @@ template <typename F> void with_form(Form f, F&& g) {
     case 16: nch(Int<16>{}); break;
     case 64: nch(Int<64>{}); break;
     case 256: nch(Int<256>{}); break;
-    default: g(Int<1024>{}, Int<2>{}); break;
+    case 512:
+      if (f.nch == 3) g(Int<512>{}, Int<3>{});
+      else g(Int<512>{}, Int<4>{});
+      break;
+    default:
+      if constexpr (ELT == REELS_HIP_F32) {
+        if (f.nch == 3) g(Int<1024>{}, Int<3>{});
+        else g(Int<1024>{}, Int<4>{});
+      }
+      break;
   }
 }
 
@@ -627,7 +664,7 @@ int norm_forward(const char* fn, const char* label, bool quant, NormArgs a, int 
         else norm_long_kernel<E, false><<<(unsigned)a.rows, kLongThreads, 0, st>>>(a);
         return;
       }
-      with_form(f, [&](auto tpr, auto nch) {
+      with_form<E>(f, [&](auto tpr, auto nch) {
         constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = T < 256 ? 256 : T;
         const unsigned grid = (unsigned)ceil_div(a.rows, NT / T);
         if (!quant) norm_kernel<E, T, C, 0><<<grid, NT, 0, st>>>(a);
@@ -638,11 +675,14 @@ int norm_forward(const char* fn, const char* label, bool quant, NormArgs a, int 
   return check_launch(label);
 }
 
-// workgroups of the backward with dw (each writes one partial row): enough to fill the GPU, and at
-// least two rows for each group of threads, so that the partial rows stay a small part of the traffic
-int64_t norm_parts(int64_t rows, Form f) {
+// Workgroups of the backward with dw (each writes one partial row): as many as the GPU holds at once by
+// their registers (1024 where 768 fit cost a second round: 32760 x 5120 380 -> 261 us), and at least two
+// rows for each group of threads, so that the partial rows stay a small part of the traffic
+int64_t norm_parts(int64_t rows, int elt, Form f) {
   const int64_t rpb = f.tpr == 0 ? 1 : (f.tpr < 256 ? 256 / f.tpr : 1);
-  const int64_t want = f.tpr == 0 ? 64 : (f.tpr <= 256 ? 1024 : 256), need = ceil_div(rows, 2 * rpb);
+  const int values = f.nch * 16 / elt_bytes(elt);  // of a thread
+  const int64_t want = f.tpr == 0 ? 64 : f.tpr >= 512 ? 256 : values >= 24 ? 768 : elt == REELS_HIP_F32 || values >= 16 || f.tpr == 256 ? 1024 : 1792;
+  const int64_t need = ceil_div(rows, 2 * rpb);
   return need < want ? need : want;
 }
 
@@ -673,7 +713,7 @@ extern "C" size_t reels_hip_rms_norm_workspace_bytes(int64_t rows, int64_t cols)
   // the most partial rows of any element type
   int64_t n = 1;
   for (int elt : {REELS_HIP_F32, REELS_HIP_BF16}) {
-    const int64_t p = norm_parts(rows, norm_form(elt, cols));
+    const int64_t p = norm_parts(rows, elt, norm_form(elt, cols));
     n = p > n ? p : n;
   }
   return align_up((size_t)n * (size_t)cols * 4, 256);
@@ -694,7 +734,7 @@ extern "C" int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void*
   if (rows == 0 && dw == nullptr) return REELS_HIP_OK;
   NormBwdArgs a{dy, s, dsum, weight, rstd, dx, (float*)workspace, rows, cols, 1.0 / (double)cols, w_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32};
   const Form f = norm_form(dtype, cols);
-  const int64_t parts = rows == 0 ? 0 : norm_parts(rows, f);
+  const int64_t parts = rows == 0 ? 0 : norm_parts(rows, dtype, f);
   if (rows > 0) {
     TraceScope _ts(st, "norm_bwd_kernel");
     with_any_elt(dtype, [&](auto e) {
@@ -704,7 +744,7 @@ extern "C" int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void*
         if (dw != nullptr) norm_dw_long_kernel<E><<<dim3((unsigned)ceil_div(cols, 256), (unsigned)parts), 256, 0, st>>>(a);
         return;
       }
-      with_form(f, [&](auto tpr, auto nch) {
+      with_form<E>(f, [&](auto tpr, auto nch) {
         constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = T < 256 ? 256 : T;
         if (dw != nullptr) norm_bwd_kernel<E, T, C, true><<<(unsigned)parts, NT, 0, st>>>(a);
         else norm_bwd_kernel<E, T, C, false><<<(unsigned)ceil_div(rows, NT / T), NT, 0, st>>>(a);
