@@ -44,7 +44,8 @@ __device__ __forceinline__ float gelu_logistic(float x) {
 // of step kt + 2 into the stage of step kt - 1 already during the first half of step kt. Per step a
 // wave reads TJ + 4 fragments for 4 TJ MFMAs, twice. Rows past the edges read as zeros (the buffer's
 // bounds). K and the rows' addresses are multiples of 4 here, which the copies need; others run on
-// padded copies.
+// padded copies. Bound by the matrix cores at the power cap: 32760 x 13824 -> 5120 1.66 ms (2.79 POP/s;
+// the vendor's int8 product 2.49 on this size), with bias and residual 1.72.
 template <int TJ> struct Tile {
   static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 128;
   static constexpr int ACT = BM * BK, WB = BN * BK, LDS = 3 * ACT + 2 * WB;
@@ -450,9 +451,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(ProductArgs
 // A wave takes one output over the whole K: each lane multiplies 16 codes of every KiB with v_dot4,
 // so the weight streams in whole lines and its rows spread evenly over the CUs, where the 16-row
 // tiles above leave some CUs twice the work of others. Taken at K of 4096 and more, where it has
-// several loads in flight: 1 x 13824 -> 5120 20.5 -> 15.4 us (4.6 TB/s), 5120 -> 13824 16.1 -> 15.1,
-// 5120 -> 5120 8.6 -> 7.7; below it loses (1536 -> 8960 5.4 -> 7.7 us). Two or four outputs a wave
-// share the activations' loads and are slower at every one of these sizes.
+// several loads in flight: 1 x 13824 -> 5120 20.5 -> 13.9 us (5.1 TB/s), 5120 -> 13824 16.1 -> 13.5,
+// 5120 -> 5120 8.6 -> 6.2; below it the two are level (1536 -> 8960 4.5 and 4.7 us). Two or four
+// outputs a wave share the activations' loads and are slower at every one of these sizes.
 constexpr int64_t kDotCodes = 4096;
 
 template <int ELT>

@@ -6,7 +6,8 @@
 //   interleaved: pair p is elements 2p, 2p + 1; else p and p + P, P the number of pairs. Elements
 //   past 2P are copied. The backward is the rotation by the negative angle (inverse).
 //
-// Bound by memory: one read and one write of q and k. A token's angles are shared by all its heads
+// Bound by memory: one read and one write of q and k (32760 tokens of 80 heads of 128 in bf16: 230 us,
+// 5.8 TB/s). A token's angles are shared by all its heads
 // and by q and k, so a workgroup computes them once for its tokens into LDS. An angle is formed in
 // turns in 64 bits (pos times the frequency over 2 pi) and only its fraction is taken to sine and
 // cosine in 32 bits, so a position of any size loses nothing to the reduction of its angle.
@@ -35,7 +36,8 @@ struct RotaryArgs {
 };
 
 // Items of a head: interleaved V elements (V/2 pairs); else V pairs (their V lower and V upper
-// elements) and after them V copied elements each
+// elements) and after them V copied elements each. One item a thread and turn: four with their loads in
+// flight before the angles take more registers and are slower (32760 x 80 heads 268 -> 293 us).
 template <int ELT, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   constexpr int EB = elt_bytes(ELT);
@@ -152,7 +154,7 @@ extern "C" int reels_hip_rotary(const void* q, int64_t ld_q, const void* k, int6
   a.S = (int)S; a.D = (int)D; a.P = (int)P; a.axes = axes; a.inverse = inverse != 0;
   a.heads[0] = (int)Hq; a.heads[1] = (int)Hk;
   // tokens of a workgroup: about 32 KiB, so that the angles are a small part of its work, but no more
-  // than leaves 2048 workgroups (1560 tokens of 6 KiB: 11.2 us in workgroups of five)
+  // than leaves 2048 workgroups (1560 tokens of 6 KiB: 11.2 us in workgroups of five, 8.2 one by one)
   const int64_t token_bytes = (Hq + Hk) * D * elt_bytes(dtype);
   int64_t tb = 32768 / token_bytes;
   if (tb > a.tokens / 2048) tb = a.tokens / 2048;

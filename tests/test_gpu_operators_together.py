@@ -1,0 +1,142 @@
+"""The operators around the linears as a program uses them together: a block's run forward and
+backward, other streams, two streams at once, tensors whose offsets pass 32 bits."""
+import math
+
+import pytest
+import torch
+
+import reels_amd as ra
+from tests._util import U, assert_within
+
+pytestmark = pytest.mark.gpu
+
+
+def test_self_attention_of_a_block_trains(dev):
+    """norm -> projections -> norms of q and k -> rotary -> attention, and back down to the gradients of
+    the norms' weights, clipped: against the same in 64 bits. Float32 compute: the operators' errors
+    are a few u of the sizes involved, the attention's and the linears' 1e-5 of them."""
+    B, S, H, D = 1, 36, 2, 32
+    K = H * D
+    g = torch.Generator(device=dev).manual_seed(4)
+
+    def rnd(*s, scale=1.0):
+        return torch.randn(*s, generator=g, device=dev) * scale
+    x, res, dout = rnd(B, S, K), rnd(B, S, K), rnd(B, S, H, D)
+    w0, wq, wk = 1 + rnd(K, scale=0.1), 1 + rnd(K, scale=0.1), 1 + rnd(K, scale=0.1)
+    mats = [ra.quantize_frozen_matrix(rnd(K, K, scale=K ** -0.5)) for _ in range(3)]
+    pos, axes = ra.grid_positions(2, 3, 6, dev), ra.rotary_axes(D)
+
+    n = ra.rms_norm(x, w0, 1e-6, res)
+    flat = n.output.reshape(S, K)
+    q, k, v = (ra.i8lora_forward(flat, m)[0] for m in mats)
+    nq, nk = ra.rms_norm(q, wq), ra.rms_norm(k, wk)
+    rq, rk = ra.rotary_qk(nq.output.view(B, S, H, D), nk.output.view(B, S, H, D), pos, axes)
+    out, cache = ra.memory_efficient_attention(rq, rk, v.view(B, S, H, D))
+    ga = ra.memory_efficient_attention_backward(rq, rk, v.view(B, S, H, D), dout, cache)
+    dq, dk = ra.rotary_qk_backward(ga.q, ga.k, pos, axes)
+    gq = ra.rms_norm_backward(dq.reshape(S, K), q, wq, nq.rstd)
+    gk = ra.rms_norm_backward(dk.reshape(S, K), k, wk, nk.rstd)
+    dflat = sum(ra.i8lora_backward(d, None, m)[0]
+                for d, m in zip((gq.x, gk.x, ga.v.reshape(S, K)), mats))
+    g0 = ra.rms_norm_backward(dflat.view(B, S, K), n.sum, w0, n.rstd, dsum=res)
+    grads = [g0.weight, gq.weight, gk.weight]
+
+    # the same in 64 bits by autograd
+    xs, ws = [t.double().requires_grad_(True) for t in (x, res)], [t.double().requires_grad_(True) for t in (w0, wq, wk)]
+    deq = [m.values.double() * m.scales.double()[:, None] for m in mats]
+
+    def norm(t, w):
+        return t / torch.sqrt(t.square().mean(-1, keepdim=True) + float(torch.tensor(1e-6))) * w
+
+    def rot(t):
+        ang = torch.cat([pos[:, a:a + 1].double() * torch.tensor([1e4 ** (-j / p) for j in range(p)], dtype=torch.float64,
+                                                                 device=dev) for a, p in enumerate(axes)], -1)
+        c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+        a, b = t[..., 0::2], t[..., 1::2]
+        return torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2)
+    sm = xs[0] + xs[1]
+    f = norm(sm, ws[0]).reshape(S, K)
+    Q, Kk, V = (f @ m.t() for m in deq)
+    rQ, rK = rot(norm(Q, ws[1]).view(B, S, H, D)), rot(norm(Kk, ws[2]).view(B, S, H, D))
+    p = torch.softmax((rQ.transpose(1, 2) @ rK.transpose(1, 2).transpose(-1, -2)) / math.sqrt(D), -1)
+    O = (p @ V.view(B, S, H, D).transpose(1, 2)).transpose(1, 2)
+    want = torch.autograd.grad((O, sm), xs + ws, (dout.double(), res.double()))
+    for got, ref in [(out, O), (g0.x, want[0]), (g0.x, want[1])] + list(zip(grads, want[2:])):
+        assert_within(got, ref, 1e-4 * ref.detach().abs().max(), "block")
+    before = [t.clone() for t in grads]
+    total = math.sqrt(sum(float(t.double().square().sum()) for t in before))
+    norm_dev = ra.clip_gradients(grads, total / 3)
+    assert abs(float(norm_dev) - total) <= 2 * U * total
+    for t, b in zip(grads, before):
+        assert_within(t, b.double() / 3, 1e-6 * b.abs(), "clipped")
+
+
+def calls(seed):
+    """Every operator once on inputs of its own; returns what they give."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x, r = (torch.randn(200, 1000, generator=g, device="cuda").bfloat16() for _ in range(2))
+    w = torch.rand(1000, generator=g, device="cuda")
+    n = ra.rms_norm(x, w, 1e-6, r)
+    b = ra.rms_norm_backward(x, n.sum, w, n.rstd, r)
+    q = ra.rms_norm_quantized(x, w, 1e-6, r).output
+    m = ra.quantize_rows(torch.randn(700, 1000, generator=g, device="cuda").bfloat16())
+    y = ra.quantized_linear(q, m, activation="gelu_tanh")
+    z = ra.quantized_linear(ra.QuantizedMatrix(q.values[:3], q.scales[:3], q.compute_dtype), m)
+    o = ra.quantized_linear(ra.quantize_rows(x[:, :999]), ra.quantize_rows(x[:50, 1:]))
+    h = x[:, :960].reshape(1, 200, 15, 64)
+    a, c = ra.rotary_qk(h, h[:, :, :5], ra.grid_positions(1, 10, 20, "cuda"), (12, 10, 10))
+    gs = [t.float() for t in (x, r)]
+    norm = ra.clip_gradients(gs, 1.0)
+    return [n.output, n.sum, n.rstd, b.x, b.weight, q.values, q.scales, y, z, o, a, c, norm, *gs]
+
+
+def test_other_streams_and_two_at_once(dev):
+    want = [[t.clone() for t in calls(s)] for s in (1, 2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for turn in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = calls(i + 1)
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(map(torch.equal, got[i], want[i])), (turn, i)
+
+
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 elements: the last rows are those of a call on them alone."""
+    M, C = 420_000, 5120  # 2.15e9 elements
+    x = torch.empty(M, C, dtype=torch.bfloat16, device=dev).normal_()
+    w = torch.rand(C, device=dev)
+    last = x[-3:].clone()
+    n = ra.rms_norm(x, w)
+    assert torch.equal(n.output[-3:], ra.rms_norm(last, w).output)
+    gx = ra.rms_norm_backward(x, x, w, n.rstd, want_dweight=False).x
+    assert torch.equal(gx[-3:], ra.rms_norm_backward(last, last, w, n.rstd[-3:], want_dweight=False).x)
+    del n, gx
+    q = ra.rms_norm_quantized(x, w).output
+    assert torch.equal(q.values[-3:], ra.rms_norm_quantized(last, w).output.values)
+    del q
+    pos = torch.arange(M, dtype=torch.int32, device=dev)[:, None]
+    y = ra.rotary(x.view(1, M, 40, 128), pos, (64,))
+    assert torch.equal(y[:, -3:], ra.rotary(last.view(1, 3, 40, 128), pos[-3:], (64,)))
+    del y
+    out = torch.empty_like(x)
+    norm = ra.clip_gradients([x], 1.0, out=[out])
+    assert abs(float(norm) / math.sqrt(M * C) - 1) < 1e-3
+    f = float(torch.tensor(1.0 / (float(norm) + 1e-6)))
+    assert_within(out[-3:], last.double() * f, 4 * U * last.double().abs() * f, "clipped")
+    del out
+    xq, m = ra.quantize_rows(x[:, :64]), ra.quantize_rows(x[:C, 64:128])
+    y = ra.quantized_linear(xq, m)
+    part = ra.quantized_linear(ra.QuantizedMatrix(xq.values[-3:], xq.scales[-3:], xq.compute_dtype), m)
+    assert torch.equal(y[-3:], part)
+
+
+def test_rows_that_are_not_finite_are_seen_after_quantising(dev):
+    x = torch.randn(4, 300, device=dev).bfloat16()
+    x[1, 7], x[2, 299] = float("nan"), float("inf")
+    q = ra.quantize_rows(x)
+    v = q.values.double() * q.scales.double()[:, None]
+    assert torch.isfinite(v[[0, 3]]).all() and not torch.isfinite(v[1]).all() and not torch.isfinite(v[2]).all()
