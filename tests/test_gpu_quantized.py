@@ -50,7 +50,7 @@ def check(y, x, w, bias, res, act, what=""):
 SIZES = [(1, 1, 1), (1, 64, 16), (1, 5120, 1000), (2, 100, 77), (3, 17, 5), (7, 1536, 1537), (16, 256, 64),
          (17, 130, 33), (31, 512, 130), (33, 1000, 300), (64, 64, 64), (65, 65, 65), (100, 2048, 513),
          (128, 384, 256), (129, 1024, 257), (200, 4096, 640), (255, 640, 255), (300, 131071, 20),
-         (513, 128, 769), (300, 4, 70), (300, 100, 130), (70, 252, 65), (1100, 1796, 1024), (2050, 1300, 2049), (777, 1000, 3001), (1025, 896, 1024), (2100, 1537, 130), (5000, 256, 512)]
+         (513, 128, 769), (300, 4, 70), (300, 100, 130), (70, 252, 65), (1100, 1796, 1024), (2050, 1300, 2049), (777, 1000, 3001), (4100, 1024, 2304), (4099, 1028, 2310), (40000, 100, 2048), (20001, 256, 2049), (1025, 896, 1024), (2100, 1537, 130), (5000, 256, 512)]
 
 
 @pytest.mark.parametrize("dtype", list(DT))
