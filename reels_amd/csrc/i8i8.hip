@@ -7,7 +7,7 @@
 // form and split gives the same bits; the epilogue runs in f32 and rounds once.
 #include "vec.h"
 
-#include <mutex>
+#include <atomic>
 
 namespace reels {
 namespace {
@@ -527,16 +527,19 @@ __global__ __launch_bounds__(256) void product_pad_kernel(const int8_t* __restri
 
 template <int TJ> int launch_tiles(const ProductArgs& a, int dtype, hipStream_t st) {
   using T = Tile<TJ>;
-  static std::once_flag once;
-  static hipError_t attr_err = hipSuccess;
-  std::call_once(once, [&] {
+  // the LDS size is an attribute of a kernel on a device: set once for each
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err == hipSuccess && (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1))) {
     const void* ks[] = {(const void*)product_tile_kernel<REELS_HIP_BF16, TJ>, (const void*)product_tile_kernel<REELS_HIP_F16, TJ>,
                         (const void*)product_tile_kernel<REELS_HIP_F32, TJ>};
     for (const void* k : ks)
-      if (attr_err == hipSuccess) attr_err = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-  });
-  if (attr_err != hipSuccess)
-    return fail(REELS_HIP_EHIP, std::string("product_tile: hipFuncSetAttribute: ") + hipGetErrorString(attr_err));
+      if (err == hipSuccess) err = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (err == hipSuccess && dev < 64) done.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+  }
+  if (err != hipSuccess)
+    return fail(REELS_HIP_EHIP, std::string("product_tile: hipFuncSetAttribute: ") + hipGetErrorString(err));
   const int64_t tn = ceil_div(a.N, T::BN), tm = ceil_div(a.M, T::BM);
   if (tn * tm > ((int64_t)1 << 31) - 1) return fail(REELS_HIP_EINVAL, "reels_hip_i8i8_linear: too many output tiles");
   { TraceScope _ts(st, TJ == 8 ? "product_tile_kernel<256>" : "product_tile_kernel<128>");
