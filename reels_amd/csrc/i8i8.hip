@@ -71,8 +71,11 @@ template <int ROWS, int NT> __device__ __forceinline__ void clear_tail(uint8_t* 
   asm volatile("" ::: "memory");
 }
 
+// Two waves on a SIMD are asked for by name: left alone the compiler holds the whole residual of an f32
+// tile in registers at TJ = 4, one workgroup then has the CU to itself, and 6000 x 512 -> 768 in f32
+// takes 17.3 us instead of 11.1.
 template <int ELT, int TJ>
-__global__ __launch_bounds__(Tile<TJ>::NT) void product_tile_kernel(ProductArgs a, int tiles_n, int tiles_m) {
+__global__ __launch_bounds__(Tile<TJ>::NT, 2) void product_tile_kernel(ProductArgs a, int tiles_n, int tiles_m) {
   using T = Tile<TJ>;
   constexpr int V = 16 / elt_bytes(ELT);
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
