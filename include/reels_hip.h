@@ -369,6 +369,8 @@ int reels_hip_attention_bwd(const void* q, const void* k, const void* v, const v
  *   dw[c] = sum_m dy s rstd   (f32; NULL to skip)
  * dw needs a workspace of reels_hip_rms_norm_workspace_bytes(rows, cols) bytes (NULL without it).
  * Bitwise reproducible: no atomics, fixed orders of summation. rows = 0 gives dw = 0.
+ * Sizes whose launch would need 2^32 threads or more are refused with REELS_HIP_EINVAL, here and
+ * by the two operators that follow (rows take 16 to 1024 threads each, the fewer the shorter).
  */
 int reels_hip_rms_norm(const void* x, int64_t ld_x, const void* residual, int64_t ld_r,
                        const void* weight, int w_dtype, int dtype, int64_t rows, int64_t cols,

@@ -498,15 +498,16 @@ __global__ __launch_bounds__(64) void product_dot_kernel(ProductArgs a) {
   finish4<ELT>(a, 0, n, 1, sum, a.xs[0], sc, bs);
 }
 
-template <typename K> int launch_rows(K kernel, const char* label, unsigned grid, int threads, const ProductArgs& a, hipStream_t st) {
+template <typename K> int launch_rows(K kernel, const char* label, int64_t grid, int threads, const ProductArgs& a, hipStream_t st) {
+  if (!grid_fits(grid, threads)) return fail(REELS_HIP_EINVAL, "reels_hip_i8i8_linear: too many columns for one launch");
   { TraceScope _ts(st, label);
-    kernel<<<grid, threads, 0, st>>>(a); }
+    kernel<<<(unsigned)grid, threads, 0, st>>>(a); }
   return check_launch(label);
 }
 
 int launch_small(const ProductArgs& a, int dtype, hipStream_t st) {
   const int64_t tn = ceil_div(a.N, small::BT), tm = ceil_div(a.M, small::BT);
-  if (tn * tm > ((int64_t)1 << 31) - 1) return fail(REELS_HIP_EINVAL, "reels_hip_i8i8_linear: too many output tiles");
+  if (!grid_fits(tn * tm, small::NT)) return fail(REELS_HIP_EINVAL, "reels_hip_i8i8_linear: too many output tiles for one launch");
   { TraceScope _ts(st, "product_small_kernel");
     with_any_elt(dtype, [&](auto e) {
       product_small_kernel<decltype(e)::value><<<(unsigned)(tn * tm), small::NT, 0, st>>>(a, (int)tm);
@@ -530,6 +531,8 @@ __global__ __launch_bounds__(256) void product_pad_kernel(const int8_t* __restri
 
 template <int TJ> int launch_tiles(const ProductArgs& a, int dtype, hipStream_t st) {
   using T = Tile<TJ>;
+  const int64_t tn = ceil_div(a.N, T::BN), tm = ceil_div(a.M, T::BM);
+  if (!grid_fits(tn * tm, T::NT)) return fail(REELS_HIP_EINVAL, "reels_hip_i8i8_linear: too many output tiles for one launch");
   // the LDS size is an attribute of a kernel on a device: set once for each
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -543,8 +546,6 @@ template <int TJ> int launch_tiles(const ProductArgs& a, int dtype, hipStream_t 
   }
   if (err != hipSuccess)
     return fail(REELS_HIP_EHIP, std::string("product_tile: hipFuncSetAttribute: ") + hipGetErrorString(err));
-  const int64_t tn = ceil_div(a.N, T::BN), tm = ceil_div(a.M, T::BM);
-  if (tn * tm > ((int64_t)1 << 31) - 1) return fail(REELS_HIP_EINVAL, "reels_hip_i8i8_linear: too many output tiles");
   { TraceScope _ts(st, TJ == 8 ? "product_tile_kernel<256>" : "product_tile_kernel<128>");
     with_any_elt(dtype, [&](auto e) {
       product_tile_kernel<decltype(e)::value, TJ><<<(unsigned)(tn * tm), T::NT, T::LDS, st>>>(a, (int)tn, (int)tm);
@@ -604,8 +605,8 @@ extern "C" int reels_hip_i8i8_linear(const int8_t* x, const float* xs, const int
     int rc = REELS_HIP_OK;
     with_any_elt(dtype, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      if (M == 1 && K >= kDotCodes) rc = launch_rows(product_dot_kernel<E>, "product_dot_kernel", (unsigned)N, 64, a, st);
-      else rc = launch_rows(product_few_kernel<E>, "product_few_kernel", (unsigned)ceil_div(N, 16), kFewWaves * 64, a, st);
+      if (M == 1 && K >= kDotCodes) rc = launch_rows(product_dot_kernel<E>, "product_dot_kernel", N, 64, a, st);
+      else rc = launch_rows(product_few_kernel<E>, "product_few_kernel", ceil_div(N, 16), kFewWaves * 64, a, st);
     });
     return rc;
   }

@@ -607,9 +607,14 @@ Form norm_form(int elt, int64_t cols) {
   const int64_t chunks = ceil_div(cols, 16 / elt_bytes(elt));
   for (int tpr : {16, 64, 256})
     if (chunks <= 4 * tpr) return {tpr, (int)ceil_div(chunks, tpr)};
-  if (chunks <= 2048) return {512, chunks <= 1536 ? 3 : 4};
-  if (elt == REELS_HIP_F32 && chunks <= 4096) return {1024, chunks <= 3072 ? 3 : 4};  // half the values a chunk
+  if (chunks <= 2048) return {512, (int)ceil_div(chunks, 512)};
+  if (elt == REELS_HIP_F32 && chunks <= 4096) return {1024, (int)ceil_div(chunks, 1024)};  // half the values a chunk
   return {0, 0};
+}
+
+bool norm_fits(int64_t rows, Form f) {  // a group of threads for each row
+  const int threads = f.tpr == 0 ? kLongThreads : f.tpr, wg = threads < 256 ? 256 : threads;
+  return grid_fits(ceil_div(rows, wg / threads), wg);
 }
 
 template <int N> using Int = std::integral_constant<int, N>;
@@ -659,6 +664,7 @@ int norm_forward(const char* fn, const char* label, bool quant, NormArgs a, int 
   a.w_f32 = w_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32;
   a.per_col = 1.0 / (double)a.cols;
   const Form f = norm_form(dtype, a.cols);
+  if (!norm_fits(a.rows, f)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
   { TraceScope _ts(st, label);
     with_any_elt(dtype, [&](auto e) {
       constexpr int E = decltype(e)::value;
@@ -737,6 +743,8 @@ extern "C" int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void*
   if (rows == 0 && dw == nullptr) return REELS_HIP_OK;
   NormBwdArgs a{dy, s, dsum, weight, rstd, dx, (float*)workspace, rows, cols, 1.0 / (double)cols, w_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32};
   const Form f = norm_form(dtype, cols);
+  if (((dw == nullptr || f.tpr == 0) && !norm_fits(rows, f)) || (dw != nullptr && !grid_fits(ceil_div(cols, 32), 1024)))
+    return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows or columns for one launch");
   const int64_t parts = rows == 0 ? 0 : norm_parts(rows, dtype, f);
   if (rows > 0) {
     TraceScope _ts(st, "norm_bwd_kernel");

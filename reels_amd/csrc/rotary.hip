@@ -160,6 +160,7 @@ extern "C" int reels_hip_rotary(const void* q, int64_t ld_q, const void* k, int6
   if (tb > a.tokens / 2048) tb = a.tokens / 2048;
   a.tb = (int)(tb < 1 ? 1 : tb > 16 ? 16 : tb);
   const unsigned grid = (unsigned)ceil_div(a.tokens, a.tb);
+  if (!grid_fits(ceil_div(a.tokens, a.tb), kThreads)) return fail(REELS_HIP_EINVAL, fn + "too many tokens for one launch");
   const size_t lds = (size_t)a.tb * P * sizeof(float2);
   // the widest vector that divides the parts of a head
   int v = 16 / elt_bytes(dtype);

@@ -118,6 +118,8 @@ template <typename F> inline void with_any_elt(int elt, F&& f) {
   else if (elt == REELS_HIP_F16) f(std::integral_constant<int, REELS_HIP_F16>{});
   else f(std::integral_constant<int, REELS_HIP_BF16>{});
 }
+// A launch holds less than 2^32 threads
+inline bool grid_fits(int64_t blocks, int threads) { return blocks < ((int64_t)1 << 32) / threads; }
 inline bool known_elt(int elt) { return elt == REELS_HIP_F32 || elt == REELS_HIP_BF16 || elt == REELS_HIP_F16; }
 
 // Sum or maximum over groups of G lanes (16 or 64, all of them active), the same bits in every lane:

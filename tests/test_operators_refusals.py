@@ -107,6 +107,26 @@ def test_clip_c_refusals():
     assert clip(g=(4096, 4100, 12288), o=(20000, 30000, 40000), norm=None) == -1  # (gradients may overlap; norm NULL)
 
 
+def test_launches_of_2_to_32_threads_are_refused():
+    """A launch holds less than 2^32 threads: 16 for a row of up to 512 (f32 256) elements, 1024 for the
+    longest; 256 for each 16 tokens of a small head; 512 for 16 columns of a few tokens' product."""
+    L = _lib.lib()
+    pairs = (ctypes.c_int32 * 1)(1)
+    for C, rows in ((8, 1 << 28), (8, (1 << 28) - 1), (1 << 20, 1 << 22)):
+        assert L.reels_hip_rms_norm(F, C, None, C, None, 1, 1, rows, C, 1e-6, None, F, F, None) == -1
+        assert L.reels_hip_rms_norm_i8(F, C, None, C, None, 1, 1, rows, C, 1e-6, None, F, F, None) == -1
+        assert L.reels_hip_rms_norm_bwd(F, F, None, None, 1, F, 1, rows, C, F, None, None, 0, None) == -1
+        assert "rows" in _err()
+    C = 1 << 28
+    assert L.reels_hip_rms_norm_bwd(F, F, None, None, 1, F, 1, 1, C, F, F, F, 1 << 62, None) == -1 and "columns" in _err()
+    S = (1 << 31) - 1
+    assert L.reels_hip_rotary(F, 2, None, 0, F, 3, 1, 1, 1, S, 1, 0, 2, pairs, 1, 1e4, 1, 0, F, None, None) == -1
+    assert "tokens" in _err()
+    prod = L.reels_hip_i8i8_linear
+    for M, K, N in ((1, 4096, 1 << 26), (4, 64, 1 << 30), (1 << 30, 64, 1 << 30)):
+        assert prod(F, F, F, F, None, None, 0, 1, M, K, N, F, None, 0, None) == -1 and "launch" in _err()
+
+
 def test_python_refusals():
     x = torch.zeros(4, 8, dtype=BF)
     for call in (lambda: ra.rms_norm(x), lambda: ra.rms_norm_quantized(x), lambda: ra.quantize_rows(x),
