@@ -1,11 +1,15 @@
 """The operators around the linears as a program uses them together: a block's run forward and
-backward, other streams, two streams at once, tensors whose offsets pass 32 bits."""
+backward, other streams, two streams at once, tensors whose offsets pass 32 bits,
+outputs in the place of inputs."""
+import ctypes
 import math
 
 import pytest
 import torch
 
 import reels_amd as ra
+from reels_amd import _lib
+from reels_amd.layers import _DTYPE_CODE, _launch, _stream
 from tests._util import U, assert_within
 
 pytestmark = pytest.mark.gpu
@@ -140,3 +144,56 @@ def test_rows_that_are_not_finite_are_seen_after_quantising(dev):
     q = ra.quantize_rows(x)
     v = q.values.double() * q.scales.double()[:, None]
     assert torch.isfinite(v[[0, 3]]).all() and not torch.isfinite(v[1]).all() and not torch.isfinite(v[2]).all()
+
+
+@pytest.mark.parametrize("C,dtype", [(101, torch.float32), (2049, torch.bfloat16), (5121, torch.float16),
+                                     (8191, torch.float32), (20001, torch.bfloat16)])
+def test_sum_in_place(dev, C, dtype):
+    """The sum may take the place of x or of the residual: the same bits as into a buffer of its own,
+    where a row ends inside a chunk and where the row is read twice (20001)."""
+    x, r = (torch.randn(9, C, device=dev).to(dtype) for _ in range(2))
+    w = torch.randn(C, device=dev)
+    want, wantq = ra.rms_norm(x, w, 1e-6, r), ra.rms_norm_quantized(x, w, 1e-6, r)
+    code = _DTYPE_CODE[dtype]
+    for into in (0, 1):
+        for quantized in (False, True):
+            ops = [x.clone(), r.clone()]
+            s = ops[into]
+            out = torch.empty(9, C, dtype=torch.int8 if quantized else dtype, device=dev)
+            row = torch.empty(9, device=dev)
+            _launch("reels_hip_rms_norm_i8" if quantized else "reels_hip_rms_norm", dev, ops[0].data_ptr(), C,
+                    ops[1].data_ptr(), C, w.data_ptr(), _lib.F32, code, 9, C, 1e-6, s.data_ptr(), out.data_ptr(),
+                    row.data_ptr(), _stream(dev))
+            assert torch.equal(s, want.sum)
+            if quantized:
+                assert torch.equal(out, wantq.output.values) and torch.equal(row, wantq.output.scales)
+            else:
+                assert torch.equal(out, want.output) and torch.equal(row, want.rstd)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 77), (5, 100, 130), (65, 63, 70), (300, 256, 131), (1100, 1796, 1025),
+                                   (4099, 1028, 2311)])
+def test_product_over_its_residual(dev, M, K, N, dtype):
+    """y may be the residual itself, in every form of the product."""
+    x, w = (ra.quantize_rows(torch.randn(n, K, device=dev).to(dtype)) for n in (M, N))
+    res = torch.randn(M, N, device=dev).to(dtype)
+    want = ra.quantized_linear(x, w, None, "gelu_tanh", res)
+    nbytes = _lib.lib().reels_hip_i8i8_workspace_bytes(M, K, N)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch("reels_hip_i8i8_linear", dev, x.values.data_ptr(), x.scales.data_ptr(), w.values.data_ptr(),
+            w.scales.data_ptr(), None, res.data_ptr(), _lib.ACT_GELU_TANH, _DTYPE_CODE[dtype], M, K, N,
+            res.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
+    assert torch.equal(res, want)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D,axes", [(128, (22, 21, 21)), (64, (8, 8)), (10, (1, 2))])
+def test_rotary_in_place(dev, D, axes, interleaved):
+    q, k = (torch.randn(2, 37, h, D, device=dev).bfloat16() for h in (3, 2))
+    pos = torch.randint(0, 50, (37, len(axes)), device=dev, dtype=torch.int32)
+    want = ra.rotary_qk(q, k, pos, axes, 1e4, interleaved)
+    pairs = (ctypes.c_int32 * len(axes))(*axes)
+    _launch("reels_hip_rotary", dev, q.data_ptr(), 3 * D, k.data_ptr(), 2 * D, pos.data_ptr(), _lib.I32, 1, _lib.BF16,
+            2, 37, 3, 2, D, pairs, len(axes), 1e4, int(interleaved), 0, q.data_ptr(), k.data_ptr(), _stream(dev))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
