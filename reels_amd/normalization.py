@@ -11,6 +11,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .layers import _DTYPE_CODE, QuantizedMatrix, _act_dtype, _contig, _launch, _ptr, _stream
@@ -167,6 +168,7 @@ class RMSNormFunction(torch.autograd.Function):
         return r.output if residual is None else (r.output, r.sum)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dsum=None):
         s, weight, rstd = ctx.saved_tensors
         residual = ctx.needs_input_grad[2]

@@ -13,6 +13,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .layers import _DTYPE_CODE, _act_dtype, _launch, _ptr, _stream
@@ -136,6 +137,7 @@ class RotaryFunction(torch.autograd.Function):
         return _rotate(q, k, positions, axes, theta, interleaved, 0)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
         dq, dk = _rotate(dq, dk, positions, *ctx.args, 1)

@@ -197,3 +197,15 @@ def test_rotary_in_place(dev, D, axes, interleaved):
     _launch("reels_hip_rotary", dev, q.data_ptr(), 3 * D, k.data_ptr(), 2 * D, pos.data_ptr(), _lib.I32, 1, _lib.BF16,
             2, 37, 3, 2, D, pairs, len(axes), 1e4, int(interleaved), 0, q.data_ptr(), k.data_ptr(), _stream(dev))
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_second_derivatives_raise(dev):
+    """The backward kernels have no derivative of their own: asking for it is an error, not a term left out."""
+    x, r = (torch.randn(4, 64, device=dev, requires_grad=True) for _ in range(2))
+    w = torch.ones(64, device=dev, requires_grad=True)
+    pos = torch.arange(4, dtype=torch.int32, device=dev)[:, None]
+    for y in (ra.RMSNormFunction.apply(x, w, None, 1e-6), ra.RMSNormFunction.apply(x, w, r, 1e-6)[1],
+              ra.RotaryFunction.apply(x.view(1, 4, 2, 32), None, pos, (16,), 1e4, True)[0]):
+        (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.square().sum().backward()
