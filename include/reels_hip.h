@@ -360,8 +360,9 @@ int reels_hip_attention_bwd(const void* q, const void* k, const void* v, const v
  *
  * reels_hip_rms_norm_i8 writes the row in 8 bits instead, in the layout of reels_hip_i8_pack:
  *   scales[m] = max_c |s weight| rstd / 127,  q = round_ties_even(127 s weight / max_c |s weight|)
- * (q * scales is the norm's row; the quotient is formed in 64 bits). A zero row has scale 1. A row
- * whose scale is not finite (NaN or infinities in it) has scale NaN and zero codes.
+ * (q * scales is the norm's row; the quotient is formed in 64 bits). A zero row has scale 1 (with
+ * eps = 0 NaN, as y). A row whose scale is not finite, or that holds NaN or infinities, also where
+ * their weight is zero, has scale NaN and zero codes.
  *
  * reels_hip_rms_norm_bwd, with s the sum that the forward wrote (x where it had no residual), its
  * rstd, and dsum the gradient that reaches s from elsewhere (the residual stream; NULL for none):

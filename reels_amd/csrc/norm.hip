@@ -80,7 +80,9 @@ struct Quant {
   __device__ __forceinline__ Quant(double t, double rstd, bool even) : top(t) {
     const double size = top * rstd;  // the row's largest value
     scale = (float)(size * (1.0 / 127.0));
-    const bool whole = __builtin_isfinite(scale);
+    // rstd is 0 or NaN where the row holds an infinity or NaN: top may have lost it, where its weight
+    // is zero and the product NaN
+    const bool whole = __builtin_isfinite(scale) && rstd > 0.0;
     if (!whole) scale = __builtin_nanf("");
     else if (top == 0.0) scale = 1.0f;
     zero = !whole || top == 0.0;

@@ -2,6 +2,8 @@
 roundings of the kernels (u = 2^-24): y has two products and rstd's rounding (3 u); dx forms g = dy w
 (u), k = rstd^2 mean(g s) from rounded g and rstd (4 u on the mean of |g s|), their difference and its
 product with rstd (3 u); dw adds rows / 256 + 100 terms at most one after the other."""
+import math
+
 import pytest
 import torch
 
@@ -294,3 +296,33 @@ def test_norm_feeds_attention(dev):
     ref = torch.matmul(p, x.view(B, S, H, D).double().transpose(1, 2).contiguous()).transpose(1, 2)
     # P is rounded to bf16 and the result once more
     assert (out.double() - ref).abs().max() <= 2.0 ** -7 * x.double().abs().max()
+
+
+@pytest.mark.parametrize("dtype,wtype", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("C", [5, 96, 5120, 16384, 40000])
+def test_infinities_under_zero_weights_reach_the_quantized_rows(dev, C, dtype, wtype):
+    """An infinity times a zero weight is NaN in the norm's row, whatever the other products are: its
+    scale is NaN and its codes are 0."""
+    at = C // 2
+    x = (torch.randn(6, C, device=dev) + 3).to(DT[dtype])
+    x[1, at], x[2, at], x[3, at] = math.inf, -math.inf, math.nan
+    r = torch.zeros_like(x)
+    if dtype == "f16":  # the sum overflows
+        x[4, at] = r[4, at] = 60000.0
+    else:
+        r[4, at] = math.inf
+    one = torch.ones(C, device=dev, dtype=DT[wtype])
+    one[at] = 0
+    for w, ordinary in ((one, None), (torch.zeros_like(one), 1.0)):
+        for residual in (None, r):
+            bad = [1, 2, 3] if residual is None else [1, 2, 3, 4]
+            good = [i for i in range(6) if i not in bad]
+            y = rms_norm(x, w, 1e-6, residual).output
+            assert torch.isnan(y[bad, at]).all() and torch.isfinite(y[good]).all()
+            q = rms_norm_quantized(x, w, 1e-6, residual).output
+            assert torch.isnan(q.scales[bad]).all() and not q.values[bad].any()
+            assert torch.isfinite(q.scales[good]).all()
+            if ordinary is not None:
+                assert (q.scales[good] == ordinary).all() and not q.values[good].any()
+            else:
+                assert (q.values[good].abs().amax(1) == 127).all()
