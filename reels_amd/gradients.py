@@ -10,6 +10,7 @@ from operator import attrgetter
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .layers import _DTYPE_CODE, _launch, _need_device, _stream
@@ -71,6 +72,9 @@ def _call(grads, checked, max_norm, out):
     else:
         outs = ptrs if out is None else _pointers(out)
         _launch("reels_hip_clip_gradients", dev, of, outs.buffer_info()[0], *to, max_norm, *end)
+        # the kernel writes behind torch's back: a graph that has saved one of these has to see it (50 ns
+        # a tensor, while the kernels run)
+        increment_version(grads if out is None else out)
     return norm
 
 
@@ -94,7 +98,8 @@ def clip_gradients(grads: Sequence[Optional[torch.Tensor]], max_norm: float,
     sizes and types (and, where they are not contiguous, shapes and strides), such as the pieces of an
     optimizer's buffer. None entries are skipped in both. Gradients whose norm is not finite are left (or
     copied) as they are. Outputs that overlap each other or another gradient raise, a gradient that is
-    given twice to be clipped in place among them."""
+    given twice to be clipped in place among them. Tensors that are written count as changed in place
+    (a replay of a captured call does not count)."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError("max_norm must not be negative or NaN")

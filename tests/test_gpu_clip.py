@@ -132,3 +132,30 @@ def test_adapter_gradients_are_clipped_together(dev):
     assert want > 1 and abs(float(n) - want) <= 1.01 * U * want
     for t, b in zip(grads, before):
         assert_within(t, b.double() / (want + 1e-6), 2 * U * b.abs() / want, "clipped")
+
+
+def test_what_is_clipped_counts_as_changed(dev):
+    """A graph that has saved a tensor notices that it was clipped in place, or written as an output."""
+    g, h, out = (torch.randn(40, device=dev) for _ in range(3))
+    p = torch.randn(40, device=dev, requires_grad=True)
+    for write in (lambda: clip_gradients([g, None, h], 0.1), lambda: clip_gradients([h], 0.1, out=[g])):
+        loss = (p * g).sum()
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    # what is only read does not count as changed
+    loss = (p * g).sum()
+    clip_gradients([g], 0.1, out=[out])
+    gradient_norm([g])
+    loss.backward()
+    assert torch.equal(p.grad, g)
+
+
+def test_clipping_a_tensor_of_inference_mode(dev):
+    """Tensors of inference mode have no count of changes; they are clipped like others."""
+    with torch.inference_mode():
+        g = torch.randn(100, device=dev)
+        want = norm64([g])
+        b = g.clone()
+        clip_gradients([g], 0.5)
+        assert_within(g, b.double() * (0.5 / (want + 1e-6)), 2 * U * b.double().abs() * (0.5 / want), "clipped")
