@@ -430,8 +430,8 @@ int reels_hip_rotary(const void* q, int64_t ld_q, const void* k, int64_t ld_k, c
  *   outs[i] = rnd(grads[i] * min(1, max_norm / (norm + 1e-6)))
  * grads, outs [count] HOST arrays of device pointers, sizes [count] elements, dtypes [count]
  * REELS_HIP_F32, _BF16 or _F16 (of the gradient and its output); outs[i] may be grads[i] (in
- * place) and overlaps nothing else, which is checked. Gradients whose norm is not finite are left
- * (or copied) unscaled. The host arrays may be freed on return, and a call records into a graph,
+ * place) and overlaps nothing else, which is checked. Gradients whose norm is not finite (in f32, as
+ * it is returned) are left (or copied) unscaled. The host arrays may be freed on return, and a call records into a graph,
  * which then holds these pointers. Bitwise reproducible for the same sizes. workspace:
  * reels_hip_grad_workspace_bytes(count) bytes.
  */

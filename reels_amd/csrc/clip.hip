@@ -186,10 +186,10 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const Entry* table
   const Finder at(table, count, cache);
   const double t = total_norm(part, n, slot);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)t;
-  // gradients whose norm is not finite are left as they are: a factor of 0 or NaN would hide which
-  // of them it came from
+  // gradients whose norm, as it is returned, is not finite are left as they are: a factor of 0 or NaN
+  // would hide which of them it came from
   const double f = (double)max_norm / (t + 1e-6);
-  const float factor = __builtin_isfinite(t) && f < 1.0 ? (float)f : 1.0f;
+  const float factor = __builtin_isfinite((float)t) && f < 1.0 ? (float)f : 1.0f;
   each_piece<true>(at, pieces, [&](const Entry& e, int64_t off, int64_t m) {
     if (factor == 1.0f && e.g == e.o) return;  // in place and nothing to clip
     with_type(entry_type(e), [&](auto ty) {

@@ -96,8 +96,8 @@ def clip_gradients(grads: Sequence[Optional[torch.Tensor]], max_norm: float,
     """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)), norm their ``gradient_norm``,
     which it returns (without waiting for it). In place, or into ``out``: tensors of the gradients'
     sizes and types (and, where they are not contiguous, shapes and strides), such as the pieces of an
-    optimizer's buffer. None entries are skipped in both. Gradients whose norm is not finite are left (or
-    copied) as they are. Outputs that overlap each other or another gradient raise, a gradient that is
+    optimizer's buffer. None entries are skipped in both. Gradients whose norm is not finite in
+    float32 are left (or copied) as they are. Outputs that overlap each other or another gradient raise, a gradient that is
     given twice to be clipped in place among them. Tensors that are written count as changed in place
     (a replay of a captured call does not count)."""
     max_norm = float(max_norm)

@@ -159,3 +159,15 @@ def test_clipping_a_tensor_of_inference_mode(dev):
         b = g.clone()
         clip_gradients([g], 0.5)
         assert_within(g, b.double() * (0.5 / (want + 1e-6)), 2 * U * b.double().abs() * (0.5 / want), "clipped")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norms_past_the_f32_range_leave_the_gradients(dev, dtype):
+    """The norm that is returned decides: where it is infinite, the gradients stay."""
+    for n in (2, 1000, 40001):
+        g = [torch.full((n,), 3e38, device=dev).to(DT[dtype]), torch.randn(5, device=dev)]
+        want = [t.clone() for t in g]
+        out = [torch.empty_like(t) for t in g]
+        assert float(gradient_norm(g)) == math.inf
+        assert float(clip_gradients(g, 1.0, out=out)) == math.inf and all(map(torch.equal, out, want))
+        assert float(clip_gradients(g, 1.0)) == math.inf and all(map(torch.equal, g, want))
