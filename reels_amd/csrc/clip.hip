@@ -120,13 +120,14 @@ template <int ELT> __device__ __forceinline__ double piece_sum(const uint8_t* g,
   return t;
 }
 
-template <int ELT> __device__ __forceinline__ void piece_scale(const uint8_t* g, uint8_t* o, int n, float factor) {
+// F: float, or double for a factor that f32 holds with fewer bits than 24 or not at all
+template <int ELT, typename F> __device__ __forceinline__ void piece_scale(const uint8_t* g, uint8_t* o, int n, F factor) {
   constexpr int V = Chunk<ELT>::V;
   each_chunk<ELT>(g, n, [&](const Chunk<ELT>& c, int at, int left) {
     float f[V];
     Chunk<ELT> d;
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = c.get(j) * factor;
+    for (int j = 0; j < V; ++j) f[j] = (float)((F)c.get(j) * factor);
     d.pack(f);
     if (left == V) store_global(o + at, d.d);
     else d.store(o + at, left);
@@ -190,11 +191,15 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const Entry* table
   // would hide which of them it came from
   const double f = (double)max_norm / (t + 1e-6);
   const float factor = __builtin_isfinite((float)t) && f < 1.0 ? (float)f : 1.0f;
+  const bool small = factor < 1.0f && f > 0.0 && f < 0x1p-126;
   each_piece<true>(at, pieces, [&](const Entry& e, int64_t off, int64_t m) {
     if (factor == 1.0f && e.g == e.o) return;  // in place and nothing to clip
     with_type(entry_type(e), [&](auto ty) {
       constexpr int E = decltype(ty)::value;
-      piece_scale<E>((const uint8_t*)e.g + off * elt_bytes(E), (uint8_t*)e.o + off * elt_bytes(E), (int)m, factor);
+      const uint8_t* g = (const uint8_t*)e.g + off * elt_bytes(E);
+      uint8_t* o = (uint8_t*)e.o + off * elt_bytes(E);
+      if (small) piece_scale<E>(g, o, (int)m, f);
+      else piece_scale<E>(g, o, (int)m, factor);
     });
   });
 }

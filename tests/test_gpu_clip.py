@@ -171,3 +171,16 @@ def test_norms_past_the_f32_range_leave_the_gradients(dev, dtype):
         assert float(gradient_norm(g)) == math.inf
         assert float(clip_gradients(g, 1.0, out=out)) == math.inf and all(map(torch.equal, out, want))
         assert float(clip_gradients(g, 1.0)) == math.inf and all(map(torch.equal, g, want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_factors_below_the_f32_range(dev, dtype):
+    """A factor that f32 holds with fewer bits, or not at all: the products keep theirs."""
+    for size, max_norm in ((1e36, 1e-6), (1e36, 1e-3), (1.2e36, 2e-9), (1e30, 1e-15), (1e36, 0.01)):
+        g = [torch.randn(70001, device=dev).mul_(size).to(DT[dtype])]
+        want = norm64(g)
+        f = float(torch.tensor(max_norm)) / want
+        b = g[0].double()
+        n = clip_gradients(g, max_norm)
+        assert abs(float(n) - want) <= 1.01 * U * want
+        assert_within(g[0], b * f, 2 * U * b.abs() * f, f"{size} {max_norm}")
