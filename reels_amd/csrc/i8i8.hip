@@ -35,6 +35,14 @@ __device__ __forceinline__ float gelu_logistic(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
+// The f32 product of a sum and the row's scale stays in range below this scale (the sum is below 2^31).
+// Rows past it (values of 1e30 and more) are scaled by 2^-64 on the way, which loses no bits: the
+// weight's scale brings them back.
+constexpr float kBigScale = 0x1p96f;
+__device__ __forceinline__ float scaled_big(int acc, float xs, float ws, float bias) {
+  return (float)acc * (xs * 0x1p-64f) * ws * 0x1p64f + bias;
+}
+
 // ---- tiled form --------------------------------------------------------------------------------
 // 32 TJ x 32 TJ outputs per workgroup of TJ waves (TJ = 8: 256 x 256, TJ = 4: 128 x 128), a step of
 // 128 codes, each wave 16 TJ tokens x 64 columns in 16 x 16 x 64 MFMAs. The operands travel from HBM
@@ -233,9 +241,14 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void product_tile_kernel(ProductAr
       for (int i = 0; i < 4; ++i) {
         f32x4 o;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          o[v] = (float)acc[i][h * 4 + j][v] * xs * sc[i][v] + bs[i][v];
-          if (a.gelu) o[v] = gelu_logistic(o[v]);
+        for (int v = 0; v < 4; ++v) o[v] = (float)acc[i][h * 4 + j][v] * xs * sc[i][v] + bs[i][v];
+        if (fabsf(xs) >= kBigScale) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[v] = scaled_big(acc[i][h * 4 + j][v], xs, sc[i][v], bs[i][v]);
+        }
+        if (a.gelu) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[v] = gelu_logistic(o[v]);
         }
         *reinterpret_cast<f32x4*>(stage + r * 256 + (((i * 4 + lq) ^ (r & 15)) << 4)) = o;
       }
@@ -287,6 +300,7 @@ __device__ __forceinline__ void finish4(const ProductArgs& a, int64_t m, int64_t
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     o[v] = (float)acc[v] * xs * sc[v] + bs[v];
+    if (fabsf(xs) >= kBigScale) o[v] = scaled_big(acc[v], xs, sc[v], bs[v]);
     if (a.gelu) o[v] = gelu_logistic(o[v]);
   }
   const int64_t at = (m * a.N + n) * elt_bytes(ELT);

@@ -170,3 +170,15 @@ def test_feed_forward_in_8_bits_is_near_the_linear_one(dev):
     # and bf16 roundings: below 3% of the update's rms
     err = (y.float() - ref).square().mean().sqrt()
     assert float(err) < 0.03 * float((ref - x.float()).square().mean().sqrt()) + 2.0 ** -9 * float(ref.abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(1, 4111, 33), (5, 300, 70), (70, 260, 100), (1100, 1796, 1024), (4100, 1024, 2304)])
+def test_sums_past_the_f32_range_before_the_weight_scale(dev, M, K, N, dtype):
+    """Rows of 1e30 and more under a weight of small scales: the sum times the row's scale alone passes
+    the f32 range, the result does not."""
+    x, w, bias, res = make(M, K, N, dtype)
+    x.scales[::2] = torch.rand(x.scales[::2].shape, device=dev) * 3e36 + 1e32
+    w.scales.copy_(torch.rand(N, device=dev) * 1e-12 + 1e-14)
+    for kw in (dict(), dict(bias=bias), dict(bias=bias, residual=res)):
+        check(quantized_linear(x, w, **kw), x, w, kw.get("bias"), kw.get("residual"), False, str(list(kw)))
