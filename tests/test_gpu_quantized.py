@@ -182,3 +182,35 @@ def test_sums_past_the_f32_range_before_the_weight_scale(dev, M, K, N, dtype):
     w.scales.copy_(torch.rand(N, device=dev) * 1e-12 + 1e-14)
     for kw in (dict(), dict(bias=bias), dict(bias=bias, residual=res)):
         check(quantized_linear(x, w, **kw), x, w, kw.get("bias"), kw.get("residual"), False, str(list(kw)))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("K,N", [(4097, 9), (4111, 33), (5135, 64), (7501, 17), (8190, 40), (131071, 5)])
+def test_one_token_of_any_length(dev, K, N, dtype):
+    """One long token: lanes with fewer turns than others, pieces of 16 codes that end in the row's
+    end, codes at odd addresses."""
+    x, w, bias, res = make(1, K, N, dtype)
+    check(quantized_linear(x, w), x, w, None, None, False, "plain")
+    want = quantized_linear(x, w, bias, "gelu_tanh", res)
+    check(want, x, w, bias, res, True, "bias, gelu, residual")
+    for off in (1, 2, 7):
+        flat = torch.zeros(off + K + N * K, dtype=torch.int8, device=dev)
+        xv, wv = flat[off:off + K].view(1, K), flat[off + K:].view(N, K)
+        xv.copy_(x.values)
+        wv.copy_(w.values)
+        y = quantized_linear(QuantizedMatrix(xv, x.scales, x.compute_dtype),
+                             QuantizedMatrix(wv, w.scales, w.compute_dtype), bias, "gelu_tanh", res)
+        assert torch.equal(y, want), off
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_long_rows_do_not_depend_on_their_place(dev, dtype):
+    """One token, a few, hundreds and thousands take different kernels; a row has the same bits in all."""
+    for M, K, N in ((300, 4111, 99), (1500, 4111, 260), (1500, 5120, 300), (4200, 5120, 1100)):
+        x, w, bias, res = make(M, K, N, dtype)
+        for act in (None, "gelu_tanh"):
+            whole = quantized_linear(x, w, bias, act, res)
+            for a, b in ((0, 1), (M - 1, M), (3, 19), (1, 70), (M // 2, M)):
+                part = quantized_linear(QuantizedMatrix(x.values[a:b], x.scales[a:b], x.compute_dtype), w, bias,
+                                        act, res[a:b])
+                assert torch.equal(part, whole[a:b]), (K, N, act, a, b)
