@@ -78,6 +78,11 @@ def _call(grads, checked, max_norm, out):
     return norm
 
 
+def _none_at(ts):
+    """The places of None, looked for only where the list's types have it."""
+    return [i for i, t in enumerate(ts) if t is None] if type(None) in set(map(type, ts)) else []
+
+
 def _without_none(ts):
     return [t for t in ts if t is not None]
 
@@ -96,20 +101,21 @@ def clip_gradients(grads: Sequence[Optional[torch.Tensor]], max_norm: float,
     """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)), norm their ``gradient_norm``,
     which it returns (without waiting for it). In place, or into ``out``: tensors of the gradients'
     sizes and types (and, where they are not contiguous, shapes and strides), such as the pieces of an
-    optimizer's buffer. None entries are skipped in both. Gradients whose norm is not finite in
-    float32 are left (or copied) as they are. Outputs that overlap each other or another gradient raise, a gradient that is
-    given twice to be clipped in place among them. Tensors that are written count as changed in place
-    (a replay of a captured call does not count)."""
+    optimizer's buffer. None entries are skipped in both. Gradients whose norm is not finite in float32
+    are left (or copied) as they are. Outputs that overlap each other or another gradient raise, a
+    gradient that is given twice to be clipped in place among them. Tensors that are written count as
+    changed in place (a replay of a captured call does not count)."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError("max_norm must not be negative or NaN")
     grads = list(grads)
+    none = _none_at(grads)
     if out is not None:
         out = list(out)
-        if len(out) != len(grads) or [o is None for o in out] != [g is None for g in grads]:
+        if len(out) != len(grads) or _none_at(out) != none:
             raise ValueError("out must match the gradients one by one")
-        out = _without_none(out)
-    grads = _without_none(grads)
+    if none:
+        grads, out = _without_none(grads), None if out is None else _without_none(out)
     if not grads:
         raise ValueError("no gradients")
     checked = _tensors(grads, "gradients")

@@ -184,3 +184,15 @@ def test_factors_below_the_f32_range(dev, dtype):
         n = clip_gradients(g, max_norm)
         assert abs(float(n) - want) <= 1.01 * U * want
         assert_within(g[0], b * f, 2 * U * b.abs() * f, f"{size} {max_norm}")
+
+
+def test_none_in_both_lists(dev):
+    g = make([5, 7, 9], ["f32"] * 3)
+    want = [t.clone() for t in g]
+    clip_gradients(want, 0.25)
+    out = [torch.zeros_like(t) for t in g]
+    clip_gradients([None, g[0], None, g[1], g[2]], 0.25, out=[None, out[0], None, out[1], out[2]])
+    assert all(map(torch.equal, out, want))
+    for bad in ([None, *out, None], [out[0], None, None, out[1], out[2]], out):
+        with pytest.raises(ValueError, match="one by one"):
+            clip_gradients([None, g[0], None, g[1], g[2]], 0.25, out=bad)
