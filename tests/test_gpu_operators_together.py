@@ -209,3 +209,37 @@ def test_second_derivatives_raise(dev):
         (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.square().sum().backward()
+
+
+@pytest.mark.parametrize("dtype,tiny", [(torch.float32, 3e-41), (torch.bfloat16, 4e-39), (torch.float16, 2e-6)])
+def test_subnormal_values_are_kept(dev, dtype, tiny):
+    """Inputs, sums and results below the type's normal range are rounded to its steps there, not to zero."""
+    g = torch.Generator(device=dev).manual_seed(9)
+    x, r = ((torch.randn(6, 517, generator=g, device=dev, dtype=torch.float64) * tiny).to(dtype) for _ in range(2))
+    w = torch.full((517,), 2.0 ** -6, device=dev)
+    n = ra.rms_norm(x, w, 1e-6, r)
+    want = (x.double() + r.double()).cpu().to(dtype).to(dev)
+    assert torch.equal(n.sum, want) and n.sum.count_nonzero() > 2000
+    s = want.double()
+    y = s / torch.sqrt(s.square().mean(-1, keepdim=True) + float(torch.tensor(1e-6))) * w.double()
+    assert_within(n.output, y, 4 * U * y.abs(), "y")
+    big = torch.full((5,), 3.0, device=dev, dtype=dtype)
+    grads = [x.clone(), big.clone()]
+    norm = ra.clip_gradients(grads, 1.0)
+    f = 1.0 / (math.sqrt(float(big.double().square().sum() + x.double().square().sum())) + 1e-6)
+    assert_within(grads[0], x.double() * f, 2 * U * x.double().abs() * f, "clipped")
+    assert float(norm) > 3
+    q = x[:, :512].reshape(1, 6, 8, 64)
+    pos = torch.arange(6, device=dev, dtype=torch.int32)[:, None]
+    back = ra.rotary_backward(ra.rotary(q, pos, (32,)), pos, (32,))
+    # two rotations of a pair: two roundings of each to the type's step there, and 18 u of sizes
+    step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    size = q.double().unflatten(-1, (32, 2)).abs().sum(-1, keepdim=True).expand(1, 6, 8, 32, 2).flatten(-2)
+    assert ((back.double() - q.double()).abs() <= 2 * step + (18 * U + 3 * torch.finfo(dtype).eps) * size).all()
+    codes = ra.QuantizedMatrix(torch.randint(-127, 128, (6, 300), generator=g, device=dev, dtype=torch.int8),
+                               torch.full((6,), 3e-42, device=dev), dtype)
+    m = ra.QuantizedMatrix(torch.randint(-127, 128, (70, 300), generator=g, device=dev, dtype=torch.int8),
+                           torch.full((70,), 1.5, device=dev) if dtype != torch.float16 else
+                           torch.full((70,), 1e31, device=dev))
+    v = torch.matmul(codes.values.double(), m.values.double().t().contiguous()) * codes.scales.double()[:, None] * m.scales.double()
+    assert_within(ra.quantized_linear(codes, m), v, 4 * U * v.abs(), "product")
