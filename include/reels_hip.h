@@ -356,7 +356,9 @@ int reels_hip_attention_bwd(const void* q, const void* k, const void* v, const v
  * REELS_HIP_F32), NULL for ones. Rows of x and residual lie ld_x and ld_r elements apart (>= cols),
  * rows of the outputs cols. Any alignment of the element type. sum receives s when residual is set
  * (it may be x or residual themselves where their stride is cols) and is not written otherwise; y
- * overlaps no other operand. A row of zeros with eps = 0 gives NaN, as the formula does.
+ * overlaps no other operand. A row of zeros with eps = 0 gives NaN, as the formula does. rstd is an
+ * f32 value in y as well: with eps = 0 a row whose root mean square is below 2.9e-39 has rstd = Inf and
+ * infinite or NaN elements, and above 8.5e37 it has fewer bits (2^-22 at the end of the range).
  *
  * reels_hip_rms_norm_i8 writes the row in 8 bits instead, in the layout of reels_hip_i8_pack:
  *   scales[m] = max_c |s weight| rstd / 127,  q = round_ties_even(127 s weight / max_c |s weight|)
@@ -368,6 +370,7 @@ int reels_hip_attention_bwd(const void* q, const void* k, const void* v, const v
  * rstd, and dsum the gradient that reaches s from elsewhere (the residual stream; NULL for none):
  *   g = dy * weight;  dx = rnd(rstd (g - s rstd^2 mean_c(g s)) + dsum)   (of x and residual alike)
  *   dw[c] = sum_m dy s rstd   (f32; NULL to skip)
+ * dx overlaps no other operand.
  * dw needs a workspace of reels_hip_rms_norm_workspace_bytes(rows, cols) bytes (NULL without it).
  * Bitwise reproducible: no atomics, fixed orders of summation. rows = 0 gives dw = 0.
  * Sizes whose launch would need 2^32 threads or more are refused with REELS_HIP_EINVAL, here and
@@ -392,7 +395,9 @@ int reels_hip_rms_norm_bwd(const void* dy, const void* s, const void* dsum, cons
  *   w [N][K] int8, ws [N] f32: a weight of reels_hip_i8_pack
  *   bias [N], residual [M][N] (either NULL) and y [M][N] of dtype REELS_HIP_F32, _BF16 or _F16;
  *   y may be residual itself
- *   activation REELS_HIP_ACT_NONE or REELS_HIP_ACT_GELU_TANH (reels_hip_gelu_tanh in f32)
+ *   activation REELS_HIP_ACT_NONE or REELS_HIP_ACT_GELU_TANH: gelu_tanh in f32, formed as
+ *   x / (1 + exp(-2 sqrt(2/pi) (x + 0.044715 x^3))), the same function as reels_hip_gelu_tanh's but
+ *   not the same bits (nearer to it where the result is small)
  * The sums are exact whole numbers (K < 131072), the rest runs in f32 and rounds once, so a row of
  * y does not depend on M nor on its place. Any alignment. workspace:
  * reels_hip_i8i8_workspace_bytes(M, K, N) bytes (0 for up to 16 tokens), for zero-padded copies of
@@ -415,8 +420,9 @@ int reels_hip_i8i8_linear(const int8_t* x, const float* xs, const int8_t* w, con
  * Pair j of axis a turns by pos[token][a] * theta^(-j / axis_pairs[a]) (by its negative with
  * inverse, which is the backward): (u, v) -> (u cos - v sin, u sin + v cos). With interleaved pair
  * p is elements 2p and 2p + 1 of a head, otherwise p and p + P; elements past 2 P are copied.
- * Angles are reduced in 64 bits, so far positions lose nothing; rotations run in f32 and round
- * once. D even, up to 512. Any alignment of the element type.
+ * Angles are formed and reduced in 64 bits (the angle of pair j within (j + 2) 2^-52 of itself, of
+ * theta as the f32 value that it is); rotations run in f32 and round once. D even, up to 512. Any
+ * alignment of the element type.
  */
 int reels_hip_rotary(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* pos,
                      int pos_dtype, int64_t pos_batches, int dtype, int64_t B, int64_t S,

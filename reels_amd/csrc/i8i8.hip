@@ -52,8 +52,9 @@ __device__ __forceinline__ float scaled_big(int acc, float xs, float ws, float b
 // of step kt + 2 into the stage of step kt - 1 already during the first half of step kt. Per step a
 // wave reads TJ + 4 fragments for 4 TJ MFMAs, twice. Rows past the edges read as zeros (the buffer's
 // bounds). K and the rows' addresses are multiples of 4 here, which the copies need; others run on
-// padded copies. Bound by the matrix cores at the power cap: 32760 x 13824 -> 5120 1.66 ms (2.79 POP/s;
-// the vendor's int8 product 2.49 on this size), with bias and residual 1.72.
+// padded copies. Bound by the matrix cores at the power cap: 32760 x 13824 -> 5120 1.66-1.68 ms (2.75-2.79
+// POP/s; the vendor's int8 product 2.49 on this size), with bias and residual 1.65-1.74, single launches
+// 1.73-1.87; f32 output 1.73, with its residual 1.85.
 template <int TJ> struct Tile {
   static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 128;
   static constexpr int ACT = BM * BK, WB = BN * BK, LDS = 3 * ACT + 2 * WB;
@@ -398,9 +399,12 @@ __global__ __launch_bounds__(small::NT) void product_small_kernel(ProductArgs a,
 // ---- few tokens --------------------------------------------------------------------------------
 // Up to 16 tokens: 16 outputs per workgroup, its eight waves take lines of 128 codes in turn and read
 // weight and activations straight into registers (each code of the weight is used once, so LDS would
-// only add a trip), then add their whole-number sums in LDS. Any K and alignment. Bound by the
-// weight's bytes: 1 x 5120 -> 13824 16.1 us (4.4 TB/s), 16 x 5120 -> 5120 11.5 us; four and sixteen
-// waves are within 4% of that at one token of 5120, 2 to 14% slower at 13824 outputs.
+// only add a trip), then add their whole-number sums in LDS. Any K and alignment. The weight's bytes would
+// take 5.0 us at 5120 -> 5120 and 13.4 at 5120 -> 13824; measured are 8.8, 9.2, 10.0 and 11.5 us for 2, 4,
+// 8 and 16 tokens -> 5120 (2.3-3.0 TB/s) and 23.5 us for 16 -> 13824 (3.0). Latency and balance make the
+// difference: N / 16 workgroups are 320 on 256 CUs at 5120 outputs, and a wave's five lines there are
+// two trips of loads, one after the other. With one token, four and sixteen waves are within 4% at 5120
+// outputs, 2 to 14% slower at 13824.
 constexpr int kFewTokens = 16, kFewWaves = 8, kFewUnroll = 4;
 
 // 16 codes at p, the first `left` of which belong to its row of K, zeros for the others: a part of 16

@@ -11,15 +11,16 @@
 //   backward, g = dy w: dx = rnd(rstd (g - s rstd^2 mean_c(g s)) + dsum);  dw = sum_m dy s rstd (f32)
 //
 // All of it is bound by memory: each kernel reads its operands once and keeps the row, as stored, in
-// registers between the reduction and the output. A row belongs to a group of TPR threads that hold NCH
-// 16-byte chunks each: TPR is the smallest of 16, 64 and 256 whose threads need at most four chunks, or
+// registers between the reduction and the output (the backward without dw also spills a few there: 7 of
+// 128 at 5120 bf16, at most 11; f32 rows of 16384 with dw 26). A row belongs to a group of TPR threads
+// that hold NCH 16-byte chunks each: TPR is the smallest of 16, 64 and 256 whose threads need at most four chunks, or
 // 512 (f32: or 1024) with three or four, so short rows (one head) share a wave and long ones have many
 // loads in flight. Rows past 16384 elements run the loop form, which reads them again from L2. Squares
 // and products are summed in 64 bits (MI355X adds those at the rate of 32-bit ones), so the squares of
 // large values do not leave the range; rstd itself is kept in 32 bits.
 //
-// 32760 x 5120 bf16: forward 124 us (5.4 TB/s), with the residual 237 us (5.7), backward 205-225 us
-// (4.5-4.9), with dw and dsum 261 us (5.1), int8 rows with the residual 209-234 us (5.0-5.6); a copy of
+// 32760 x 5120 bf16: forward 120-125 us (5.4-5.6 TB/s), with the residual 237 us (5.7), backward 205-242 us
+// (4.2-4.9), with dw and dsum 261 us (5.1), int8 rows with the residual 209-240 us (4.9-5.6); a copy of
 // 1 GiB runs at 5.3 TB/s.
 #include "vec.h"
 
@@ -440,6 +441,7 @@ struct NormBwdArgs {
 // thread keeps the sums of its own columns in registers over all its rows, and the groups of a
 // workgroup add theirs in LDS in group order, one partial row per workgroup.
 // Waves a SIMD has to hold, by the registers that a row's three operands, weights and sums of dw take
+// (without dw a few less than the compiler wants)
 constexpr int bwd_waves(int tpr, int nch, bool dw) {
   if (tpr == 1024) return 4;
   return dw ? (nch == 1 ? 7 : nch == 2 ? 4 : nch == 3 ? 3 : 2) : (nch == 1 ? 7 : nch == 2 ? 5 : nch == 3 ? 4 : 3);

@@ -19,7 +19,7 @@ _ACTIVATIONS = {None: _lib.ACT_NONE, "gelu_tanh": _lib.ACT_GELU_TANH}
 def quantize_rows(x: torch.Tensor) -> QuantizedMatrix:
     """The rows of an activation matrix ``[M][K]`` as int8 codes with one scale each, by
     ``quantize_frozen_matrix``'s formula but without its check (and its wait) for values that are
-    not finite, whose codes are 0."""
+    not finite: a row that holds one has zero codes and the scale NaN or Inf, so its values are NaN."""
     dt = _act_dtype(x, "x")
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be a [M][K] matrix, got shape {tuple(x.shape)}")

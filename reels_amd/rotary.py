@@ -103,7 +103,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], theta:
            interleaved: bool = True) -> torch.Tensor:
     """x with pair j of axis a turned by ``positions[..., a] * theta ** (-j / axes[a])``. The pairs
     of an axis follow those of the axis before it; pair p is elements 2p and 2p + 1 of a head, or
-    with interleaved=False elements p and p + sum(axes). Elements past 2 sum(axes) are copied."""
+    with interleaved=False elements p and p + sum(axes). Elements past 2 sum(axes) are copied. theta
+    is taken as a float32 value."""
     return _rotate(x, None, positions, axes, theta, interleaved, 0)[0]
 
 
