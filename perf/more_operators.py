@@ -121,7 +121,7 @@ def _packed(x):
     """Rows in microscaled 4 bits as a program keeps them: codes [M][K / 2] of K padded to a multiple
     of 256, the even column in the low half of a byte; a scale's exponent + 127 for each block; and
     those bytes again in the order in which the matrix cores take them, tiles of 64 rows x 8 blocks:
-    [tile of rows][tile of blocks][block % 4][row % 16][block / 4][row / 16]."""
+    [tile of rows][tile of blocks][block % 2][row % 32][block / 2][row / 32]."""
     M, K = x.shape
     Kp = -(-K // 256) * 256
     values, e = _round4(torch.nn.functional.pad(x.float(), (0, Kp - K)))
@@ -130,7 +130,7 @@ def _packed(x):
     codes = codes[:, 0::2] + 16 * codes[:, 1::2]
     scales = (e + 127).to(torch.uint8)
     tiles = torch.nn.functional.pad(scales, (0, 0, 0, -M % 64))
-    tiles = tiles.view(-1, 4, 16, Kp // 256, 2, 4).permute(0, 3, 5, 2, 4, 1).contiguous()
+    tiles = tiles.view(-1, 2, 32, Kp // 256, 4, 2).permute(0, 3, 5, 2, 4, 1).contiguous()
     return codes.contiguous(), scales, tiles.view(-1, Kp // 256, 512)
 
 
