@@ -183,7 +183,7 @@ def _round4(x):
     """(values, exponents) of rows in 4 bits: whole multiples of a step that grows with the value."""
     v = _blocks(x)
     e = (_exponent(v, 2) - 2).clamp_min(-127)
-    unit = torch.ldexp(torch.ones_like(v[..., :1]), e[..., None])
+    unit = torch.exp2(e[..., None].float())
     a = v / unit
     size = a.abs()
     step = 0.5 * (1.0 + (size >= 2.0) + 2.0 * (size >= 4.0))
@@ -193,14 +193,14 @@ def _round4(x):
 def _values4(x):
     """The values that rows stand for in 4 bits."""
     v, e = _round4(x)
-    return (_blocks(v) * torch.ldexp(torch.ones_like(v[:, :1, None]), e[..., None])).flatten(1)[:, :x.shape[1]]
+    return (_blocks(v) * torch.exp2(e[..., None].float())).flatten(1)[:, :x.shape[1]]
 
 
 def _values8(x):
     """The values that rows stand for in 8 bits."""
     v = _blocks(x.float())
     e = _exponent(v, 7).clamp_min(-127)
-    unit = torch.ldexp(torch.ones_like(v[..., :1]), e[..., None] - 6)
+    unit = torch.exp2((e[..., None] - 6).float())
     return (torch.round(v / unit) * unit).flatten(1)[:, :x.shape[1]]
 
 
@@ -210,7 +210,7 @@ def _unpacked(rows, K):
     at = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], device=_DEV)
     at = torch.cat((at, -at))
     v = at[torch.stack((codes & 15, codes >> 4), dim=-1).flatten(1).int()]
-    unit = torch.ldexp(torch.ones((), device=_DEV), scales.int() - 127)
+    unit = torch.exp2(scales.float() - 127.0)
     return (v.view(v.shape[0], -1, _BLOCK) * unit[..., None]).flatten(1)[:, :K]
 
 
