@@ -449,6 +449,112 @@ int reels_hip_clip_gradients(const void* const* grads, void* const* outs, const 
                              void* workspace, size_t ws_bytes, void* stream);
 
 /*
+ * The norm between two sublayers of a transformer block, its output modulated by the conditioning
+ * (modulation, src/layers/modulation.jl:2-11), with the gated residual before it:
+ *   s    = rnd(x + gate * branch)           [rows][cols]  (the product and the sum rounded to f32 first;
+ *                                            x + branch without a gate, x itself without a branch)
+ *   mean = mean_c s, or 0 where center is 0 (the root-mean-square norm)
+ *   rstd = (mean_c (s - mean)^2 + eps)^(-1/2)
+ *   y    = rnd((s - mean) * rstd * (1 + scale) + shift)     (scale and shift: both or neither)
+ * dtype REELS_HIP_F32, _BF16 or _F16 for x, branch, sum and y, rows of x and branch ld_x and ld_branch
+ * elements apart (>= cols), the outputs dense; any alignment of the element type. gate, scale and
+ * shift [rows / rows_per_group][cols] of m_dtype (dtype or REELS_HIP_F32), their rows ld_gate, ld_scale
+ * and ld_shift elements apart: row m takes row m / rows_per_group; rows is a multiple of rows_per_group.
+ * 0 < cols <= 16384. sum receives s where there is a branch (it may be x or branch themselves where
+ * their stride is cols); y overlaps no other operand. stats [rows][3] f32: the mean as the sum of two
+ * values, and rstd. Means and squares are summed in 64 bits, the squares about the mean.
+ * kept_sum, kept_branch with their scales (NULL: not wanted): s and branch as reels_hip_act8_keep would
+ * write them, for the backward; kept_branch only together with kept_sum.
+ *
+ * reels_hip_modulated_norm_mx4 writes the rows of y in 4 bits instead, as reels_hip_mx4_pack lays them
+ * out: codes of reels_hip_mx4_codes_bytes(rows, cols) bytes (4-byte aligned), scales of
+ * reels_hip_mx4_scales_bytes. The values are formed in 64 bits and rounded to f32 before the codes.
+ *
+ * reels_hip_modulated_norm_bwd, with n = (s - mean) rstd, g = dy (1 + scale), and dsum the gradient
+ * that reaches s from elsewhere (NULL for none):
+ *   d = rstd (g - mean_c g - n mean_c(g n)) + dsum   (without mean_c g where center is 0)
+ *   dx = rnd(d);  dbranch = rnd(gate d)  (with a gate; without one it is dx)
+ *   dgate = sum d branch, dscale = sum dy n, dshift = sum dy over each group's rows, f32
+ *     [rows / rows_per_group][cols]; dgate may be NULL, dscale and dshift are both given or both NULL
+ * s and branch dense in dtype, or (s_scales, branch_scales not NULL) the kept codes of both, [rows][cols]
+ * int8. branch is read for dgate alone. dx may be dy or dsum themselves, dbranch overlaps no other operand.
+ * workspace: reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group) bytes where dgate or dscale
+ * is wanted (it may be 0). Bitwise reproducible: no atomics, fixed orders of summation. rows = 0 returns at once.
+ */
+int reels_hip_modulated_norm(const void* x, int64_t ld_x, const void* branch, int64_t ld_branch,
+                             const void* gate, int64_t ld_gate, const void* scale, int64_t ld_scale,
+                             const void* shift, int64_t ld_shift, int m_dtype, int dtype,
+                             int64_t rows, int64_t cols, int64_t rows_per_group, float eps,
+                             int center, void* sum, void* y, float* stats, int8_t* kept_sum,
+                             uint8_t* kept_sum_scales, int8_t* kept_branch,
+                             uint8_t* kept_branch_scales, void* stream);
+int reels_hip_modulated_norm_mx4(const void* x, int64_t ld_x, const void* branch, int64_t ld_branch,
+                                 const void* gate, int64_t ld_gate, const void* scale,
+                                 int64_t ld_scale, const void* shift, int64_t ld_shift, int m_dtype,
+                                 int dtype, int64_t rows, int64_t cols, int64_t rows_per_group,
+                                 float eps, int center, void* sum, uint8_t* codes, uint8_t* scales,
+                                 void* stream);
+size_t reels_hip_modulated_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t rows_per_group);
+int reels_hip_modulated_norm_bwd(const void* dy, const void* s, const uint8_t* s_scales,
+                                 const void* dsum, const void* branch, const uint8_t* branch_scales,
+                                 const void* gate, int64_t ld_gate, const void* scale,
+                                 int64_t ld_scale, const float* stats, int m_dtype, int dtype,
+                                 int64_t rows, int64_t cols, int64_t rows_per_group, int center,
+                                 void* dx, void* dbranch, float* dgate, float* dscale, float* dshift,
+                                 void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Activations kept in 8 bits for the backward. Blocks of 32 neighbours of a row (the last one of a row
+ * may be shorter) share a power of two 2^E: E is the exponent of the block's largest magnitude after
+ * that is rounded to 7 significant bits (between -127 and 127), codes are round_ties_even(x 2^(6-E)), at
+ * most 127, values code * 2^(E-6).
+ *   codes [rows][cols] int8;  scales [rows][ceil(cols / 32)]: E + 127, or 255 where the block holds NaN
+ *   or an infinity (all of its values are NaN)
+ *   reels_hip_act8_keep: the codes of x [rows][cols] (dense, any alignment of the element type)
+ *   reels_hip_act8_gelu_tanh: the same, and y = rnd(gelu_tanh(x)) from x itself
+ *   reels_hip_act8_restore: the values, rounded to dtype (binary16: at most 65504)
+ *   reels_hip_act8_gelu_tanh_bwd: dx = rnd(dy gelu_tanh'(value)); dx may be dy itself
+ * dtype REELS_HIP_F32, _BF16 or _F16. rows < 2^31, 0 < cols <= 2^30.
+ */
+int reels_hip_act8_keep(const void* x, int dtype, int64_t rows, int64_t cols, int8_t* codes,
+                        uint8_t* scales, void* stream);
+int reels_hip_act8_gelu_tanh(const void* x, int dtype, int64_t rows, int64_t cols, void* y,
+                             int8_t* codes, uint8_t* scales, void* stream);
+int reels_hip_act8_restore(const int8_t* codes, const uint8_t* scales, int dtype, int64_t rows,
+                           int64_t cols, void* x, void* stream);
+int reels_hip_act8_gelu_tanh_bwd(const int8_t* codes, const uint8_t* scales, const void* dy, int dtype,
+                                 int64_t rows, int64_t cols, void* dx, void* stream);
+
+/*
+ * Rows in microscaled 4 bits and their product. A value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign
+ * (codes 0 .. 7, the sign in bit 3) times 2^E, E shared by 32 neighbours of a row: the exponent of the
+ * block's largest magnitude after that is rounded to 2 significant bits, minus 2 (between -127 and 125);
+ * codes are the nearest values of x 2^-E, ties to the even code.
+ *   codes  [rows][Kp / 2], Kp = cols up to a multiple of 256: column 2 i in the low half of byte i, zeros
+ *          past cols
+ *   scales [ceil(rows / 64)][Kp / 256][512]: E + 127, or 255 where the block holds NaN or an infinity (its
+ *          values are NaN); block b (of 8) of row r (of 64) at (b % 2 * 32 + r % 32) * 8 + b / 2 * 2 + r / 32
+ * both 16-byte aligned, of the sizes that reels_hip_mx4_codes_bytes and reels_hip_mx4_scales_bytes give;
+ * rows < 2^31, cols < 2^24.
+ *   reels_hip_mx4_pack: rows ld_x elements apart (>= cols), any alignment of the element type
+ *   reels_hip_mx4_unpack: the values, dense, rounded to dtype (binary16: at most 65504)
+ *   reels_hip_mx4_linear: y[m][n] = rnd(act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]), x [M][K] and
+ *     w [N][K] in this form; bias [N], residual [M][N] (either NULL) and y [M][N] of dtype
+ *     REELS_HIP_F32, _BF16 or _F16; y may be residual itself; activation as in reels_hip_i8i8_linear.
+ *     Sums in f32, in an order that depends on M, N and K: bitwise reproducible for the same sizes.
+ */
+size_t reels_hip_mx4_codes_bytes(int64_t rows, int64_t cols);
+size_t reels_hip_mx4_scales_bytes(int64_t rows, int64_t cols);
+int reels_hip_mx4_pack(const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t cols,
+                       uint8_t* codes, uint8_t* scales, void* stream);
+int reels_hip_mx4_unpack(const uint8_t* codes, const uint8_t* scales, int dtype, int64_t rows,
+                         int64_t cols, void* y, void* stream);
+int reels_hip_mx4_linear(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w,
+                         const uint8_t* w_scales, const void* bias, const void* residual,
+                         int activation, int dtype, int64_t M, int64_t K, int64_t N, void* y,
+                         void* stream);
+
+/*
  * Kernel timing instrumentation. No counterpart in the reference (it has no profiler hooks);
  * used by benchmarks to time individual kernels with HIP events on the stream each kernel is
  * launched on. While enabled, every kernel the library enqueues is bracketed by two event

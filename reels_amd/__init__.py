@@ -4,6 +4,12 @@ The compute lives in libreels_hip.so (C ABI: include/reels_hip.h); this package 
 mirror of the reference layer API (src/layers/quantization.jl, lora.jl, linear.jl, attention.jl).
 """
 from ._lib import ReelsHIPError, ReelsHIPUnavailable, library_path  # noqa: F401
+from .activations import (  # noqa: F401
+    CompressedActivations,
+    GeluTanhCompressedFunction,
+    compress_activations,
+    gelu_tanh_compressed,
+)
 from .attention import (  # noqa: F401
     TiledAttentionCache,
     memory_efficient_attention,
@@ -34,6 +40,17 @@ from .layers import (  # noqa: F401
     quantize_frozen_matrix,
     set_adapter_enabled,
     workspace_bytes,
+)
+from .microscaled import MicroscaledMatrix, microscaled_linear, quantize_microscaled  # noqa: F401
+from .modulation import (  # noqa: F401
+    KeptRows,
+    ModulatedNormFunction,
+    ModulatedNormGradients,
+    ModulatedNormQuantized,
+    ModulatedNormResult,
+    modulated_norm,
+    modulated_norm_backward,
+    modulated_norm_quantized,
 )
 from .normalization import (  # noqa: F401
     RMSNormFunction,

@@ -60,6 +60,19 @@ EXPORTS = (
     "reels_hip_grad_workspace_bytes",
     "reels_hip_grad_norm",
     "reels_hip_clip_gradients",
+    "reels_hip_modulated_norm",
+    "reels_hip_modulated_norm_mx4",
+    "reels_hip_modulated_norm_workspace_bytes",
+    "reels_hip_modulated_norm_bwd",
+    "reels_hip_act8_keep",
+    "reels_hip_act8_gelu_tanh",
+    "reels_hip_act8_restore",
+    "reels_hip_act8_gelu_tanh_bwd",
+    "reels_hip_mx4_codes_bytes",
+    "reels_hip_mx4_scales_bytes",
+    "reels_hip_mx4_pack",
+    "reels_hip_mx4_unpack",
+    "reels_hip_mx4_linear",
     "reels_hip_trace_start",
     "reels_hip_trace_only",
     "reels_hip_trace_stop",
@@ -164,6 +177,31 @@ def lib():
     L.reels_hip_grad_norm.restype = ci
     L.reels_hip_clip_gradients.argtypes = [vp, vp, vp, vp, i64, cf, vp, vp, sz, vp]
     L.reels_hip_clip_gradients.restype = ci
+    rows = [vp, i64] * 5 + [ci, ci, i64, i64, i64, cf, ci]  # operands with their strides, sizes
+    L.reels_hip_modulated_norm.argtypes = rows + [vp] * 8
+    L.reels_hip_modulated_norm.restype = ci
+    L.reels_hip_modulated_norm_mx4.argtypes = rows + [vp] * 4
+    L.reels_hip_modulated_norm_mx4.restype = ci
+    L.reels_hip_modulated_norm_workspace_bytes.argtypes = [i64, i64, i64]
+    L.reels_hip_modulated_norm_workspace_bytes.restype = sz
+    L.reels_hip_modulated_norm_bwd.argtypes = [vp] * 6 + [vp, i64, vp, i64, vp, ci, ci, i64, i64, i64, ci] + [vp] * 6 + [sz, vp]
+    L.reels_hip_modulated_norm_bwd.restype = ci
+    L.reels_hip_act8_keep.argtypes = [vp, ci, i64, i64, vp, vp, vp]
+    L.reels_hip_act8_keep.restype = ci
+    L.reels_hip_act8_gelu_tanh.argtypes = [vp, ci, i64, i64, vp, vp, vp, vp]
+    L.reels_hip_act8_gelu_tanh.restype = ci
+    L.reels_hip_act8_restore.argtypes = [vp, vp, ci, i64, i64, vp, vp]
+    L.reels_hip_act8_restore.restype = ci
+    L.reels_hip_act8_gelu_tanh_bwd.argtypes = [vp, vp, vp, ci, i64, i64, vp, vp]
+    L.reels_hip_act8_gelu_tanh_bwd.restype = ci
+    for fn in (L.reels_hip_mx4_codes_bytes, L.reels_hip_mx4_scales_bytes):
+        fn.argtypes, fn.restype = [i64, i64], sz
+    L.reels_hip_mx4_pack.argtypes = [vp, i64, ci, i64, i64, vp, vp, vp]
+    L.reels_hip_mx4_pack.restype = ci
+    L.reels_hip_mx4_unpack.argtypes = [vp, vp, ci, i64, i64, vp, vp]
+    L.reels_hip_mx4_unpack.restype = ci
+    L.reels_hip_mx4_linear.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, i64, i64, i64, vp, vp]
+    L.reels_hip_mx4_linear.restype = ci
     L.reels_hip_trace_start.argtypes = [ctypes.c_int]
     L.reels_hip_trace_start.restype = ctypes.c_int
     L.reels_hip_trace_stop.restype = ctypes.c_int

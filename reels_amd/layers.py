@@ -209,6 +209,14 @@ def workspace_bytes(M: int, K: int, N: int, r: int, which: int,
     return int(L.reels_hip_i8lora_workspace_bytes(M, K, N, r, which))
 
 
+def _saved_x(x, dtype: torch.dtype, needed: bool) -> Optional[torch.Tensor]:
+    """The input of a linear as its backward takes it: activations kept in 8 bits
+    (CompressedActivations) become the tensor that they stand for, where the call reads it."""
+    if x is not None and not isinstance(x, torch.Tensor):
+        x = x.restore(dtype) if needed else None
+    return _contig(x, dtype, "x")
+
+
 def _on_device(weight: QuantizedMatrix, device) -> QuantizedMatrix:
     """An offloaded weight (codes in host memory, cpu_offload) is copied to the device for this
     call, as the reference's _materialize_weight does (quantization.jl:46-59)."""
@@ -294,7 +302,8 @@ def i8lora_backward(dy, x, weight: QuantizedMatrix, A=None, B=None, lora_scale=1
     A and B share one dtype, bfloat16, float16 or float32 (reels_hip_i8lora_bwd / _bwd_f16 /
     _bwd_f32); dx comes back in it. With want_dbias, a fourth result: the gradient of a trainable
     bias, dbias f32 [N] = sum over tokens of dy (reels_hip_i8lora_bwd_bias*), the pullback of the
-    forward's mixed_add (linear.jl:7-13; lora.jl:37-38, 64-67)."""
+    forward's mixed_add (linear.jl:7-13; lora.jl:37-38, 64-67). x may be CompressedActivations: its
+    values are restored for the call where it reads them."""
     if dy.dim() != 2:
         raise ValueError(f"dy must be a [M][N] matrix, got shape {tuple(dy.shape)}")
     M, N = dy.shape
@@ -311,7 +320,7 @@ def i8lora_backward(dy, x, weight: QuantizedMatrix, A=None, B=None, lora_scale=1
     weight = _on_activation_device(weight, dy.device)
     A = _contig(A, dt, "A")
     B = _contig(B, dt, "B")
-    x = _contig(x, dt, "x") if x is not None else None
+    x = _saved_x(x, dt, r > 0 and (want_dA or (want_dB and h is None)))
     h = _contig(h, dt, "h")
     dev = dy.device
     dx = torch.empty((M, K), dtype=dt, device=dev) if want_dx else None
@@ -340,8 +349,9 @@ def i8lora_backward_gelu(dy, x, gx, weight: QuantizedMatrix, A=None, B=None, lor
     """i8lora_backward of the projection after a GELU, with dx replaced by the GELU's pullback
     gelu_tanh_backward(gx, dx), gx [M][K] the GELU's input (reels_hip_i8lora_bwd_gelu*: in the
     dX GEMM's epilogue where that GEMM is unsplit, bit-identical to the two calls). Returns
-    (dgx, dA, dB), and dbias with want_dbias. float32 runs the two calls."""
-    if dy.dim() == 2 and dy.dtype == torch.float32:
+    (dgx, dA, dB), and dbias with want_dbias. float32 runs the two calls. x and gx may be
+    CompressedActivations (gx runs the two calls then)."""
+    if dy.dim() == 2 and (dy.dtype == torch.float32 or not isinstance(gx, (torch.Tensor, type(None)))):
         res = i8lora_backward(dy, x, weight, A, B, lora_scale, h, True, want_dA, want_dB, want_dbias)
         return (gelu_tanh_backward(gx, res[0]),) + tuple(res[1:])
     if dy.dim() != 2:
@@ -362,7 +372,7 @@ def i8lora_backward_gelu(dy, x, gx, weight: QuantizedMatrix, A=None, B=None, lor
     dy = dy.contiguous()
     weight = _on_activation_device(weight, dy.device)
     A, B, h, gx = _contig(A, dt, "A"), _contig(B, dt, "B"), _contig(h, dt, "h"), _contig(gx, dt, "gx")
-    x = _contig(x, dt, "x") if x is not None else None
+    x = _saved_x(x, dt, r > 0 and (want_dA or (want_dB and h is None)))
     dev = dy.device
     dx = torch.empty((M, K), dtype=dt, device=dev)
     dA = torch.empty((K, r), dtype=torch.float32, device=dev) if (want_dA and r) else None
@@ -520,17 +530,21 @@ def merged_weight(layer: LoRALinear) -> torch.Tensor:
 class I8LoRALinearFunction(torch.autograd.Function):
     """Autograd rule for lora_forward: the fused analogue of the reference's Zygote pullbacks
     (src/training/ad_rules.jl:53-80 for the frozen weight, Zygote's own rule for B*(A*z)).
-    Returns no gradient for the frozen weight, like NoTangent()."""
+    Returns no gradient for the frozen weight, like NoTangent(). kept: x in 8 bits
+    (compress_activations), saved in x's place; the projections of one x share it."""
 
     @staticmethod
-    def forward(ctx, x, A, B, values, scales, bias, lora_scale):
+    def forward(ctx, x, A, B, values, scales, bias, lora_scale, kept=None):
         weight = QuantizedMatrix(values, scales)
         # f32 master parameters with 16-bit activations: the kernels take rounded copies, the
         # gradients come back in f32 (the reference's AdamW keeps f32 state, optimizer.jl:9-24)
         Ac = A if A.dtype == x.dtype else A.to(x.dtype)
         Bc = B if B.dtype == x.dtype else B.to(x.dtype)
         y, h = i8lora_forward(x, weight, Ac, Bc, bias, lora_scale, save_h=True)
-        ctx.save_for_backward(x, Ac, Bc, values, scales, h)
+        if kept is not None and tuple(kept.shape) != tuple(x.shape):
+            raise ValueError(f"kept must have x's shape {tuple(x.shape)}, got {tuple(kept.shape)}")
+        saved = (x, None) if kept is None else (kept.values, kept.scales)
+        ctx.save_for_backward(*saved, Ac, Bc, values, scales, h)
         ctx.lora_scale = lora_scale
         ctx.param_dtypes = (A.dtype, B.dtype)
         ctx.bias_dtype = None if bias is None else bias.dtype
@@ -538,7 +552,10 @@ class I8LoRALinearFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, A, B, values, scales, h = ctx.saved_tensors
+        x, x_scales, A, B, values, scales, h = ctx.saved_tensors
+        if x_scales is not None:
+            from .activations import CompressedActivations
+            x = CompressedActivations(x, x_scales, dy.dtype)
         weight = QuantizedMatrix(values, scales)
         dy = dy.contiguous()
         # a trainable bias (LoRALinear train_bias): the pullback of mixed_add (linear.jl:7-13)
@@ -554,7 +571,7 @@ class I8LoRALinearFunction(torch.autograd.Function):
         # otherwise they take the parameter dtype
         ad, bd = ctx.param_dtypes
         return (dx, None if dA is None else dA.to(ad),
-                None if dB is None else dB.to(bd), None, None, dbias, None)
+                None if dB is None else dB.to(bd), None, None, dbias, None, None)
 
 
 def gelu_tanh(x: torch.Tensor) -> torch.Tensor:
@@ -567,7 +584,11 @@ def gelu_tanh(x: torch.Tensor) -> torch.Tensor:
     return y
 
 
-def gelu_tanh_backward(x: torch.Tensor, dy: torch.Tensor) -> torch.Tensor:
+def gelu_tanh_backward(x, dy: torch.Tensor) -> torch.Tensor:
+    """dy gelu_tanh'(x); x is the GELU's input, or what gelu_tanh_compressed kept of it."""
+    if not isinstance(x, torch.Tensor):
+        from .activations import _gelu_backward
+        return _gelu_backward(x, dy)
     dt = _act_dtype(x, "x")
     x = x.contiguous()
     dy = _contig(dy, dt, "dy")

@@ -1,0 +1,393 @@
+"""The modulated norm, its rows in 8 and 4 bits and its backward against the formulas in 64 bits. Bounds
+count f32 roundings (u = 2^-24). y: s - mean has 2 u, rstd and its product 2 u, 1 + scale u, the sum u. d:
+g = dy (1 + scale) 2 u, n 4 u; mean g and mean g n add chunks of at most eight terms in f32 (8 u) before
+they go on in 64 bits, and are rounded: 12 u and 18 u of the means of magnitudes; then three differences and
+products. Sums over rows follow each other in a thread, then over at most 4 groups, 32 slices and
+parts / 32 partial rows: 100 + rows / 64 roundings at most."""
+import pytest
+import torch
+
+from reels_amd import (CompressedActivations, ModulatedNormFunction, modulated_norm, modulated_norm_backward,
+                       modulated_norm_quantized, rms_norm)
+from tests._blocks import blocks4, blocks8, nibbles
+from tests._util import U, assert_within
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+EPS = 1e-6
+
+# samples, tokens, columns: one element, below and past a chunk, the forms of a wave and of a workgroup
+SIZES = [(1, 1, 1), (2, 3, 2), (1, 5, 7), (3, 11, 8), (2, 50, 101), (1, 17, 128), (2, 20, 256), (3, 3, 517), (2, 33, 1000),
+         (1, 64, 1536), (2, 7, 2049), (1, 5, 4096), (2, 3, 5120), (1, 5, 8193), (1, 3, 13824), (2, 2, 16384)]
+
+
+def make(B, S, C, dtype, mtype, kind, seed=0, dev="cuda"):
+    g = torch.Generator(device=dev).manual_seed(seed + B * 7 + S * 131 + C)
+    dt = DT[dtype]
+
+    def rnd(*s):
+        return torch.randn(s, generator=g, device=dev)
+    m = {"all": (C,), "sample": (B, C), "token": (B, S, C)}[kind]
+    t = dict(x=(rnd(B, S, C) * 1.5 + 2 * rnd(C)).to(dt), branch=rnd(B, S, C).to(dt), dy=rnd(B, S, C).to(dt),
+             dsum=rnd(B, S, C).to(dt))
+    return t, dict(gate=rnd(*m).to(DT[mtype]), scale=(0.3 * rnd(*m)).to(DT[mtype]), shift=rnd(*m).to(DT[mtype]))
+
+
+def rows(m, B):
+    return m[:, None, :] if m.dim() == 2 else m
+
+
+def unit(s, center, eps=EPS):
+    sd = s.double()
+    mean = sd.mean(-1, keepdim=True) if center else torch.zeros_like(sd[..., :1])
+    rstd = 1.0 / torch.sqrt((sd - mean).square().mean(-1, keepdim=True) + float(torch.tensor(eps)))
+    return sd, mean, rstd
+
+
+def check_forward(res, x, branch, gate, scale, shift, center, B):
+    if branch is None:
+        assert res.sum is x
+    else:
+        p = branch.float() if gate is None else rows(gate, B).float() * branch.float()
+        assert torch.equal(res.sum, (x.float() + p).to(x.dtype))
+    sd, mean, rstd = unit(res.sum, center)
+    st = res.stats.double()
+    mag = sd.abs().mean(-1)
+    assert bool(((st[..., 0] + st[..., 1] - mean[..., 0]).abs() <= 2.0 ** -40 * mag).all())
+    assert_within(res.stats[..., 2], rstd[..., 0], U * rstd[..., 0], "rstd")
+    n = (sd - mean) * rstd
+    up = 1.0 if scale is None else 1.0 + rows(scale, B).double()
+    y = n * up + (0.0 if shift is None else rows(shift, B).double())
+    assert_within(res.output, y, 7 * U * (n * up).abs() + U * y.abs(), "y")
+
+
+def check_backward(g, t, s, branch, stats, gate, scale, dsum, center, B, S):
+    C = t["dy"].shape[-1]
+    st = stats.double()
+    n = (s - (st[..., 0] + st[..., 1])[..., None]) * st[..., 2:]
+    rs = st[..., 2:]
+    up = torch.ones(C, dtype=torch.float64, device=s.device) if scale is None else 1.0 + rows(scale, B).double()
+    dy = t["dy"].double()
+    gd = dy * up
+    m0 = gd.mean(-1, keepdim=True) if center else 0.0
+    m1 = (gd * n).mean(-1, keepdim=True)
+    a0 = gd.abs().mean(-1, keepdim=True) if center else 0.0
+    a1 = (gd * n).abs().mean(-1, keepdim=True)
+    d = rs * (gd - m0 - n * m1)
+    slack = rs * U * (8 * gd.abs() + 16 * a0 + 28 * n.abs() * a1)
+    if dsum is not None:
+        d = d + dsum.double()
+        slack = slack + 2 * U * (dsum.double().abs() + d.abs())
+    assert_within(g.x, d, slack, "dx")
+    if gate is None:
+        assert g.branch is g.x
+    else:
+        gt = rows(gate, B).double()
+        assert_within(g.branch, d * gt, slack * gt.abs() + U * (d * gt).abs(), "dbranch")
+
+    def total(v, like):
+        return v if like.dim() == 3 else v.sum(1) if like.dim() == 2 else v.sum((0, 1))
+    deep = (100 + B * S / 64) * U
+    if scale is not None:
+        assert_within(g.scale, total(dy * n, scale), total(deep * (dy * n).abs(), scale), "dscale")
+        assert_within(g.shift, total(dy, scale), total(deep * dy.abs(), scale), "dshift")
+        assert g.scale.shape == scale.shape
+    if gate is not None and branch is not None:
+        assert_within(g.gate, total(d * branch, gate), total(slack * branch.abs() + deep * (d * branch).abs(), gate), "dgate")
+
+
+@pytest.mark.parametrize("dtype,mtype", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("B,S,C", SIZES)
+def test_forward_and_backward(dev, B, S, C, dtype, mtype):
+    for kind, center, compress in (("sample", True, False), ("token", False, False), ("all", True, True), ("sample", False, True),
+                                   ("token", True, True)):
+        t, m = make(B, S, C, dtype, mtype, kind)
+        r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], EPS, center, compress)
+        check_forward(r, t["x"], t["branch"], m["gate"], m["scale"], m["shift"], center, B)
+        s, b, sd, bd = r.sum, t["branch"], r.sum.double(), t["branch"].double()
+        if compress:
+            s, b = r.kept.sum, r.kept.branch
+            for k, of in ((s, r.sum), (b, t["branch"])):
+                q, sc, v = blocks8(of.double().reshape(-1, C))
+                assert torch.equal(k.values.reshape(-1, C), q) and torch.equal(k.scales.reshape(B * S, -1), sc)
+            sd, bd = (blocks8(v.reshape(-1, C))[2].reshape(B, S, C) for v in (sd, bd))
+        else:
+            assert r.kept is None
+        g = modulated_norm_backward(t["dy"], s, r.stats, m["scale"], b, m["gate"], t["dsum"], center)
+        check_backward(g, t, sd, bd, r.stats, m["gate"], m["scale"], t["dsum"], center, B, S)
+        again = modulated_norm_backward(t["dy"], s, r.stats, m["scale"], b, m["gate"], t["dsum"], center)
+        for u, v in zip(g, again):
+            assert torch.equal(u, v)
+        few = modulated_norm_backward(t["dy"], s, r.stats, m["scale"], None, m["gate"], t["dsum"], center, want_modulation=False)
+        assert few.gate is None and few.scale is None and torch.equal(few.x, g.x) and torch.equal(few.branch, g.branch)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("B,S,C", [(1, 5, 7), (2, 9, 300), (1, 3, 5120)])
+def test_parts_left_out(dev, B, S, C, dtype):
+    """No modulation, no gate, no branch, no other gradient."""
+    t, m = make(B, S, C, dtype, "f32", "sample")
+    for branch, gate, scale, dsum in ((None, None, None, None), ("branch", None, None, None), (None, None, "scale", "dsum"),
+                                      ("branch", "gate", None, "dsum"), ("branch", None, "scale", None)):
+        b, gt, sc, ds = (t.get(n, m.get(n)) if n else None for n in (branch, gate, scale, dsum))
+        sh = None if sc is None else m["shift"]
+        for compress in (False, True):
+            r = modulated_norm(t["x"], sc, sh, b, gt, EPS, True, compress)
+            check_forward(r, t["x"], b, gt, sc, sh, True, B)
+            s = r.kept.sum if compress else r.sum
+            sd = s.restore(torch.float32).double() if compress else s.double()
+            kb = b if b is None or not compress else r.kept.branch
+            bd = None if b is None else kb.restore(torch.float32).double() if compress else b.double()
+            g = modulated_norm_backward(t["dy"], s, r.stats, sc, kb, gt, ds, True)
+            check_backward(g, t, sd, bd, r.stats, gt, sc, ds, True, B, S)
+            assert (g.gate is None) == (gt is None) and (g.scale is None) == (sc is None)
+    if dtype != "f32" or C < 5000:
+        # without a mean and a modulation it is the root-mean-square norm
+        r, want = modulated_norm(t["x"], eps=EPS, center=False), rms_norm(t["x"], None, EPS)
+        assert_within(r.output, want.output.double(), 4 * U * want.output.double().abs()
+                      + torch.finfo(DT[dtype]).eps * want.output.double().abs(), "rms")
+
+
+@pytest.mark.parametrize("dtype,mtype", [("bf16", "f32"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("B,S,C", SIZES)
+def test_rows_in_4_bits(dev, B, S, C, dtype, mtype):
+    """Values in 64 bits rounded to f32, then their codes; a value whose 64-bit sum falls within 2^-45 of a
+    border may take either side, and a block whose largest does."""
+    for kind, center in (("sample", True), ("token", False)):
+        t, m = make(B, S, C, dtype, mtype, kind)
+        r = modulated_norm_quantized(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], EPS, center)
+        s = (t["x"].float() + rows(m["gate"], B).float() * t["branch"].float()).to(DT[dtype])
+        assert torch.equal(r.sum, s)
+        sd, mean, rstd = unit(s, center)
+        part, shift = (sd - mean) * rstd * (1.0 + rows(m["scale"], B).double()), rows(m["shift"], B).double()
+        y, mag = (part + shift).reshape(-1, C), (part.abs() + shift.abs()).reshape(-1, C)
+        c, sc, _ = blocks4(y.float().double())
+        near = torch.zeros_like(c, dtype=torch.bool)
+        for f in (-2.0 ** -45, 2.0 ** -45):  # codes that another sum of these values may give
+            cf, sf, _ = blocks4((y + f * mag).float().double())
+            near |= (cf != c) | (sf != sc).repeat_interleave(32, 1)[:, :C]
+        assert r.output.shape == (B * S, C) and r.output.compute_dtype == DT[dtype]
+        differ = nibbles(r.output) != c
+        assert not bool((differ & ~near).any()), int((differ & ~near).sum())
+        assert float(near.float().mean()) < 0.01 or C < 64
+        whole = torch.stack((r.output.codes & 15, r.output.codes >> 4), dim=-1).flatten(1)
+        assert not bool(whole[:, C:].any())
+
+
+def test_far_mean(dev):
+    """Rows whose mean is many times their spread keep their digits."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    for far in (1e3, 1e5):
+        x = (torch.randn(4, 1536, generator=g, device=dev).double() + far).float()
+        r = modulated_norm(x, eps=EPS)
+        sd, mean, rstd = unit(x, True)
+        n = (sd - mean) * rstd
+        assert_within(r.output, n, 6 * U * n.abs() + 2.0 ** -40 * far, "y")
+
+
+def test_large_and_small_values(dev):
+    """Squares past the f32 range and below it."""
+    for size in (1e30, 1e-25):
+        x = (torch.randn(3, 300, device=dev) * size)
+        r = modulated_norm(x, eps=0.0)
+        sd, mean, rstd = unit(x, True, 0.0)
+        n = (sd - mean) * rstd
+        assert_within(r.output, n, 8 * U * n.abs() + 2.0 ** -40, "y")
+
+
+def test_not_finite(dev):
+    """A row that holds NaN or an infinity is NaN, and so are its blocks; the others are as without it.
+    An infinite gate or scale stays in its own sample."""
+    t, m = make(2, 9, 300, "bf16", "f32", "sample")
+    x = t["x"].clone()
+    x[0, 3, 7], x[1, 5, 299] = float("nan"), float("inf")
+    a = modulated_norm(x, m["scale"], m["shift"], t["branch"], m["gate"])
+    b = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+    bad = torch.zeros(2, 9, dtype=torch.bool, device=dev)
+    bad[0, 3] = bad[1, 5] = True
+    assert torch.isnan(a.output[bad]).all() and torch.equal(a.output[~bad], b.output[~bad])
+    q = modulated_norm_quantized(x, m["scale"], m["shift"], t["branch"], m["gate"]).output.dequantize().view(2, 9, 300)
+    p = modulated_norm_quantized(t["x"], m["scale"], m["shift"], t["branch"], m["gate"]).output.dequantize().view(2, 9, 300)
+    assert torch.isnan(q[bad]).all() and torch.equal(q[~bad], p[~bad])
+    g = modulated_norm_backward(t["dy"], a.sum, a.stats, m["scale"], t["branch"], m["gate"], t["dsum"])
+    w = modulated_norm_backward(t["dy"], b.sum, b.stats, m["scale"], t["branch"], m["gate"], t["dsum"])
+    assert torch.isnan(g.x[bad]).all() and torch.equal(g.x[~bad], w.x[~bad])
+    gate = m["gate"].clone()
+    gate[1, 0] = float("inf")
+    c = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], gate)
+    assert torch.equal(c.output[0], b.output[0]) and torch.isnan(c.output[1]).all()
+    scale = m["scale"].clone()
+    scale[1, 0] = float("inf")
+    c = modulated_norm(t["x"], scale, m["shift"], t["branch"], m["gate"])
+    assert torch.equal(c.output[0], b.output[0]) and torch.equal(c.output[1, :, 1:], b.output[1, :, 1:])
+
+
+def test_strides_and_slices(dev):
+    """The modulations as slices of one projection, rows of wider buffers, odd addresses, expanded rows."""
+    B, S, C = 3, 20, 258
+    g = torch.Generator(device=dev).manual_seed(9)
+    six = torch.randn(B, 6, C, generator=g, device=dev)
+    x, br, dy = (torch.randn(B, S, C, generator=g, device=dev).bfloat16() for _ in range(3))
+    sh, sc, gt = (six[:, i:i + 1] for i in (0, 1, 5))
+
+    def both(*mods, x=x, br=br):
+        a = modulated_norm(x, mods[0], mods[1], br, mods[2])
+        d = modulated_norm_backward(dy.view_as(a.output), a.sum, a.stats, mods[0], br, mods[2])
+        return [t.reshape(-1) for t in (a.output, a.sum) + tuple(d)]
+    want = both(sc.reshape(B, C).clone(), sh.reshape(B, C).clone(), gt.reshape(B, C).clone())
+    for u, v in zip(both(sc, sh, gt), want):
+        assert torch.equal(u, v)
+    each = [t.expand(B, S, C) for t in (sc, sh, gt)]
+    for u, v in zip(both(*each)[:4], want):
+        assert torch.equal(u, v)
+    tokens = torch.randn(B, S, 6, C, generator=g, device=dev)
+    mods = [tokens[:, :, i] for i in range(3)]
+    for u, v in zip(both(*mods), both(*[t.clone() for t in mods])):
+        assert torch.equal(u, v)
+    wide = torch.randn(B * S, C + 6, generator=g, device=dev).bfloat16()
+    wide[:, 3:3 + C] = x.view(-1, C)
+    flat = torch.cat([br.reshape(-1)[:1], br.reshape(-1)])[1:].view(B * S, C)
+    one = [t[0].reshape(C) for t in (sc, sh, gt)]
+    for u, v in zip(both(*one, x=wide[:, 3:3 + C], br=flat), both(*one, x=x.reshape(-1, C), br=br.reshape(-1, C))):
+        assert torch.equal(u, v)
+    mixed = modulated_norm(x.transpose(0, 1), one[0], one[1], br.transpose(0, 1), one[2])
+    assert torch.equal(mixed.output, modulated_norm(x.transpose(0, 1).contiguous(), one[0], one[1],
+                                                    br.transpose(0, 1).contiguous(), one[2]).output)
+
+
+def test_over_the_inputs(dev):
+    """The sum over x or the branch, dx over dy or the other gradient: what the C entries allow."""
+    from reels_amd import _lib
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for B, S, C in ((2, 9, 300), (1, 7, 5125)):
+        t, m = make(B, S, C, "bf16", "f32", "sample")
+        r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+        want = modulated_norm_backward(t["dy"], r.sum, r.stats, m["scale"], None, m["gate"], t["dsum"], want_modulation=False)
+        p = {n: v.data_ptr() for n, v in m.items()}
+        for over in ("x", "branch"):
+            c = {n: v.clone() for n, v in t.items()}
+            y, stats = torch.empty_like(r.output), torch.empty_like(r.stats)
+            assert L.reels_hip_modulated_norm(c["x"].data_ptr(), C, c["branch"].data_ptr(), C, p["gate"], C, p["scale"], C, p["shift"],
+                                              C, 0, 1, B * S, C, S, EPS, 1, c[over].data_ptr(), y.data_ptr(), stats.data_ptr(),
+                                              None, None, None, None, st) == 0
+            assert torch.equal(c[over], r.sum) and torch.equal(y, r.output) and torch.equal(stats, r.stats)
+        for over in ("dy", "dsum"):
+            c = {n: v.clone() for n, v in t.items()}
+            db = torch.empty_like(r.output)
+            assert L.reels_hip_modulated_norm_bwd(c["dy"].data_ptr(), r.sum.data_ptr(), None, c["dsum"].data_ptr(), None, None,
+                                                  p["gate"], C, p["scale"], C, r.stats.data_ptr(), 0, 1, B * S, C, S, 1,
+                                                  c[over].data_ptr(), db.data_ptr(), None, None, None, None, 0, st) == 0
+            assert torch.equal(c[over], want.x) and torch.equal(db, want.branch)
+
+
+def test_many_rows(dev):
+    """Groups whose sums run over many workgroups, and many small groups."""
+    for B, S, C, kind in [(1, 5000, 130, "sample"), (3, 1111, 515, "sample"),
+                          (700, 3, 64, "sample"), (700, 2, 64, "all")]:
+        t, m = make(B, S, C, "f32", "f32", kind)
+        r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+        g = modulated_norm_backward(t["dy"], r.sum, r.stats, m["scale"], t["branch"], m["gate"], t["dsum"])
+        check_backward(g, t, r.sum.double(), t["branch"].double(), r.stats, m["gate"], m["scale"], t["dsum"], True, B, S)
+
+
+def test_empty(dev):
+    for shape in ((0, 5, 40), (3, 0, 40), (0, 40)):
+        x = torch.empty(shape, device=dev)
+        mod = [torch.randn(40, device=dev) for _ in range(3)]
+        r = modulated_norm(x, mod[0], mod[1], x, mod[2], compress=True)
+        assert r.output.shape == shape and r.kept.sum.shape == shape
+        assert modulated_norm_quantized(x, mod[0], mod[1]).output.shape == (0, 40)
+        g = modulated_norm_backward(x, r.sum, r.stats, mod[0], x, mod[2])
+        assert g.x.shape == shape and not g.scale.any() and not g.shift.any() and not g.gate.any()
+    x = torch.empty(3, 0, 40, device=dev)
+    g = modulated_norm_backward(x, x, torch.empty(3, 0, 3, device=dev), torch.randn(3, 40, device=dev))
+    assert g.scale.shape == (3, 40) and not g.scale.any() and not g.shift.any()
+
+
+def test_autograd(dev):
+    """Against torch's own gradients of the formula in 64 bits."""
+    for kind, compress in (("sample", False), ("token", False), ("all", True)):
+        t, m = make(2, 6, 100, "f32", "f32", kind, seed=3)
+        leaves = [t["x"], m["scale"], m["shift"], t["branch"], m["gate"]]
+        leaves = [v.clone().requires_grad_() for v in leaves]
+        y, s = ModulatedNormFunction.apply(*leaves, EPS, True, compress)
+        grads = torch.autograd.grad((y, s), leaves, (t["dy"], t["dsum"]))
+        wide = [v.detach().double().requires_grad_() for v in leaves]
+        sd = wide[0] + rows(wide[4], 2) * wide[3]
+        c = sd - sd.mean(-1, keepdim=True)
+        yd = c * torch.rsqrt(c.square().mean(-1, keepdim=True) + EPS) * (1 + rows(wide[1], 2)) + rows(wide[2], 2)
+        want = torch.autograd.grad((yd, sd), wide, (t["dy"].double(), t["dsum"].double()))
+        # f32, or a backward from 7 bits: a step of the block's largest is 2^-6 of it at most
+        tol = 2.0 ** -5 if compress else 1e-5
+        for a, b in zip(grads, want):
+            assert a.shape == b.shape
+            assert float((a.double() - b).norm() / b.norm()) < tol
+        only = torch.autograd.grad(ModulatedNormFunction.apply(*leaves, EPS, True, compress)[1], leaves, t["dsum"])
+        assert torch.equal(only[0], t["dsum"]) and not only[1].any() and not only[2].any()
+    x = t["x"].clone().requires_grad_()
+    y = ModulatedNormFunction.apply(x, None, None, None, None)
+    torch.autograd.grad(y.sum(), x)
+    with pytest.raises(RuntimeError):
+        (d,) = torch.autograd.grad(ModulatedNormFunction.apply(x, None, None, None, None).sum(), x, create_graph=True)
+        torch.autograd.grad(d.sum(), x)
+
+
+def test_differences(dev):
+    """The gradient along a direction against differences of the forward."""
+    t, m = make(2, 5, 70, "f32", "f32", "sample", seed=8)
+    names = ("x", "scale", "shift", "branch", "gate")
+    at = {**t, **m}
+    g = torch.Generator(device=dev).manual_seed(1)
+    dirs = {n: torch.randn(at[n].shape, generator=g, device=dev) for n in names}
+
+    def value(h):
+        v = {n: at[n] + h * dirs[n] for n in names}
+        r = modulated_norm(v["x"], v["scale"], v["shift"], v["branch"], v["gate"])
+        return float((r.output.double() * t["dy"].double()).sum() + (r.sum.double() * t["dsum"].double()).sum())
+    r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+    d = modulated_norm_backward(t["dy"], r.sum, r.stats, m["scale"], t["branch"], m["gate"], t["dsum"])
+    got = sum(float((getattr(d, n).double() * dirs[n].double()).sum()) for n in names)
+    h = 1e-2
+    # the error of the fourth-order difference is h^4 times a fifth derivative of order one per term
+    want = (8 * (value(h) - value(-h)) - (value(2 * h) - value(-2 * h))) / (12 * h)
+    assert abs(got - want) < 2e-3 * max(1.0, abs(want)), (got, want)
+
+
+def test_other_stream_and_graph(dev):
+    t, m = make(2, 300, 1000, "bf16", "f32", "sample")
+
+    def step():
+        r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], compress=True)
+        g = modulated_norm_backward(t["dy"], r.kept.sum, r.stats, m["scale"], r.kept.branch, m["gate"], t["dsum"])
+        q = modulated_norm_quantized(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+        return [r.output, r.sum, q.output.dequantize()] + list(g)
+    want = step()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = step()
+    torch.cuda.current_stream().wait_stream(st)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs = []
+    for _ in range(2):  # two graphs, each with its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, step()))
+    for i in range(3):
+        for v in t.values():
+            v.copy_(torch.randn_like(v))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_kept_rows_of_another_shape(dev):
+    t, m = make(2, 6, 64, "bf16", "f32", "sample")
+    r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], compress=True)
+    with pytest.raises(ValueError, match="both"):
+        modulated_norm_backward(t["dy"], r.kept.sum, r.stats, m["scale"], t["branch"], m["gate"])
+    with pytest.raises(ValueError, match="shape"):
+        modulated_norm_backward(t["dy"], CompressedActivations(r.kept.sum.values[:1], r.kept.sum.scales[:1]), r.stats)
