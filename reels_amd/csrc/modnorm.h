@@ -1,54 +1,131 @@
 // What the forward and the backward of the modulated norm share.
 #pragma once
 #include "microscale.h"
-#include "rows.h"
 
 namespace reels {
 
-struct ModForm { int tpr, nch; };
+// Who has a row: a wave (tpr 64, four rows to a workgroup; rows of up to 512 elements), or a workgroup of
+// `threads` (tpr 0) with nch chunks of 16 bytes a thread. 8 elements a thread up to four waves (three waves
+// at 1536 leave no lane idle), then 16, up to 16 waves.
+struct ModForm { int tpr, nch, threads; };
+constexpr int64_t kModCols = 16384;  // the longest row
+inline ModForm mod_form(int elt, int64_t cols) {
+  const int64_t waves = ceil_div(cols, 512);
+  const int per = elt == REELS_HIP_F32 ? 2 : 1;
+  if (waves <= 1) return {64, per, 256};
+  if (waves <= 4) return {0, per, (int)waves * 64};
+  return {0, 2 * per, (int)ceil_div(waves, 2) * 64};
+}
+// How the chunks of a row fall on its threads: every thread has whole ones, or some have a part or none, or
+// the row is shorter than a chunk
+enum ModKind { kEven = 0, kAny = 1, kTiny = 2 };
+
+// calls g(tpr, nch, most threads of a workgroup, kind) as integral constants
+template <int N> using ModInt = std::integral_constant<int, N>;
+template <int ELT, typename F> void with_mod_form(ModForm f, int64_t cols, F&& g) {
+  constexpr int P = ELT == REELS_HIP_F32 ? 2 : 1, V = Chunk<ELT>::V;
+  auto kind = [&](auto tpr, auto nch, auto nt) {
+    if (cols == (int64_t)(f.tpr == 0 ? f.threads : 64) * f.nch * V) g(tpr, nch, nt, ModInt<kEven>{});
+    else g(tpr, nch, nt, ModInt<kAny>{});
+  };
+  if (cols < V) g(ModInt<64>{}, ModInt<P>{}, ModInt<256>{}, ModInt<kTiny>{});
+  else if (f.tpr == 64) kind(ModInt<64>{}, ModInt<P>{}, ModInt<256>{});
+  else if (f.nch == P) kind(ModInt<0>{}, ModInt<P>{}, ModInt<256>{});
+  else if (f.threads <= 512) kind(ModInt<0>{}, ModInt<2 * P>{}, ModInt<512>{});
+  else kind(ModInt<0>{}, ModInt<2 * P>{}, ModInt<1024>{});
+}
 
 namespace {
 
-// Threads of a row and its chunks a thread: a wave up to 256 chunks, 256 threads up to 1024, and 512 (f32:
-// 1024 past 2048 chunks) up to 16384 elements, the longest row.
-constexpr int64_t kModCols = 16384;
-inline ModForm mod_form(int elt, int64_t cols) {
-  const int64_t chunks = ceil_div(cols, 16 / elt_bytes(elt));
-  for (int tpr : {64, 256, 512})
-    if (chunks <= 4 * tpr) return {tpr, (int)ceil_div(chunks, tpr)};
-  return {1024, (int)ceil_div(chunks, 1024)};
-}
-template <int ELT, typename F> void with_mod_form(ModForm f, F&& g) {
-  auto some = [&](auto tpr) {
-    if (f.nch == 2) g(tpr, Int<2>{});
-    else if (f.nch == 3) g(tpr, Int<3>{});
-    else g(tpr, Int<4>{});
-  };
-  switch (f.tpr) {
-    case 64:
-      if (f.nch == 1) g(Int<64>{}, Int<1>{});
-      else some(Int<64>{});
-      break;
-    case 256: some(Int<256>{}); break;
-    case 512:
-      if (f.nch == 3) g(Int<512>{}, Int<3>{});
-      else g(Int<512>{}, Int<4>{});
-      break;
-    default:
-      if constexpr (ELT == REELS_HIP_F32) {
-        if (f.nch == 3) g(Int<1024>{}, Int<3>{});
-        else g(Int<1024>{}, Int<4>{});
-      }
-      break;
+// a and b summed over a row's threads in 64 bits: a wave's, or a workgroup's of at most 16 waves through LDS,
+// wave by wave in one order. slots: one of two in turn, so that a wave may enter the next row's sums while
+// another still reads this one's. The barrier leaves loads in flight.
+template <int TPR> __device__ __forceinline__ void row_sums(double& a, double& b, double (&slots)[16][2]) {
+  a = group_reduce<64, false>(a);
+  b = group_reduce<64, false>(b);
+  if constexpr (TPR == 0) {
+    if ((threadIdx.x & 63) == 0) {
+      slots[threadIdx.x >> 6][0] = a;
+      slots[threadIdx.x >> 6][1] = b;
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int i = threadIdx.x & 15;
+    const bool in = i < (int)(blockDim.x >> 6);
+    a = group_reduce<16, false>(in ? slots[i][0] : 0.0);
+    b = group_reduce<16, false>(in ? slots[i][1] : 0.0);
   }
 }
 
-// Modulations: [groups][cols] rows ld elements apart, f32 or the rows' type. A thread's values of a chunk
-// that it has not are those of another one.
-template <typename R, int N, int V>
-__device__ __forceinline__ void load_mod(const R& at, const void* p, int64_t ld, int f32, int64_t group, float (&f)[N][V]) {
-  at.load_w((const uint8_t*)p + group * ld * (f32 ? 4 : R::EB), f32, f);
-}
+// A thread's chunks of a row: chunk i at element col(i). They are read without a branch, so that all loads of
+// a row are in flight together: a thread without a chunk reads the row's first one, and where the row's
+// length is no multiple of V its last V elements stand for the partial chunk; `trim` puts that right once the
+// data is there, in the waves that have such threads. Rows shorter than a chunk are
+// read by elements.
+template <int ELT, int TPR, int NCH, int KIND> struct ModRow {
+  static constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
+  int cols, lane, base;
+  __device__ __forceinline__ static int threads() {
+    if constexpr (TPR == 0) return (int)blockDim.x;
+    else return TPR;
+  }
+  __device__ __forceinline__ explicit ModRow(int64_t n) : cols((int)n) {
+    lane = TPR == 0 ? threadIdx.x : threadIdx.x % 64;
+    base = TPR == 0 ? __builtin_amdgcn_readfirstlane(lane & ~63) : 0;
+  }
+  __device__ __forceinline__ int col(int i) const { return (lane + threads() * i) * V; }
+  __device__ __forceinline__ int left(int i) const { return cols - col(i); }
+  // of the whole wave, in scalar registers: whether a lane has a chunk i, and whether all have whole ones
+  __device__ __forceinline__ bool some(int i) const { return KIND == kEven || (base + threads() * i) * V < cols; }
+  __device__ __forceinline__ bool all(int i) const {
+    return KIND == kEven || (KIND == kAny && (base + threads() * i + 64) * V <= cols);
+  }
+  __device__ __forceinline__ void load(const void* row, Chunk<ELT> (&d)[NCH]) const {
+    const uint8_t* p = (const uint8_t*)row;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int l = left(i);
+      if constexpr (KIND == kTiny) {
+        d[i].zero();
+        if (l > 0) d[i].load(p + (int64_t)col(i) * EB, l);
+      } else {
+        const int at = KIND == kEven || l >= V ? col(i) : l > 0 ? cols - V : 0;
+        d[i].d = load_any<u32x4>((const typename Store<ELT>::raw*)(p + (uint32_t)(at * EB)));  // 32-bit offsets from a scalar base
+      }
+    }
+  }
+  __device__ __forceinline__ void trim(Chunk<ELT> (&d)[NCH]) const {
+    if constexpr (KIND != kAny) return;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (all(i)) continue;
+      const int l = left(i);
+      const unsigned __int128 u = __builtin_bit_cast(unsigned __int128, d[i].d);
+      if (l < V) d[i].d = __builtin_bit_cast(u32x4, l > 0 ? u >> (8 * EB * (V - l)) : (unsigned __int128)0);
+    }
+  }
+  __device__ __forceinline__ void store(void* row, int i, const Chunk<ELT>& d) const {
+    uint8_t* p = (uint8_t*)row + (uint32_t)(col(i) * EB);
+    if (all(i)) store_any((typename Store<ELT>::raw*)p, d.d);
+    else if (left(i) > 0) d.store(p, left(i));
+  }
+  // the same in f32
+  __device__ __forceinline__ void store(float* row, int i, const float (&f)[V]) const {
+    if (all(i)) store_vec<REELS_HIP_F32, V>(row + (uint32_t)col(i), V, f);
+    else if (left(i) > 0) store_vec<REELS_HIP_F32, V>(row + (uint32_t)col(i), left(i), f);
+  }
+  // a row of modulations in f32 (or the rows' type), zeros where the thread has no element
+  __device__ __forceinline__ void mods(const void* p, int64_t ld, int f32, int64_t group, float (&f)[NCH][V]) const {
+    const uint8_t* r = (const uint8_t*)p + group * ld * (f32 ? 4 : EB);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int l = all(i) ? V : left(i) > 0 ? left(i) : 0, at = l > 0 ? col(i) : 0;
+      if (f32) load_vec<REELS_HIP_F32, V>((const float*)r + (uint32_t)at, l, f[i]);
+      else load_vec<ELT, V>(r + (uint32_t)(at * EB), l, f[i]);
+    }
+  }
+};
 
 inline int mod_check(const char* fn, int dtype, int m_dtype, int64_t rows, int64_t cols, int64_t rpg) {
   if (!known_elt(dtype) || (m_dtype != dtype && m_dtype != REELS_HIP_F32))

@@ -8,10 +8,9 @@
 //   kept: s and b as 8-bit blocks for the backward;  4 bits: y's row as 4-bit blocks instead of y
 //
 // gate, scale and shift have one row for each group of rows (a sample's tokens, or a single token).
-// Bound by memory: x and b are read once, s and y written once, the row stays in registers between the two
-// reductions (the mean first, then the squares about it: with rows far from zero the difference of two large
-// sums would lose the variance). Both are summed in 64 bits; the mean is kept as two f32 values, so that
-// s - mean loses nothing where the mean is many times the spread. Rows in 4 bits are formed in 64 bits and
+// Bound by memory: x and b are read once, s and y written once, the row stays in registers in between. Sums
+// are in 64 bits about the row's first element, which one pass over the row can take; the mean is kept as two
+// f32 values, so that s - mean loses nothing where the mean is many times the spread. Rows in 4 bits are formed in 64 bits and
 // rounded to f32 before their codes are taken, so a code does not depend on the order of f32 operations.
 #include "modnorm.h"
 
@@ -42,129 +41,168 @@ __device__ __forceinline__ void keep_chunk(const float (&f)[V], int8_t* codes, u
   if (col % kMxBlock == 0) scales[row * ((cols + kMxBlock - 1) / kMxBlock) + col / kMxBlock] = (uint8_t)byte;
 }
 
-// MODE 0: y; 1: y and the kept rows; 2: y's rows in 4 bits
-template <int ELT, int TPR, int NCH, int MODE>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void mod_kernel(ModArgs a) {
-  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), NT = TPR < 256 ? 256 : TPR;
-  __shared__ double slots[2][NT / 64];
-  // rows in 4 bits: neighbours share lines of scale bytes, so each XCD takes a run of rows
-  unsigned wg = blockIdx.x;
-  if constexpr (MODE == 2) {
-    const unsigned n = gridDim.x, xcd = wg & 7;
-    wg = xcd * (n >> 3) + (xcd < (n & 7) ? xcd : n & 7) + (wg >> 3);
-  }
-  const int64_t row0 = (int64_t)wg * (NT / TPR) + threadIdx.x / TPR;
-  const Row<ELT, TPR, NCH> at(a.cols, row0 < a.rows);
-  const int64_t row = at.live ? row0 : a.rows - 1;
-  const int64_t group = (uint32_t)row / (uint32_t)a.rpg;
-  Chunk<ELT> s[NCH], b[NCH];
-  float m[NCH][V];
-  at.load((const uint8_t*)a.x + row * a.ld_x * EB, s);
-  if (a.branch != nullptr) {
-    at.load((const uint8_t*)a.branch + row * a.ld_b * EB, b);
-    if (a.gate != nullptr) load_mod(at, a.gate, a.ld_gate, a.m_f32, group, m);
-  }
-  double t = 0.0;
+// MODE 0: y; 1: y and the kept rows; 2: y's rows in 4 bits. A wave or workgroup walks `run` rows one after the
+// other, the next row's x and b on their way meanwhile; the modulations stay in registers while the group is the
+// same (as f32 they are half again what a row reads from memory).
+template <int ELT, int TPR, int NCH, int NT, int KIND, int MODE>
+__global__ __launch_bounds__(NT) void mod_kernel(ModArgs a, uint32_t run) {
+  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
+  __shared__ double slots[2][16][2];
+  const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
+  // rows in 32 bits, so that they and what follows from them stay in scalar registers
+  const uint32_t begin = TPR == 0 ? blockIdx.x : blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t end = (uint32_t)a.rows, rpg = (uint32_t)a.rpg;
+  if (begin >= end) return;
+  // A row's operands on their way; raw: its first elements, which every thread needs. All loads are
+  // unconditional, so that the waits for them need not count on the fewest: where there is no branch x takes
+  // its place, past the last row the last one.
+  typedef typename Store<ELT>::raw raw;
+  struct Data { Chunk<ELT> x[NCH], b[NCH]; raw x0, b0; };
+  const void* branch = a.branch != nullptr ? a.branch : a.x;
+  const int64_t ld_b = a.branch != nullptr ? a.ld_b : a.ld_x;
+  auto load = [&](uint32_t r, Data& d) {
+    const int64_t row = r < end ? r : end - 1;
+    at.load((const uint8_t*)a.x + row * a.ld_x * EB, d.x);
+    at.load((const uint8_t*)branch + row * ld_b * EB, d.b);
+    d.x0 = ((const raw*)a.x)[row * a.ld_x];
+    d.b0 = ((const raw*)branch)[row * ld_b];
+  };
+  Data cur, next;
+  load(begin, cur);
+  float gate[NCH][V], up[NCH][V], shift[NCH][V], gate0 = 1.0f;
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    if (!at.some(i)) continue;
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      gate[i][j] = 1.0f;
+      up[i][j] = shift[i][j] = 0.0f;
+    }
+  uint32_t change = begin;
+  int turn = 0;
+  for (uint32_t r = begin; r < end; r += run, turn ^= 1) {
+    const int64_t row = r;
+    if (r >= change) {
+      const uint32_t group = r / rpg;
+      change = (group + 1) * rpg;
+      if (a.gate != nullptr) {
+        at.mods(a.gate, a.ld_gate, a.m_f32, group, gate);
+        gate0 = a.m_f32 ? ((const float*)a.gate)[(int64_t)group * a.ld_gate] : Store<ELT>::get(((const raw*)a.gate)[(int64_t)group * a.ld_gate]);
+      }
+      if (a.scale != nullptr) {
+        at.mods(a.scale, a.ld_scale, a.m_f32, group, up);
+        at.mods(a.shift, a.ld_shift, a.m_f32, group, shift);
+      }
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // here, and not at each row's use
+    }
+    load(r + run, next);
+    // the sum, and its first element, which every thread forms for itself
+    Chunk<ELT>(&s)[NCH] = cur.x;  // no branch: the row itself
+    float s0 = Store<ELT>::get(cur.x0);
+    at.trim(s);
     if (a.branch != nullptr) {
-      float f[V];
-      {
 #pragma clang fp contract(off)
+      at.trim(cur.b);
+      s0 = Store<ELT>::get(Store<ELT>::put(s0 + gate0 * Store<ELT>::get(cur.b0)));
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        float f[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float p = a.gate != nullptr ? m[i][j] * b[i].get(j) : b[i].get(j);
+          const float p = gate[i][j] * cur.b[i].get(j);
           f[j] = s[i].get(j) + p;
         }
+        s[i].pack(f);
+        at.store((uint8_t*)a.sum + row * a.cols * EB, i, s[i]);
       }
-      // a lane without a chunk holds zeros in x and b; its gate is another's and may be infinite
-      if (!at.full(i)) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = at.live && j < at.left(i) ? f[j] : 0.0f;
-      }
-      s[i].pack(f);
-      at.store((uint8_t*)a.sum + row * a.cols * EB, i, s[i]);
       if constexpr (MODE == 1) {
         if (a.kb != nullptr) {
-          b[i].unpack(f);
-          keep_chunk<V>(f, a.kb, a.kbs, row, at.live ? at.col(i) : at.cols, at.cols);
+#pragma unroll
+          for (int i = 0; i < NCH; ++i) {
+            if (!at.some(i)) continue;
+            float f[V];
+            cur.b[i].unpack(f);
+            keep_chunk<V>(f, a.kb, a.kbs, row, at.col(i), at.cols);
+          }
         }
       }
     }
     if constexpr (MODE == 1) {
-      float f[V];
-      s[i].unpack(f);
-      keep_chunk<V>(f, a.ks, a.kss, row, at.live ? at.col(i) : at.cols, at.cols);
-    }
 #pragma unroll
-    for (int j = 0; j < V; ++j) t += (double)s[i].get(j);
-    s[i].hold();
-  }
-  double mean = 0.0;
-  if (a.center) mean = row_reduce<TPR, false>(t, slots[0]) * a.per_col;
-  double ss = 0.0;
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    if (!at.some(i)) continue;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const double d = (double)s[i].get(j) - mean;
-      if (at.full(i) || (at.part(i) && j < at.left(i))) ss = fma(d, d, ss);
-    }
-    s[i].hold();
-  }
-  ss = row_reduce<TPR, false>(ss, slots[1]);
-  const double rstd = rsqrt64(fma(ss, a.per_col, (double)a.eps));
-  const float hi = (float)mean, lo = (float)(mean - (double)hi), rs = (float)rstd;
-  float h[NCH][V];
-  if (a.scale != nullptr) {
-    load_mod(at, a.scale, a.ld_scale, a.m_f32, group, m);
-    load_mod(at, a.shift, a.ld_shift, a.m_f32, group, h);
-  } else {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) m[i][j] = h[i][j] = 0.0f;
-  }
-  if constexpr (MODE < 2) {
-    if (at.live && at.lane == 0) {
-      float* st = a.stats + row * 3;
-      st[0] = hi;
-      st[1] = lo;
-      st[2] = rs;
-    }
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if (!at.some(i)) continue;
-      float y[V];
-      Chunk<ELT> o;
-#pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = fmaf((s[i].get(j) - hi - lo) * rs, 1.0f + m[i][j], h[i][j]);
-      o.pack(y);
-      at.store((uint8_t*)a.y + row * a.cols * EB, i, o);
-    }
-  } else {
-    const int tiles = (at.cols + 255) / 256;
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if (!at.some(i)) continue;
-      float y[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const double n = ((double)s[i].get(j) - mean) * rstd;
-        y[j] = (float)fma(n, 1.0 + (double)m[i][j], (double)h[i][j]);
-        if (!at.full(i)) y[j] = j < at.left(i) ? y[j] : 0.0f;  // zeros up to the tile's end
+      for (int i = 0; i < NCH; ++i) {
+        if (!at.some(i)) continue;
+        float f[V];
+        s[i].unpack(f);
+        keep_chunk<V>(f, a.ks, a.kss, row, at.col(i), at.cols);
       }
-      const uint32_t byte = mx_exponent<2>(mx_top<kMxBlock / V>(mx_top_of<V>(y)));
-      const int col = at.col(i);
-      if (!at.live || col >= tiles * 256) continue;
-      const uint32_t word = mx4_codes<V>(y, byte);
-      uint8_t* p = a.codes + row * tiles * 128 + col / 2;
-      if constexpr (V == 8) *reinterpret_cast<uint32_t*>(p) = word;
-      else *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
-      if (col % kMxBlock == 0) a.scales[mx4_scale_at(row, col / kMxBlock, tiles)] = (uint8_t)byte;
     }
+    // Sums of s - s0 and of its square in one pass. s0 is one of the row's elements, at most sqrt(cols)
+    // times the spread from the mean, so the difference of the two sums loses at most log2(cols) bits of 53.
+    const double pivot = a.center ? (double)s0 : 0.0;
+    double sum = 0.0, sq = 0.0;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (at.all(i)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double d = (double)s[i].get(j) - pivot;
+          sum += d;
+          sq = fma(d, d, sq);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double d = j < at.left(i) ? (double)s[i].get(j) - pivot : 0.0;
+          sum += d;
+          sq = fma(d, d, sq);
+        }
+      }
+      s[i].hold();
+    }
+    row_sums<TPR>(sum, sq, slots[turn]);
+    const double off = a.center ? sum * a.per_col : 0.0, mean = pivot + off;
+    const double var = fmax(fma(-off, off, sq * a.per_col), 0.0) + (sum - sum);  // NaN stays
+    const double rstd = rsqrt64(var + (double)a.eps);
+    if constexpr (MODE < 2) {
+      const float hi = (float)mean, lo = (float)(mean - (double)hi), rs = (float)rstd, k = -lo * rs;
+      if (at.lane == 0) {
+        float* st = a.stats + row * 3;
+        st[0] = hi;
+        st[1] = lo;
+        st[2] = rs;
+      }
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        float y[V];
+        Chunk<ELT> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = fmaf(fmaf(s[i].get(j) - hi, rs, k), 1.0f + up[i][j], shift[i][j]);
+        o.pack(y);
+        at.store((uint8_t*)a.y + row * a.cols * EB, i, o);
+      }
+    } else {
+      const int tiles = (at.cols + 255) / 256;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        if (!at.some(i)) continue;
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          y[j] = (float)fma(((double)s[i].get(j) - mean) * rstd, 1.0 + (double)up[i][j], (double)shift[i][j]);
+        if (!at.all(i)) {  // zeros up to the tile's end
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[j] = j < at.left(i) ? y[j] : 0.0f;
+        }
+        const uint32_t byte = mx_exponent<2>(mx_top<kMxBlock / V>(mx_top_of<V>(y)));
+        const int col = at.col(i);
+        if (col >= tiles * 256) continue;
+        const uint32_t word = mx4_codes<V>(y, byte);
+        uint8_t* p = a.codes + row * tiles * 128 + col / 2;
+        if constexpr (V == 8) *reinterpret_cast<uint32_t*>(p) = word;
+        else *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
+        if (col % kMxBlock == 0) a.scales[mx4_scale_at(row, col / kMxBlock, tiles)] = (uint8_t)byte;
+      }
+    }
+    cur = next;
   }
 }
 
@@ -186,17 +224,19 @@ int mod_forward(const char* fn, const char* label, int mode, ModArgs a, int dtyp
   a.m_f32 = m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32;
   a.per_col = 1.0 / (double)a.cols;
   const ModForm f = mod_form(dtype, a.cols);
-  const int threads = f.tpr < 256 ? 256 : f.tpr;
-  const int64_t grid = ceil_div(a.rows, threads / f.tpr);
-  if (!grid_fits(grid, threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
+  // Rows that follow each other in a wave or workgroup: as many as leave every one resident, one where
+  // each row has its own modulations
+  const int64_t per = f.tpr == 64 ? 4 : 1, resident = 256 * (16 * 64 / f.threads) * per;
+  const int64_t run = a.rpg == 1 || a.rows < resident ? a.rows : resident, grid = ceil_div(run, per);
+  if (!grid_fits(grid, f.threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
   { TraceScope _ts(st, label);
     with_any_elt(dtype, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      with_mod_form<E>(f, [&](auto tpr, auto nch) {
-        constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = T < 256 ? 256 : T;
-        if (mode == 2) mod_kernel<E, T, C, 2><<<(unsigned)grid, NT, 0, st>>>(a);
-        else if (a.ks != nullptr) mod_kernel<E, T, C, 1><<<(unsigned)grid, NT, 0, st>>>(a);
-        else mod_kernel<E, T, C, 0><<<(unsigned)grid, NT, 0, st>>>(a);
+      with_mod_form<E>(f, a.cols, [&](auto tpr, auto nch, auto nt, auto kind) {
+        constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = decltype(nt)::value, Y = decltype(kind)::value;
+        if (mode == 2) mod_kernel<E, T, C, NT, Y, 2><<<(unsigned)grid, f.threads, 0, st>>>(a, (uint32_t)run);
+        else if (a.ks != nullptr) mod_kernel<E, T, C, NT, Y, 1><<<(unsigned)grid, f.threads, 0, st>>>(a, (uint32_t)run);
+        else mod_kernel<E, T, C, NT, Y, 0><<<(unsigned)grid, f.threads, 0, st>>>(a, (uint32_t)run);
       });
     }); }
   return check_launch(label);

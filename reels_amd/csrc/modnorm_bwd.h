@@ -23,7 +23,7 @@ struct ModBwdArgs {
   void *dx, *db;                                      // db with a gate only
   float *dgate, *dscale, *dshift;                     // [groups][cols], or nullptr (dshift with dscale)
   float* part;                                        // [groups][parts][3][cols] where parts > 1
-  int64_t ld_gate, ld_scale, rows, cols, rpg;
+  int64_t ld_gate, ld_scale, rows, cols, rpg, run;    // run: rows that follow each other in a wave or workgroup
   double per_col;
   int center, m_f32, parts;
 };

@@ -28,12 +28,17 @@ __global__ __launch_bounds__(1024) void mod_sum_kernel(const float* __restrict__
 }
 
 
-// Partial rows of a group: together as many workgroups as the GPU holds at once, and at least two rows for
-// each group of threads, so that the partial rows stay a small part of the traffic
-int64_t mod_parts(int64_t groups, int64_t rpg, ModForm f) {
-  const int64_t rpb = f.tpr < 256 ? 256 / f.tpr : 1;
-  const int64_t want = ceil_div(f.tpr >= 512 ? 256 : 512, groups), need = ceil_div(rpg, 2 * rpb);
-  return want < need ? want : need;
+// Walkers (waves or workgroups) of a group's rows with the sums: together as many workgroups as the GPU holds
+// at once by their registers (12 waves of a CU), and at least two rows for each, so that the partial rows stay
+// a small part of the traffic. {partial rows, rows that follow each other}
+struct ModParts { int64_t parts, run; };
+ModParts mod_parts(int64_t groups, int64_t rpg, ModForm f) {
+  const int64_t walkers = f.tpr == 64 ? 4 : 1, wgs = 256 * (12 * 64 / f.threads > 0 ? 12 * 64 / f.threads : 1);
+  const int64_t share = ceil_div(wgs, groups) * walkers;
+  int64_t run = ceil_div(rpg, share);
+  if (run < 2) run = 2;
+  const int64_t parts = ceil_div(rpg, run * walkers);
+  return {parts, parts * walkers};
 }
 
 }  // namespace
@@ -45,7 +50,7 @@ extern "C" size_t reels_hip_modulated_norm_workspace_bytes(int64_t rows, int64_t
   const int64_t groups = ceil_div(rows, rows_per_group);
   int64_t n = 0;
   for (int elt : {REELS_HIP_F32, REELS_HIP_BF16}) {  // the most of any element type
-    const int64_t p = mod_parts(groups, rows_per_group, mod_form(elt, cols));
+    const int64_t p = mod_parts(groups, rows_per_group, mod_form(elt, cols)).parts;
     n = p > n ? p : n;
   }
   return n <= 1 ? 0 : align_up((size_t)(groups * n) * 3 * (size_t)cols * 4, 256);
@@ -71,16 +76,19 @@ extern "C" int reels_hip_modulated_norm_bwd(const void* dy, const void* s, const
     return fail(REELS_HIP_EINVAL, std::string(fn) + ": s and branch are both kept in 8 bits or neither");
   if (dy == nullptr || s == nullptr || stats == nullptr || dx == nullptr) return fail(REELS_HIP_EINVAL, std::string(fn) + ": NULL operand");
   const ModForm f = mod_form(dtype, cols);
-  const int threads = f.tpr < 256 ? 256 : f.tpr;
   const int64_t groups = rows / rows_per_group;
   const bool sums = rows_per_group > 1 && (dgate != nullptr || dscale != nullptr);
-  const int64_t parts = sums ? mod_parts(groups, rows_per_group, f) : 1;
+  const int64_t walkers = f.tpr == 64 ? 4 : 1;
+  // without sums a workgroup's rows follow each other as in the forward
+  const ModParts p = sums ? mod_parts(groups, rows_per_group, f)
+                          : ModParts{1, rows};
+  const int64_t parts = p.parts;
   if (parts > 1 && (workspace == nullptr || ws_bytes < reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group)))
     return fail(REELS_HIP_EWORKSPACE, std::string(fn) + ": workspace of reels_hip_modulated_norm_workspace_bytes required");
-  const int64_t grid = sums ? groups * parts : ceil_div(rows, threads / f.tpr);
-  if (!grid_fits(grid, threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
+  const int64_t grid = sums ? groups * parts : ceil_div(p.run, walkers);
+  if (!grid_fits(grid, f.threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
   const ModBwdArgs a{dy, s, dsum, branch, gate, scale, s_scales, branch_scales, stats, dx, dbranch, dgate, dscale, dshift,
-                     (float*)workspace, ld_gate, ld_scale, rows, cols, rows_per_group, 1.0 / (double)cols, center != 0,
+                     (float*)workspace, ld_gate, ld_scale, rows, cols, rows_per_group, p.run, 1.0 / (double)cols, center != 0,
                      m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32, (int)parts};
   { TraceScope _ts(st, "mod_bwd_kernel");
     with_any_elt(dtype, [&](auto e) { launch_mod_bwd<decltype(e)::value>(a, f, s_scales != nullptr, sums, grid, st); }); }

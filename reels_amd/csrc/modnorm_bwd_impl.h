@@ -5,46 +5,63 @@ namespace reels {
 namespace {
 
 // a thread's chunks of a row of s or the branch, as stored or in 8 bits
-template <int ELT, int TPR, int NCH, bool KEPT> struct Held {
-  static constexpr int V = Chunk<ELT>::V;
+template <int ELT, int TPR, int NCH, int KIND, bool KEPT> struct Held {
   Chunk<ELT> d[NCH];
-  __device__ __forceinline__ void load(const Row<ELT, TPR, NCH>& at, const void* p, const uint8_t*, int64_t row) {
+  __device__ __forceinline__ void load(const ModRow<ELT, TPR, NCH, KIND>& at, const void* p, const uint8_t*, int64_t row) {
     at.load((const uint8_t*)p + row * at.cols * elt_bytes(ELT), d);
   }
+  __device__ __forceinline__ void trim(const ModRow<ELT, TPR, NCH, KIND>& at) { at.trim(d); }
   __device__ __forceinline__ float get(int i, int j) const { return d[i].get(j); }
 };
-template <int ELT, int TPR, int NCH> struct Held<ELT, TPR, NCH, true> {
+template <int ELT, int TPR, int NCH, int KIND> struct Held<ELT, TPR, NCH, KIND, true> {
   static constexpr int V = Chunk<ELT>::V;
   Codes<V> d[NCH];
-  __device__ __forceinline__ void load(const Row<ELT, TPR, NCH>& at, const void* p, const uint8_t* scales, int64_t row) {
+  uint32_t byte[NCH];
+  __device__ __forceinline__ void load(const ModRow<ELT, TPR, NCH, KIND>& at, const void* p, const uint8_t* scales, int64_t row) {
     const int8_t* q = (const int8_t*)p + row * at.cols;
     const uint8_t* sc = scales + row * ((at.cols + kMxBlock - 1) / kMxBlock);
-    uint32_t byte[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      d[i].zero();
-      byte[i] = 0;
-      if (at.some(i) && (at.full(i) || at.part(i))) {
-        d[i].load(q + at.col(i), at.left(i), at.cols);
-        byte[i] = sc[at.col(i) / kMxBlock];
+      const int l = at.left(i);
+      if constexpr (KIND == kTiny) {
+        d[i].zero();
+        if (l > 0) d[i].load(q + at.col(i), l, at.cols);
+      } else {
+        d[i].load(q + (uint32_t)(KIND == kEven || l >= V ? at.col(i) : l > 0 ? at.cols - V : 0), V, V);
       }
+      byte[i] = sc[(uint32_t)(KIND == kEven || l > 0 ? at.col(i) / kMxBlock : 0)];
     }
+  }
+  __device__ __forceinline__ void trim(const ModRow<ELT, TPR, NCH, KIND>& at) {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) d[i].unit = mx8_unit(byte[i]);
+    for (int i = 0; i < NCH; ++i) {
+      d[i].unit = mx8_unit(byte[i]);
+      if (KIND == kTiny || at.all(i)) continue;
+      const int l = at.left(i);
+      if (l <= 0) d[i].zero();
+      else if (l < V) d[i].shift_down(V - l);
+    }
   }
   __device__ __forceinline__ float get(int i, int j) const { return d[i].get(j); }
 };
 
-// SUMS: the gradients of the modulations are summed over a group's rows; otherwise (no such gradient, or
-// groups of one row) a group of threads has one row
-template <int ELT, int TPR, int NCH, bool KEPT, bool SUMS>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void mod_bwd_kernel(ModBwdArgs a) {
-  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
-  __shared__ double slots[2][2][NT / 64];
-  __shared__ float acc[SUMS && RPB > 1 ? RPB * TPR * NCH * V : 1];
-  const int sub = threadIdx.x / TPR;
-  const int64_t wg_group = SUMS ? blockIdx.x / (unsigned)a.parts : 0, wg_part = SUMS ? blockIdx.x % (unsigned)a.parts : blockIdx.x;
-  const int64_t first = wg_group * a.rpg, end = SUMS ? a.rpg : a.rows, step = SUMS ? (int64_t)a.parts * RPB : (int64_t)gridDim.x * RPB;
+// A wave or workgroup walks rows begin .. end of one group, the next row's operands on their way meanwhile.
+// SUMS: it leaves the sums of the modulations' gradients over them; otherwise (no such gradient, or groups
+// of one row) rows of several groups may follow each other.
+template <int ELT, int TPR, int NCH, int NT, int KIND, bool KEPT, bool SUMS>
+__global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdArgs a) {
+  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), WALKERS = TPR == 0 ? 1 : 4;
+  __shared__ double slots[2][16][2];
+  __shared__ float acc[SUMS && WALKERS > 1 ? WALKERS * 64 * NCH * V : 1];
+  // A thread's gates wait in LDS until a row's end: with the sums they do not fit three waves' registers
+  constexpr bool AWAY = SUMS && NT == 512;
+  __shared__ f32x4 gates[AWAY ? NCH * V / 4 : 1][AWAY ? NT : 1];
+  const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
+  const int sub = TPR == 0 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // rows in 32 bits, so that they and what follows from them stay in scalar registers
+  const uint32_t wg_group = SUMS ? blockIdx.x / (uint32_t)a.parts : 0, part = SUMS ? blockIdx.x % (uint32_t)a.parts : blockIdx.x;
+  const uint32_t rpg = (uint32_t)a.rpg, run = (uint32_t)a.run, last = (uint32_t)a.rows - 1;
+  const uint32_t begin = wg_group * rpg + part * WALKERS + sub, end = SUMS ? (wg_group + 1) * rpg : last + 1;
   float tg[NCH][V], tc[NCH][V], th[NCH][V];
   if constexpr (SUMS) {
 #pragma unroll
@@ -52,124 +69,148 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void mod_bwd_kernel(ModBwdAr
 #pragma unroll
       for (int j = 0; j < V; ++j) tg[i][j] = tc[i][j] = th[i][j] = 0.0f;
   }
+  // s and dy of the next row are on their way while a row is worked on, its own branch and dsum until they are
+  // needed after the row's sums (all four a row ahead take 47 registers more than three waves on a SIMD have)
+  struct Data {
+    Held<ELT, TPR, NCH, KIND, KEPT> s;
+    Chunk<ELT> dy[NCH];
+    float hi, lo, rstd;
+  };
+  // all loads are unconditional, so that the waits for them need not count on the fewest: s and dy take the
+  // place of a branch and a dsum that are not there, the last row that of one past it
+  const void* branch = a.dgate != nullptr ? a.branch : a.s;
+  const uint8_t* bs = a.dgate != nullptr ? a.bs : a.ss;
+  const void* dsum = a.dsum != nullptr ? a.dsum : a.dy;
+  auto load = [&](uint32_t r, Data& d) {
+    const int64_t row = r < last ? r : last;
+    d.s.load(at, a.s, a.ss, row);
+    at.load((const uint8_t*)a.dy + row * a.cols * EB, d.dy);
+    d.hi = a.stats[row * 3];
+    d.lo = a.stats[row * 3 + 1];
+    d.rstd = a.stats[row * 3 + 2];
+  };
+  Data cur, next;
+  load(begin, cur);
+  float up[NCH][V], gate[NCH][V];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) up[i][j] = gate[i][j] = 1.0f;
+  uint32_t change = begin;
   int turn = 0;
-  for (int64_t r0 = wg_part * RPB; r0 < end; r0 += step, turn ^= 1) {
-    const Row<ELT, TPR, NCH> at(a.cols, r0 + sub < end);
-    const int64_t row = first + (at.live ? r0 + sub : end - 1), begin = row * a.cols * EB;
-    const int64_t group = SUMS ? wg_group : (int64_t)((uint32_t)row / (uint32_t)a.rpg);
-    const float hi = a.stats[row * 3], lo = a.stats[row * 3 + 1], rstd = a.stats[row * 3 + 2];
-    Held<ELT, TPR, NCH, KEPT> s, b;
-    Chunk<ELT> dy[NCH], ds[NCH];
-    float m[NCH][V];
-    s.load(at, a.s, a.ss, row);
-    at.load((const uint8_t*)a.dy + begin, dy);
-    if (a.dgate != nullptr) b.load(at, a.branch, a.bs, row);
-    if (a.dsum != nullptr) at.load((const uint8_t*)a.dsum + begin, ds);
-    if (a.scale != nullptr) {
-      load_mod(at, a.scale, a.ld_scale, a.m_f32, group, m);
-    } else {
+  for (uint32_t r = begin; r < end; r += run, turn ^= 1) {
+    const int64_t row = r, at0 = row * a.cols * EB;
+    if (r >= change) {
+      const uint32_t group = SUMS ? wg_group : r / rpg;
+      change = (group + 1) * rpg;
+      if (a.scale != nullptr) {
+        at.mods(a.scale, a.ld_scale, a.m_f32, group, up);
 #pragma unroll
-      for (int i = 0; i < NCH; ++i)
+        for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) m[i][j] = 0.0f;
+          for (int j = 0; j < V; ++j) up[i][j] += 1.0f;
+      }
+      if (a.gate != nullptr) {
+        at.mods(a.gate, a.ld_gate, a.m_f32, group, gate);
+        if constexpr (AWAY) {
+#pragma unroll
+          for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int j = 0; j < V; j += 4)
+              gates[(i * V + j) / 4][threadIdx.x] = f32x4{gate[i][j], gate[i][j + 1], gate[i][j + 2], gate[i][j + 3]};
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // here, and not at each row's use
     }
+    Held<ELT, TPR, NCH, KIND, KEPT> b;
+    Chunk<ELT> ds[NCH];
+    b.load(at, branch, bs, row);
+    at.load((const uint8_t*)dsum + at0, ds);
+    load(r + run, next);
+    cur.s.trim(at);
+    at.trim(cur.dy);
+    const float hi = cur.hi, rstd = cur.rstd, k = -cur.lo * rstd;
     double g0 = 0.0, g1 = 0.0;
+    // dy is zero where the thread has no element, and so are its shares of the sums
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      if (!at.some(i)) continue;
-      float n[V], d[V], p0 = 0.0f, p1 = 0.0f;
-      const bool any = at.full(i) || at.part(i);
+      float p0 = 0.0f, p1 = 0.0f, up1[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        d[j] = dy[i].get(j);
-        n[j] = (s.get(i, j) - hi - lo) * rstd;
-        const bool in = at.full(i) || j < at.left(i);
-        if (!(any && in)) n[j] = 0.0f;
-        if constexpr (SUMS) {
-          th[i][j] += d[j];
-          tc[i][j] = fmaf(d[j], n[j], tc[i][j]);
-        }
-        const float g = any && in ? d[j] * (1.0f + m[i][j]) : 0.0f;
+        const float d = cur.dy[i].get(j), n = fmaf(cur.s.get(i, j) - hi, rstd, k), g = d * up[i][j];
         p0 += g;
-        p1 = fmaf(g, n[j], p1);
+        p1 = fmaf(g, n, p1);
+        if constexpr (SUMS) {
+          th[i][j] += d;
+          tc[i][j] = fmaf(d, n, tc[i][j]);
+        }
+        up1[j] = d * n;
       }
       if constexpr (!SUMS) {
-        if (a.dscale != nullptr && any) {
-          float up[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) up[j] = d[j] * n[j];
-          store_vec<REELS_HIP_F32, V>(a.dscale + row * a.cols + at.col(i), at.left(i), up);
-          store_vec<REELS_HIP_F32, V>(a.dshift + row * a.cols + at.col(i), at.left(i), d);
+        if (a.dscale != nullptr) {
+          float d[V];
+          cur.dy[i].unpack(d);
+          at.store(a.dscale + row * a.cols, i, up1);
+          at.store(a.dshift + row * a.cols, i, d);
         }
       }
       g0 += (double)p0;
       g1 += (double)p1;
     }
-    // two slots in turn: a wave may enter the next row's reduction while another still reads this one's
-    if (a.center) g0 = row_reduce<TPR, false>(g0, slots[turn][0]);
-    else g0 = 0.0;
-    g1 = row_reduce<TPR, false>(g1, slots[turn][1]);
-    const float m0 = (float)(g0 * a.per_col), m1 = (float)(g1 * a.per_col);
-    float gate[NCH][V];
-    if (a.gate != nullptr) load_mod(at, a.gate, a.ld_gate, a.m_f32, group, gate);
+    row_sums<TPR>(g0, g1, slots[turn]);
+    b.trim(at);
+    at.trim(ds);
+    const float m0 = a.center ? (float)(g0 * a.per_col) : 0.0f, m1 = (float)(g1 * a.per_col);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      if (!at.some(i)) continue;
-      const bool any = at.full(i) || at.part(i);
       float d[V];
       Chunk<ELT> o;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float n = (s.get(i, j) - hi - lo) * rstd;
-        d[j] = rstd * (dy[i].get(j) * (1.0f + m[i][j]) - m0 - n * m1);
-      }
-      if (a.dsum != nullptr) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) d[j] += ds[i].get(j);
+        const float n = fmaf(cur.s.get(i, j) - hi, rstd, k);
+        const float t = fmaf(-n, m1, fmaf(cur.dy[i].get(j), up[i][j], -m0));
+        d[j] = a.dsum != nullptr ? fmaf(rstd, t, ds[i].get(j)) : rstd * t;
       }
       o.pack(d);
-      at.store((uint8_t*)a.dx + begin, i, o);
-      if (a.dgate != nullptr && any) {
+      at.store((uint8_t*)a.dx + at0, i, o);
+      if (a.dgate != nullptr) {
         float p[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          p[j] = d[j] * b.get(i, j);
-          if constexpr (SUMS) tg[i][j] += at.full(i) || j < at.left(i) ? p[j] : 0.0f;
+          if constexpr (SUMS) tg[i][j] = fmaf(d[j], b.get(i, j), tg[i][j]);
+          else p[j] = d[j] * b.get(i, j);
         }
-        if constexpr (!SUMS) store_vec<REELS_HIP_F32, V>(a.dgate + row * a.cols + at.col(i), at.left(i), p);
+        if constexpr (!SUMS) at.store(a.dgate + row * a.cols, i, p);
       }
       if (a.gate != nullptr) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] *= gate[i][j];
+        for (int j = 0; j < V; ++j) d[j] *= AWAY ? gates[(i * V + j) / 4][threadIdx.x][j % 4] : gate[i][j];
         o.pack(d);
-        at.store((uint8_t*)a.db + begin, i, o);
+        at.store((uint8_t*)a.db + at0, i, o);
       }
     }
+    cur = next;
   }
   if constexpr (SUMS) {
-    const int lane = threadIdx.x % TPR;
     auto leave = [&](float (&v)[NCH][V], float* whole, int which) {
       if (whole == nullptr) return;
-      float* out = a.parts == 1 ? whole + wg_group * a.cols : a.part + ((int64_t)blockIdx.x * 3 + which) * a.cols;
-      if constexpr (RPB > 1) {
+      float* out = a.parts == 1 ? whole + (int64_t)wg_group * a.cols : a.part + ((int64_t)blockIdx.x * 3 + which) * a.cols;
+      if constexpr (WALKERS > 1) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[(sub * TPR * NCH + lane + TPR * i) * V + j] = v[i][j];
+          for (int j = 0; j < V; ++j) acc[sub * 64 * NCH * V + at.col(i) + j] = v[i][j];
         __syncthreads();
-        for (int c = threadIdx.x; c < (int)a.cols; c += NT) {
+        for (int c = threadIdx.x; c < (int)a.cols; c += 256) {
           float t = acc[c];
 #pragma unroll
-          for (int r = 1; r < RPB; ++r) t += acc[r * TPR * NCH * V + c];
+          for (int r = 1; r < WALKERS; ++r) t += acc[r * 64 * NCH * V + c];
           out[c] = t;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-          const int c = (lane + TPR * i) * V, left = (int)a.cols - c;
-          if (left > 0) store_vec<REELS_HIP_F32, V>(out + c, left, v[i]);
-        }
+        for (int i = 0; i < NCH; ++i) at.store(out, i, v[i]);
       }
     };
     leave(tg, a.dgate, 0);
@@ -181,14 +222,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void mod_bwd_kernel(ModBwdAr
 }  // namespace
 
 template <int ELT> void launch_mod_bwd(const ModBwdArgs& a, ModForm f, bool kept, bool sums, int64_t grid, hipStream_t st) {
-  with_mod_form<ELT>(f, [&](auto tpr, auto nch) {
-    constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = T < 256 ? 256 : T;
+  with_mod_form<ELT>(f, a.cols, [&](auto tpr, auto nch, auto nt, auto kind) {
+    constexpr int T = decltype(tpr)::value, C = decltype(nch)::value, NT = decltype(nt)::value, Y = decltype(kind)::value;
     if (kept) {
-      if (sums) mod_bwd_kernel<ELT, T, C, true, true><<<(unsigned)grid, NT, 0, st>>>(a);
-      else mod_bwd_kernel<ELT, T, C, true, false><<<(unsigned)grid, NT, 0, st>>>(a);
+      if (sums) mod_bwd_kernel<ELT, T, C, NT, Y, true, true><<<(unsigned)grid, f.threads, 0, st>>>(a);
+      else mod_bwd_kernel<ELT, T, C, NT, Y, true, false><<<(unsigned)grid, f.threads, 0, st>>>(a);
     } else {
-      if (sums) mod_bwd_kernel<ELT, T, C, false, true><<<(unsigned)grid, NT, 0, st>>>(a);
-      else mod_bwd_kernel<ELT, T, C, false, false><<<(unsigned)grid, NT, 0, st>>>(a);
+      if (sums) mod_bwd_kernel<ELT, T, C, NT, Y, false, true><<<(unsigned)grid, f.threads, 0, st>>>(a);
+      else mod_bwd_kernel<ELT, T, C, NT, Y, false, false><<<(unsigned)grid, f.threads, 0, st>>>(a);
     }
   });
 }
