@@ -36,14 +36,12 @@ template <int N> __device__ __forceinline__ uint32_t mx_top(uint32_t v) {
   if constexpr (N == 8) up((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // the other four of eight
   return v;
 }
+// the largest magnitude of V values (v_maximum3: NaN stays)
 template <int V> __device__ __forceinline__ uint32_t mx_top_of(const float (&f)[V]) {
-  uint32_t t = 0;
+  float t = fabsf(f[0]);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const uint32_t u = __float_as_uint(f[j]) & 0x7fffffffu;
-    t = t > u ? t : u;
-  }
-  return t;
+  for (int j = 1; j < V; j += 2) t = __builtin_elementwise_maximum(t, __builtin_elementwise_maximum(fabsf(f[j]), fabsf(f[j + 1 < V ? j + 1 : j])));
+  return __float_as_uint(t);
 }
 
 // ---- 8 bits --------------------------------------------------------------------------------------

@@ -45,7 +45,7 @@ __device__ __forceinline__ void keep_chunk(const float (&f)[V], int8_t* codes, u
 // other, the next row's x and b on their way meanwhile; the modulations stay in registers while the group is the
 // same (as f32 they are half again what a row reads from memory).
 template <int ELT, int TPR, int NCH, int NT, int KIND, int MODE>
-__global__ __launch_bounds__(NT) void mod_kernel(ModArgs a, uint32_t run) {
+__global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1) void mod_kernel(ModArgs a, uint32_t run) {
   constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
   __shared__ double slots[2][16][2];
   const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
@@ -186,8 +186,11 @@ __global__ __launch_bounds__(NT) void mod_kernel(ModArgs a, uint32_t run) {
         if (!at.some(i)) continue;
         float y[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
+        for (int j = 0; j < V; ++j) {
+          // the modulations stay in 32 bits between rows: as 64-bit values they take a workgroup's registers
+          asm volatile("" : "+v"(up[i][j]), "+v"(shift[i][j]));
           y[j] = (float)fma(((double)s[i].get(j) - mean) * rstd, 1.0 + (double)up[i][j], (double)shift[i][j]);
+        }
         if (!at.all(i)) {  // zeros up to the tile's end
 #pragma unroll
           for (int j = 0; j < V; ++j) y[j] = j < at.left(i) ? y[j] : 0.0f;

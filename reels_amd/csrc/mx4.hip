@@ -127,12 +127,18 @@ template <int SA, int SB> __device__ __forceinline__ f32x16 mfma(const v4i& a, c
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, SA, (int)sa, SB, (int)sb);
 }
 
+__device__ __forceinline__ u32x2 copy_now(u32x2 v) {
+  uint32_t a, b;
+  asm volatile("v_mov_b32 %0, %2\n\tv_mov_b32 %1, %3" : "=&v"(a), "=v"(b) : "v"(v[0]), "v"(v[1]));
+  return u32x2{a, b};
+}
+
 // 32 TJ x 32 TJ outputs per workgroup of TJ waves (TJ = 8: 256 x 256, TJ = 4: 128 x 128), a step of 256
 // codes (128 bytes of a row), each wave 16 TJ tokens x 64 columns. The operands travel from HBM to LDS
 // directly (rows of 128 bytes, 16-byte chunks XOR-swizzled by the row) into two stages: in the middle of
 // step kt, when every wave has read all of its stage, a barrier lets the copies of step kt + 2 go into it; they
-// have until the middle of step kt + 1. The scale words go to registers, three steps' worth, with the same
-// waits. Rows past the edges read as zeros (the buffer's bounds), columns past K are zeros in the codes.
+// have until the middle of step kt + 1. The scale words go to registers two steps ahead with
+// the same waits. Rows past the edges read as zeros (the buffer's bounds), columns past K are zeros in the codes.
 template <int TJ> struct Tile {
   static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 128;
   static constexpr int ACT = BM * BK, WB = BN * BK, LDS = 2 * ACT + 2 * WB;
@@ -155,12 +161,15 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
   const int Kb = a.tiles * 128, nk = a.tiles;
   const int rows = (int)(a.M - m0 < T::BM ? a.M - m0 : T::BM), cols = (int)(a.N - n0 < T::BN ? a.N - n0 : T::BN);
   const i32x4 rx = buffer_rsrc(a.x + m0 * Kb, (uint32_t)rows * Kb), rw = buffer_rsrc(a.w + n0 * Kb, (uint32_t)cols * Kb);
-  // copy i of wave w: tile rows 8 (4 w + i) + lane / 8, 16 bytes per lane
-  const uint32_t vo = (uint32_t)((w * 32 + (lane >> 3)) * Kb + ((lane & 7) ^ (lane >> 3)) * 16);
+  // copy i of wave w: tile rows 8 (4 w + i) + lane / 8, 16 bytes per lane. Chunk c of a row lies at
+  // c ^ (row / 2 % 8): 16 rows that a quarter of a fragment's lanes read then lie in 64 different banks (with
+  // c ^ row % 8 they met in pairs, half of the LDS's time)
+  const uint32_t vrow = (uint32_t)((w * 32 + (lane >> 3)) * Kb), vc = (uint32_t)((lane & 7) ^ (lane >> 4)) * 16;
+  const uint32_t vo[2] = {vrow + vc, vrow + (vc ^ 64)};
   auto abase = [&](int kt) { return smem + (kt & 1) * T::ACT; };
   auto wbase = [&](int kt) { return smem + 2 * T::ACT + (kt & 1) * T::WB; };
-  auto issue_x = [&](const i32x4& r, int kt, int i) { dma16(r, vo, (uint32_t)(kt * T::BK + i * 8 * Kb), abase(kt) + (w * 4 + i) * 1024); };
-  auto issue_w = [&](const i32x4& r, int kt, int i) { dma16(r, vo, (uint32_t)(kt * T::BK + i * 8 * Kb), wbase(kt) + (w * 4 + i) * 1024); };
+  auto issue_x = [&](const i32x4& r, int kt, int i) { dma16(r, vo[i & 1], (uint32_t)(kt * T::BK + i * 8 * Kb), abase(kt) + (w * 4 + i) * 1024); };
+  auto issue_w = [&](const i32x4& r, int kt, int i) { dma16(r, vo[i & 1], (uint32_t)(kt * T::BK + i * 8 * Kb), wbase(kt) + (w * 4 + i) * 1024); };
   // scale words of a step: 64 rows' in two words a lane, zeros past the last step. Tiles of rows past the
   // last read another's.
   const int64_t last_x = ((a.M + 63) >> 6) - 1, last_w = ((a.N + 63) >> 6) - 1;
@@ -184,8 +193,8 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < JT; ++j) acc[i][j] = zeros16();
-  // where a lane's 16 bytes lie: chunk 4 h + 2 ks + hi of its row, swizzled by the row
-  const int xat = (wm * 16 * TJ + l32) * 128 + ((hi ^ (l32 & 7)) << 4), wat = (wn * 64 + l32) * 128 + ((hi ^ (l32 & 7)) << 4);
+  // where a lane's 16 bytes lie: chunk 4 h + 2 ks + hi of its row, swizzled
+  const int sel = (hi ^ (l32 >> 1 & 7)) << 4, xat = (wm * 16 * TJ + l32) * 128 + sel, wat = (wn * 64 + l32) * 128 + sel;
   // fragments of half h of a step, 64 codes each: the weight's [ks][i], the activations' j = ks * JT + jt
   auto read_w = [&](const uint8_t* s, int h, v4i* f) {
 #pragma unroll
@@ -215,7 +224,7 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
     }
   };
   v4i w0[4], w1[4], x[TJ];
-  Scales s0 = load_scales(0), s1 = load_scales(1);
+  Scales s0 = load_scales(0), next = load_scales(1);
 #pragma unroll
   for (int i = 0; i < 4; ++i) { issue_x(rx, 0, i); issue_w(rw, 0, i); }
   if (nk > 1) {
@@ -251,7 +260,13 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
     asm volatile("" ::: "memory");
     if (TJ == 8 && w >= 4) __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
-    const Scales s2 = load_scales(kt + 2);
+    // step kt + 1's scale words have arrived; copied here by name, since the compiler's copy at the step's end
+    // would wait for everything in flight
+    Scales s1;
+#pragma unroll
+    for (int q = 0; q < XT; ++q) s1.x[q] = copy_now(next.x[q]);
+    s1.w = copy_now(next.w);
+    next = load_scales(kt + 2);
     i32x4 cx = rx, cw = rw;  // the last step but one has no step to copy: its copies read nothing
     cx[2] = kt + 2 < nk ? rx[2] : 0;
     cw[2] = kt + 2 < nk ? rw[2] : 0;
@@ -270,7 +285,6 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
       __builtin_amdgcn_sched_barrier(0);
     });
     s0 = s1;
-    s1 = s2;
   }
   if (TJ == 8 && w >= 4) __builtin_amdgcn_s_setprio(0);
   {
@@ -399,7 +413,7 @@ template <int ELT> __global__ __launch_bounds__(small::NT) void mx4_small_kernel
   const i32x4 rx = buffer_rsrc(a.x + m0 * Kb, (uint32_t)rows * Kb), rw = buffer_rsrc(a.w + n0 * Kb, (uint32_t)cols * Kb);
   const i32x4 rs = buffer_rsrc(w == 0 ? a.xs + tm * a.tiles * 512 : a.ws + tn * a.tiles * 512, w < 2 ? (uint32_t)a.tiles * 512 : 0u);
   const int crow = w * 8 + (lane >> 3);  // a wave copies rows 8 w .. 8 w + 7 of each tile
-  const uint32_t vo = (uint32_t)(crow * Kb + ((lane & 7) ^ (crow & 7)) * 16);
+  const uint32_t vo = (uint32_t)(crow * Kb + ((lane & 7) ^ (crow >> 1 & 7)) * 16);
   auto issue = [&](int kt) {  // past the end the copies read nothing, so that the waits count the same
     uint8_t* s = smem + (kt & (RING - 1)) * STAGE;
     const bool in = kt < nk;
@@ -415,7 +429,7 @@ template <int ELT> __global__ __launch_bounds__(small::NT) void mx4_small_kernel
 #pragma unroll
   for (int kt = 0; kt < RING - 1; ++kt) issue(kt);
   f32x16 acc = zeros16();
-  const int off0 = ((4 * h + hi) ^ (l32 & 7)) << 4, off1 = ((4 * h + 2 + hi) ^ (l32 & 7)) << 4;
+  const int off0 = ((4 * h + hi) ^ (l32 >> 1 & 7)) << 4, off1 = off0 ^ 32;
   for (int kt = 0; kt < nk; ++kt) {
     __builtin_amdgcn_s_waitcnt(0x0F76);  // vmcnt(6): step kt has landed, the two after it may fly
     __builtin_amdgcn_s_barrier();
