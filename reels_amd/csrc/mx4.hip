@@ -127,21 +127,17 @@ template <int SA, int SB> __device__ __forceinline__ f32x16 mfma(const v4i& a, c
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, SA, (int)sa, SB, (int)sb);
 }
 
-__device__ __forceinline__ u32x2 copy_now(u32x2 v) {
-  uint32_t a, b;
-  asm volatile("v_mov_b32 %0, %2\n\tv_mov_b32 %1, %3" : "=&v"(a), "=v"(b) : "v"(v[0]), "v"(v[1]));
-  return u32x2{a, b};
-}
-
-// 32 TJ x 32 TJ outputs per workgroup of TJ waves (TJ = 8: 256 x 256, TJ = 4: 128 x 128), a step of 256
-// codes (128 bytes of a row), each wave 16 TJ tokens x 64 columns. The operands travel from HBM to LDS
-// directly (rows of 128 bytes, 16-byte chunks XOR-swizzled by the row) into two stages: in the middle of
-// step kt, when every wave has read all of its stage, a barrier lets the copies of step kt + 2 go into it; they
-// have until the middle of step kt + 1. The scale words go to registers two steps ahead with
-// the same waits. Rows past the edges read as zeros (the buffer's bounds), columns past K are zeros in the codes.
+// 32 TJ x 32 TJ outputs per workgroup of TJ waves (TJ = 8: 256 x 256, TJ = 4: 128 x 128), each wave 16 TJ
+// tokens x 64 columns, in steps of 128 codes (64 bytes of a row). The operands travel from HBM to LDS directly
+// into a ring of four stages. While the products of step s run, the fragments of step s + 1 replace those that
+// are used up; behind the first products of step s, when every wave has the last fragments of step s in
+// registers, a barrier lets the copies of step s + 4 go into its stage, so a copy has three steps to arrive
+// (a step of 256 codes in two stages gave it three quarters of one: 1176 us). Scale words, two steps' worth, go
+// the same way in a ring of three. Rows past the edges read as zeros (the buffer's bounds), columns past K
+// are zeros in the codes; copies past the last step read nothing, so that every step's waits count the same.
 template <int TJ> struct Tile {
-  static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 128;
-  static constexpr int ACT = BM * BK, WB = BN * BK, LDS = 2 * ACT + 2 * WB;
+  static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 64;
+  static constexpr int ACT = BM * BK, WB = BN * BK, STAGE = ACT + WB, SCALES = NW * 512, LDS = 4 * STAGE + 3 * SCALES;
 };
 
 template <int ELT, int TJ>
@@ -158,33 +154,34 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
   const int group = 4 * tiles_n, g = logical / group, first = g * 4;
   const int gm = tiles_m - first < 4 ? tiles_m - first : 4, within = logical - g * group;
   const int64_t m0 = (int64_t)(first + within % gm) * T::BM, n0 = (int64_t)(within / gm) * T::BN;
-  const int Kb = a.tiles * 128, nk = a.tiles;
+  const int Kb = a.tiles * 128, steps = a.tiles * 2;
   const int rows = (int)(a.M - m0 < T::BM ? a.M - m0 : T::BM), cols = (int)(a.N - n0 < T::BN ? a.N - n0 : T::BN);
   const i32x4 rx = buffer_rsrc(a.x + m0 * Kb, (uint32_t)rows * Kb), rw = buffer_rsrc(a.w + n0 * Kb, (uint32_t)cols * Kb);
-  // copy i of wave w: tile rows 8 (4 w + i) + lane / 8, 16 bytes per lane. Chunk c of a row lies at
-  // c ^ (row / 2 % 8): 16 rows that a quarter of a fragment's lanes read then lie in 64 different banks (with
-  // c ^ row % 8 they met in pairs, half of the LDS's time)
-  const uint32_t vrow = (uint32_t)((w * 32 + (lane >> 3)) * Kb), vc = (uint32_t)((lane & 7) ^ (lane >> 4)) * 16;
-  const uint32_t vo[2] = {vrow + vc, vrow + (vc ^ 64)};
-  auto abase = [&](int kt) { return smem + (kt & 1) * T::ACT; };
-  auto wbase = [&](int kt) { return smem + 2 * T::ACT + (kt & 1) * T::WB; };
-  auto issue_x = [&](const i32x4& r, int kt, int i) { dma16(r, vo[i & 1], (uint32_t)(kt * T::BK + i * 8 * Kb), abase(kt) + (w * 4 + i) * 1024); };
-  auto issue_w = [&](const i32x4& r, int kt, int i) { dma16(r, vo[i & 1], (uint32_t)(kt * T::BK + i * 8 * Kb), wbase(kt) + (w * 4 + i) * 1024); };
-  // scale words of a step: 64 rows' in two words a lane, zeros past the last step. Tiles of rows past the
-  // last read another's.
-  const int64_t last_x = ((a.M + 63) >> 6) - 1, last_w = ((a.N + 63) >> 6) - 1;
-  auto words = [&](const uint8_t* p, int64_t tile, int64_t last) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p + (tile < last ? tile : last) * a.tiles * 512), (short)0, a.tiles * 512, 0x00020000);
+  // Copy i of wave w: tile rows 16 (2 w + i) + lane / 4, 16 bytes per lane. Chunk c of a row of 64 bytes lies at
+  // c ^ (row / 4 % 4): the 16 rows that a quarter of a fragment's lanes read lie in 64 different banks.
+  const uint32_t vo = (uint32_t)((w * 32 + (lane >> 2)) * Kb + ((lane & 3) ^ (lane >> 4)) * 16);
+  auto stage = [&](int s) { return smem + (s & 3) * T::STAGE; };
+  auto issue = [&](int s, int q) {  // q: 0, 1 activations, 2, 3 weight
+    i32x4 r = q < 2 ? rx : rw;
+    r[2] = s < steps ? r[2] : 0;
+    dma16(r, vo, (uint32_t)(s * T::BK + (q & 1) * 16 * Kb), stage(s) + (q < 2 ? 0 : T::ACT) + (w * 2 + (q & 1)) * 1024);
   };
-  const int64_t xt = (m0 + wm * 16 * TJ) / 64;
-  const __amdgpu_buffer_rsrc_t sx0 = words(a.xs, xt, last_x), sx1 = words(a.xs, xt + XT - 1, last_x);
-  const __amdgpu_buffer_rsrc_t sw = words(a.ws, (n0 + wn * 64) / 64, last_w);
+  // scale words: wave w brings a tile of 64 rows' for two steps, lanes 0 .. 31. Tiles of rows past the last
+  // read another's.
+  const bool xs = w < T::NW / 2;
+  const int64_t tile = xs ? m0 / 64 + w : n0 / 64 + w - T::NW / 2, last = ((xs ? a.M : a.N) + 63) / 64 - 1;
+  const i32x4 rs = buffer_rsrc((xs ? a.xs : a.ws) + (tile < last ? tile : last) * a.tiles * 512, (uint32_t)a.tiles * 512);
+  uint8_t* const ring = smem + 4 * T::STAGE;
+  auto issue_scales = [&](int pair, int slot) {
+    if (lane < 32) dma16(rs, (uint32_t)lane * 16, (uint32_t)pair * 512, ring + slot * T::SCALES + w * 512);
+  };
   struct Scales { u32x2 x[XT], w; };
-  auto load_scales = [&](int kt) {
+  auto read_scales = [&](int slot) {
+    const uint8_t* p = ring + slot * T::SCALES + lane * 8;
     Scales s;
-    s.x[0] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sx0, lane * 8, kt * 512, 0));
-    if constexpr (XT == 2) s.x[1] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sx1, lane * 8, kt * 512, 0));
-    s.w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sw, lane * 8, kt * 512, 0));
+#pragma unroll
+    for (int q = 0; q < XT; ++q) s.x[q] = *reinterpret_cast<const u32x2*>(p + (wm * XT + q) * 512);
+    s.w = *reinterpret_cast<const u32x2*>(p + (T::NW / 2 + wn) * 512);
     return s;
   };
 
@@ -193,24 +190,14 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < JT; ++j) acc[i][j] = zeros16();
-  // where a lane's 16 bytes lie: chunk 4 h + 2 ks + hi of its row, swizzled
-  const int sel = (hi ^ (l32 >> 1 & 7)) << 4, xat = (wm * 16 * TJ + l32) * 128 + sel, wat = (wn * 64 + l32) * 128 + sel;
-  // fragments of half h of a step, 64 codes each: the weight's [ks][i], the activations' j = ks * JT + jt
-  auto read_w = [&](const uint8_t* s, int h, v4i* f) {
+  // where a lane's 16 bytes lie: chunk 2 ks + hi of its row, swizzled
+  const int sel = (hi ^ (l32 >> 2 & 3)) << 4, xat = (wm * 16 * TJ + l32) * 64 + sel, wat = T::ACT + (wn * 64 + l32) * 64 + sel;
+  // fragments of a step, 64 codes each: the weight's [ks][i], the activations' j = ks * JT + jt
+  auto read_w = [&](const uint8_t* s, v4i (&f)[4]) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        f[ks * 2 + i] = *reinterpret_cast<const v4i*>(s + i * 4096 + (wat ^ ((4 * h + 2 * ks) << 4)));
+    for (int q = 0; q < 4; ++q) f[q] = *reinterpret_cast<const v4i*>(s + (q & 1) * 2048 + (wat ^ ((q >> 1) << 5)));
   };
-  auto read_x = [&](const uint8_t* s, int h, int j) {
-    return *reinterpret_cast<const v4i*>(s + (j % JT) * 4096 + (xat ^ ((4 * h + 2 * (j / JT)) << 4)));
-  };
-  auto mfma2 = [&](const v4i* f, const v4i& xf, auto jc, int h, const Scales& s) {
-    constexpr int j = decltype(jc)::value, ks = j / JT, jt = j % JT;
-    acc[0][jt] = mfma<ks * 2, ks * 2 + (jt & 1)>(f[ks * 2], xf, acc[0][jt], s.w[h], s.x[jt / 2][h]);
-    acc[1][jt] = mfma<ks * 2 + 1, ks * 2 + (jt & 1)>(f[ks * 2 + 1], xf, acc[1][jt], s.w[h], s.x[jt / 2][h]);
-  };
+  auto read_x = [&](const uint8_t* s, int j) { return *reinterpret_cast<const v4i*>(s + (j % JT) * 2048 + (xat ^ ((j / JT) << 5))); };
   auto each = [&](auto&& f) {  // over the TJ activation fragments
     f(std::integral_constant<int, 0>{});
     f(std::integral_constant<int, 1>{});
@@ -224,84 +211,59 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
     }
   };
   v4i w0[4], w1[4], x[TJ];
-  Scales s0 = load_scales(0), next = load_scales(1);
+  issue_scales(0, 0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { issue_x(rx, 0, i); issue_w(rw, 0, i); }
-  if (nk > 1) {
+  for (int q = 0; q < 8; ++q) issue(q >> 2, q & 3);
+  issue_scales(1, 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { issue_x(rx, 1, i); issue_w(rw, 1, i); }
-    __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): step 1 may stay in flight
-  } else {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  }
+  for (int q = 8; q < 16; ++q) issue(q >> 2, q & 3);
+  __builtin_amdgcn_s_waitcnt(0x0F7D);  // vmcnt(13): step 0 and its scale words have landed
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  read_w(wbase(0), 0, w0);
+  Scales s0 = read_scales(0), s1;
+  read_w(stage(0), w0);
 #pragma unroll
-  for (int j = 0; j < TJ; ++j) x[j] = read_x(abase(0), 0, j);
-  for (int kt = 0; kt + 1 < nk; ++kt) {
-    // eight waves: w and w + 4 share a SIMD, and the younger one has the priority in the second half
-    // of a step, so that both reach the barrier together
-    if (TJ == 8 && w >= 4) __builtin_amdgcn_s_setprio(0);
-    const uint8_t* sa = abase(kt);
-    const uint8_t* sb = wbase(kt);
+  for (int j = 0; j < TJ; ++j) x[j] = read_x(stage(0), j);
+  int slot = 0;  // of the pair's scale words
+  // a step: its products on f, the next step's fragments into f1
+  auto step = [&](int s, auto ec, v4i (&f)[4], v4i (&f1)[4]) {
+    constexpr int e = decltype(ec)::value, B = TJ / 4 - 1;
+    const uint8_t* sn = stage(s + 1);
     each([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      mfma2(w0, x[j], jc, 0, s0);
+      constexpr int j = decltype(jc)::value, ks = j / JT, jt = j % JT;
+      acc[0][jt] = mfma<ks * 2, ks * 2 + (jt & 1)>(f[ks * 2], x[j], acc[0][jt], s0.w[e], s0.x[jt / 2][e]);
+      acc[1][jt] = mfma<ks * 2 + 1, ks * 2 + (jt & 1)>(f[ks * 2 + 1], x[j], acc[1][jt], s0.w[e], s0.x[jt / 2][e]);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (j == 0) read_w(sb, 1, w1);
-      x[j] = read_x(sa, 1, j);
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    // every fragment of this stage is in registers, and step kt + 1 has landed
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (TJ == 8 && w >= 4) __builtin_amdgcn_s_setprio(1);
-    __builtin_amdgcn_sched_barrier(0);
-    // step kt + 1's scale words have arrived; copied here by name, since the compiler's copy at the step's end
-    // would wait for everything in flight
-    Scales s1;
+      if constexpr (j == B) {
+        // This wave's fragments have arrived, and its copies of step s + 1 with their scale words: after them
+        // two steps' copies and one of scale words were issued
+        __builtin_amdgcn_s_waitcnt(0x0079);  // vmcnt(9) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if constexpr (e == 0) issue_scales((s >> 1) + 2, slot == 0 ? 2 : slot - 1);
+        else s1 = read_scales(slot == 2 ? 0 : slot + 1);
+        read_w(sn, f1);
 #pragma unroll
-    for (int q = 0; q < XT; ++q) s1.x[q] = copy_now(next.x[q]);
-    s1.w = copy_now(next.w);
-    next = load_scales(kt + 2);
-    i32x4 cx = rx, cw = rw;  // the last step but one has no step to copy: its copies read nothing
-    cx[2] = kt + 2 < nk ? rx[2] : 0;
-    cw[2] = kt + 2 < nk ? rw[2] : 0;
-    const uint8_t* san = abase(kt + 1);
-    read_w(wbase(kt + 1), 0, w0);
-    __builtin_amdgcn_sched_barrier(0);
-    each([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      mfma2(w1, x[j], jc, 1, s0);
-      __builtin_amdgcn_sched_barrier(0);
-      x[j] = read_x(san, 0, j);
-      if constexpr (j < 4) {
-        issue_x(cx, kt + 2, j);
-        issue_w(cw, kt + 2, j);
+        for (int i = 0; i < j; ++i) x[i] = read_x(sn, i);
+      }
+      if constexpr (j >= B) {
+        x[j] = read_x(sn, j);
+        if constexpr (j - B < 4) issue(s + 4, j - B);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
+  };
+  for (int s = 0; s < steps; s += 2) {
+    step(s, std::integral_constant<int, 0>{}, w0, w1);
+    step(s + 1, std::integral_constant<int, 1>{}, w1, w0);
     s0 = s1;
+    slot = slot == 2 ? 0 : slot + 1;
   }
-  if (TJ == 8 && w >= 4) __builtin_amdgcn_s_setprio(0);
-  {
-    const uint8_t* sa = abase(nk - 1);
-    read_w(wbase(nk - 1), 1, w1);
-    each([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      mfma2(w0, x[j], jc, 0, s0);
-      x[j] = read_x(sa, 1, j);
-    });
-    each([&](auto jc) { mfma2(w1, x[decltype(jc)::value], jc, 1, s0); });
-  }
-  // Epilogue: f32 values of 64 tokens x 64 columns at a time in the wave's own 16 KiB of LDS (rows of
-  // 256 bytes, 16-byte chunks XOR-swizzled), read back as rows: bias, residual and stores in whole segments
   __builtin_amdgcn_s_waitcnt(0x0F70);  // no copy outlives the loop
   __syncthreads();
-  uint8_t* stage = smem + w * 16384;
+  uint8_t* out = smem + w * 16384;
+  // Epilogue: f32 values of 64 tokens x 64 columns at a time in the wave's own 16 KiB of LDS (rows of
+  // 256 bytes, 16-byte chunks XOR-swizzled), read back as rows: bias, residual and stores in whole segments
   constexpr int LPR = 64 / V, RPI = 64 / LPR, ITS = 64 / RPI;  // lanes of a row, rows at once, turns
   const int c = (lane % LPR) * V, left = cols - (wn * 64 + c);
   float bs[V];
@@ -332,7 +294,7 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
           f32x4 o;
 #pragma unroll
           for (int v = 0; v < 4; ++v) o[v] = acc[i][h * 2 + j][q * 4 + v];
-          *reinterpret_cast<f32x4*>(stage + r * 256 + (((i * 8 + q * 2 + hi) ^ (r & 15)) << 4)) = o;
+          *reinterpret_cast<f32x4*>(out + r * 256 + (((i * 8 + q * 2 + hi) ^ (r & 15)) << 4)) = o;
         }
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -344,7 +306,7 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
       float o[V];
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) {
-        const f32x4 f = *reinterpret_cast<const f32x4*>(stage + r * 256 + (((c / 4 + q) ^ (r & 15)) << 4));
+        const f32x4 f = *reinterpret_cast<const f32x4*>(out + r * 256 + (((c / 4 + q) ^ (r & 15)) << 4));
 #pragma unroll
         for (int v = 0; v < 4; ++v) o[q * 4 + v] = f[v] + bs[q * 4 + v];
       }
