@@ -7,6 +7,7 @@ activations themselves; only the backward sees the rounded ones.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -70,18 +71,22 @@ def _checked(k: CompressedActivations, name: str) -> CompressedActivations:
     _need_device(v, name)
     if v.dtype != torch.int8 or v.dim() < 1 or v.shape[-1] < 1:
         raise ValueError(f"{name} must have int8 values with rows of at least one, got {v.dtype} {tuple(v.shape)}")
-    want = tuple(v.shape[:-1]) + (-(-v.shape[-1] // _BLOCK),)
-    if s.dtype != torch.uint8 or tuple(s.shape) != want or s.device != v.device:
+    want = _scales_shape(v.shape)
+    if s.dtype != torch.uint8 or s.shape != want or s.device != v.device:
         raise ValueError(f"{name} must have uint8 scales of shape {want} on the values' device")
     if v.is_contiguous() and s.is_contiguous():
         return k
     return CompressedActivations(v.contiguous(), s.contiguous(), k.compute_dtype)
 
 
+@functools.lru_cache(maxsize=4096)
+def _scales_shape(shape):
+    return tuple(shape[:-1]) + (-(-shape[-1] // _BLOCK),)
+
+
 def _empty(shape, dtype, device) -> CompressedActivations:
     return CompressedActivations(torch.empty(shape, dtype=torch.int8, device=device),
-                                 torch.empty(tuple(shape[:-1]) + (-(-shape[-1] // _BLOCK),), dtype=torch.uint8,
-                                             device=device), dtype)
+                                 torch.empty(_scales_shape(shape), dtype=torch.uint8, device=device), dtype)
 
 
 def _input(x: torch.Tensor):

@@ -436,22 +436,28 @@ template <int ELT> __global__ __launch_bounds__(small::NT) void mx4_small_kernel
 
 // ---- few tokens ----------------------------------------------------------------------------------
 // Up to 16 tokens: 16 outputs per workgroup, its waves take lines of 256 codes in turn and read codes and
-// scale bytes straight into registers (each code of the weight is used once, so LDS would only add a trip),
-// then add their sums in LDS in wave order. Bound by the weight's bytes and by latency.
-constexpr int kFewTokens = 16, kFewWaves = 8;
+// scale words straight into registers (each code of the weight is used once, so LDS would only add a trip),
+// then add their sums in LDS in wave order. Lanes of tokens that are not there read nothing (an offset past the
+// buffer's bounds). Bound by the weight's bytes and by latency.
+constexpr int kFewTokens = 16, kFewWaves = 8;  // the most waves of a workgroup
 
 template <int ELT> __global__ __launch_bounds__(kFewWaves * 64) void mx4_few_kernel(Mx4Args a) {
   __shared__ f32x4 part[kFewWaves][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, lq = lane >> 4;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, lq = lane >> 4;
+  const int waves = (int)(blockDim.x >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int64_t n = n0 + l16 < a.N ? n0 + l16 : a.N - 1, m = l16 < a.M ? l16 : a.M - 1;
-  const int Kb = a.tiles * 128;
-  const uint8_t* wr = a.w + n * Kb + lq * 16;
-  const uint8_t* xr = a.x + m * Kb + lq * 16;
+  const int Kb = a.tiles * 128, rows = (int)(a.N - n0 < 16 ? a.N - n0 : 16);
+  auto buffer = [](const uint8_t* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), (short)0, (int)bytes, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t rw = buffer(a.w + n0 * Kb, (uint32_t)rows * Kb), rx = buffer(a.x, (uint32_t)a.M * Kb);
+  const __amdgpu_buffer_rsrc_t rws = buffer(a.ws + (n0 >> 6) * a.tiles * 512, (uint32_t)a.tiles * 512);
+  const __amdgpu_buffer_rsrc_t rxs = buffer(a.xs, (uint32_t)a.tiles * 512);
+  const uint32_t none = 0x80000000u, vw = (uint32_t)(l16 * Kb + lq * 16), vx = l16 < a.M ? vw : none;
   // a lane's blocks lq and 4 + lq of a line: the same byte of the two words
-  const u32x2* sw = reinterpret_cast<const u32x2*>(a.ws + (n >> 6) * a.tiles * 512) + (lq & 1) * 32 + (n & 31);
-  const u32x2* sx = reinterpret_cast<const u32x2*>(a.xs) + (lq & 1) * 32 + m;
-  const int bw = 8 * ((lq >> 1) * 2 + (int)((n >> 5) & 1)), bx = 8 * ((lq >> 1) * 2);
+  const int nr = (int)(n0 & 63) + l16;  // n0 is a multiple of 16: all rows of one tile
+  const uint32_t vws = (uint32_t)(((lq & 1) * 32 + (nr & 31)) * 8), vxs = l16 < a.M ? (uint32_t)(((lq & 1) * 32 + l16) * 8) : none;
+  const int bw = 8 * ((lq >> 1) * 2 + (nr >> 5)), bx = 8 * ((lq >> 1) * 2);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   int s = w;
   auto run = [&](auto count) {  // so many lines at once, all their loads in flight
@@ -460,17 +466,13 @@ template <int ELT> __global__ __launch_bounds__(kFewWaves * 64) void mx4_few_ker
     u32x2 cw[C], cx[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int k = s + c * kFewWaves;
-      wf[c][0] = *reinterpret_cast<const v4i*>(wr + k * 128);
-      wf[c][1] = *reinterpret_cast<const v4i*>(wr + k * 128 + 64);
-      cw[c] = sw[k * 64];
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int k = s + c * kFewWaves;
-      xf[c][0] = *reinterpret_cast<const v4i*>(xr + k * 128);
-      xf[c][1] = *reinterpret_cast<const v4i*>(xr + k * 128 + 64);
-      cx[c] = sx[k * 64];
+      const int k = s + c * waves;
+      wf[c][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, vw, k * 128, 0));
+      wf[c][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, vw + 64, k * 128, 0));
+      cw[c] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rws, vws, k * 512, 0));
+      xf[c][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, vx, k * 128, 0));
+      xf[c][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, vx + 64, k * 128, 0));
+      cx[c] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rxs, vxs, k * 512, 0));
     }
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -478,16 +480,15 @@ template <int ELT> __global__ __launch_bounds__(kFewWaves * 64) void mx4_few_ker
       for (int q = 0; q < 2; ++q)
         acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(wf[c][q]), wide(xf[c][q]), acc, 4, 4, 0, (int)(cw[c][q] >> bw), 0,
                                                                (int)(cx[c][q] >> bx));
-    s += C * kFewWaves;
+    s += C * waves;
   };
-  while (s + 2 * kFewWaves < a.tiles) run(std::integral_constant<int, 3>{});
-  if (s + kFewWaves < a.tiles) run(std::integral_constant<int, 2>{});
+  while (s + 2 * waves < a.tiles) run(std::integral_constant<int, 3>{});
+  if (s + waves < a.tiles) run(std::integral_constant<int, 2>{});
   else if (s < a.tiles) run(std::integral_constant<int, 1>{});
   part[w][lane] = acc;
   __syncthreads();
   if (w > 0) return;
-#pragma unroll
-  for (int i = 1; i < kFewWaves; ++i) {
+  for (int i = 1; i < waves; ++i) {
     const f32x4 o = part[i][lane];
 #pragma unroll
     for (int v = 0; v < 4; ++v) acc[v] += o[v];
@@ -630,9 +631,10 @@ extern "C" int reels_hip_mx4_linear(const uint8_t* x, const uint8_t* x_scales, c
   const Mx4Args a{x, x_scales, w, w_scales, bias, residual, y, M, N, (int)ceil_div(K, 256), activation == REELS_HIP_ACT_GELU_TANH};
   if (M <= kFewTokens) {
     const int64_t grid = ceil_div(N, 16);
-    if (!grid_fits(grid, kFewWaves * 64)) return too_many();
+    const int waves = a.tiles < kFewWaves ? a.tiles : kFewWaves;  // 4 to 16 are within 2% of each other where there are as many lines
+    if (!grid_fits(grid, waves * 64)) return too_many();
     { TraceScope _ts(st, "mx4_few_kernel");
-      with_any_elt(dtype, [&](auto e) { mx4_few_kernel<decltype(e)::value><<<(unsigned)grid, kFewWaves * 64, 0, st>>>(a); }); }
+      with_any_elt(dtype, [&](auto e) { mx4_few_kernel<decltype(e)::value><<<(unsigned)grid, waves * 64, 0, st>>>(a); }); }
     return check_launch("mx4_few_kernel");
   }
   const int tile = tile_of(M, N, a.tiles);

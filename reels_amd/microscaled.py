@@ -5,6 +5,7 @@ with a sign. It has no gradient.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -21,6 +22,7 @@ def _padded(K: int) -> int:
     return -(-K // _TILE) * _TILE
 
 
+@functools.lru_cache(maxsize=4096)
 def _layout(M: int, K: int):
     """Shapes of the codes and of the scales."""
     return (M, _padded(K) // 2), (-(-M // 64), _padded(K) // _TILE, 512)
@@ -83,14 +85,16 @@ class MicroscaledMatrix:
 
 def _checked(q: MicroscaledMatrix, name: str) -> MicroscaledMatrix:
     """Types, shapes, device and alignment of the operand, dense."""
-    M, K = (int(n) for n in q.size)
+    M, K = q.size
     if M < 0 or K < 1:
         raise ValueError(f"{name} must have rows of at least one element, got size {(M, K)}")
     _need_device(q.codes, name)
     codes, scales = q.codes, q.scales
-    for t, n, shape in zip((codes, scales), ("codes", "scales"), _layout(M, K)):
-        if t.dtype != torch.uint8 or tuple(t.shape) != shape or t.device != codes.device:
-            raise ValueError(f"{n} of {name} must be uint8 of shape {shape} on one device, got {t.dtype} {tuple(t.shape)}")
+    want = _layout(M, K)
+    if (codes.dtype != torch.uint8 or codes.shape != want[0] or scales.dtype != torch.uint8 or scales.shape != want[1]
+            or scales.device != codes.device):
+        raise ValueError(f"{name} must have uint8 codes and scales of shapes {want} on one device, got {codes.dtype} "
+                         f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
         codes, scales = codes.contiguous(), scales.contiguous()
     if (codes.data_ptr() | scales.data_ptr()) & 15:

@@ -10,6 +10,7 @@ whole. Every call runs the HIP kernels on the current stream of the rows' device
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Union
 
@@ -50,43 +51,53 @@ class ModulatedNormGradients(NamedTuple):
     shift: Optional[torch.Tensor]
 
 
-def _groups(shape, t, name):
-    """How many rows of the modulation t the rows of `shape` have: 1, one for each sample, or one each."""
+@functools.lru_cache(maxsize=4096)  # a function of the shapes alone
+def _groups(shape, mod, name):
+    """How many rows a modulation of shape `mod` has for rows of `shape`: 1, one for each sample, or one each."""
     C = shape[-1]
-    if tuple(t.shape) == tuple(shape):
+    if mod == shape:
         return math.prod(shape[:-1])
-    if tuple(t.shape) == (C,) or (len(shape) == 2 and tuple(t.shape) == (1, C)):
+    if mod == (C,) or (len(shape) == 2 and mod == (1, C)):
         return 1
-    if len(shape) > 2 and tuple(t.shape) in ((shape[0], C), (shape[0],) + (1,) * (len(shape) - 2) + (C,)):
+    if len(shape) > 2 and mod in ((shape[0], C), (shape[0],) + (1,) * (len(shape) - 2) + (C,)):
         return shape[0]
     raise ValueError(f"{name} must have shape {(C,)}, one row for each sample or the rows' shape {tuple(shape)}, "
-                     f"got {tuple(t.shape)}")
+                     f"got {tuple(mod)}")
 
 
-def _modulations(shape, dt, device, **mods):
-    """({name: (tensor, row stride)}, type code, rows of a group) of the modulations that are given."""
-    given = {n: t for n, t in mods.items() if t is not None}
-    M, C = math.prod(shape[:-1]), shape[-1]
-    out, code = {n: (None, C) for n in mods}, _DTYPE_CODE[dt]
-    if not given:
-        return out, code, max(M, 1)
-    for n, t in given.items():
+def _modulations(x, dt, mods):
+    """([tensor or None, row stride] for each modulation one after the other, type code, rows of a group). mods:
+    (tensor or None, name) pairs. The tensors hold the memory until the launch."""
+    shape, dev, C = x.shape, x.device, x.shape[-1]
+    out, G, mt, first = [], None, dt, None
+    for t, name in mods:
+        if t is None:
+            out += (None, C)
+            continue
+        n = _groups(shape, t.shape, name)
         if t.dtype != dt and t.dtype != torch.float32:
-            raise TypeError(f"{n} must be {dt} or float32, got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{n} is on {t.device}, the rows on {device}")
-    kinds = {n: _groups(shape, t, n) for n, t in given.items()}
-    if len(set(kinds.values())) > 1 or len({t.dtype for t in given.values()}) > 1:
-        raise ValueError("gate, scale and shift must be of one kind and type, got "
-                         + ", ".join(f"{n} {tuple(t.shape)} {t.dtype}" for n, t in given.items()))
-    G = next(iter(kinds.values()))
-    for n, t in given.items():
-        t = t.reshape(G, C)
-        if C > 1 and t.stride(1) != 1:
-            t = t.contiguous()
-        out[n] = (t, t.stride(0) if G > 1 else C)
-        code = _DTYPE_CODE[t.dtype]
-    return out, code, max(M // G, 1) if G else 1
+            raise TypeError(f"{name} must be {dt} or float32, got {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the rows on {dev}")
+        if G is None:
+            G, mt, first = n, t.dtype, name
+        elif n != G or t.dtype != mt:
+            raise ValueError(f"gate, scale and shift must be of one kind and type; {name} is {tuple(t.shape)} "
+                             f"{t.dtype}, unlike {first}")
+        ld = C
+        if not t.is_contiguous():
+            t = t.reshape(G, C)
+            if C > 1 and t.stride(1) != 1:
+                t = t.contiguous()
+            ld = t.stride(0) if G > 1 else C
+        out += (t, ld)
+    M = x.numel() // C
+    return out, _DTYPE_CODE[mt], max(M // G, 1) if G else max(M, 1)
+
+
+@functools.lru_cache(maxsize=4096)  # a function of the sizes alone
+def _workspace_bytes(rows, cols, rows_per_group):
+    return _lib.lib().reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group)
 
 
 def _check_rows(x, name):
@@ -107,7 +118,7 @@ def _beside(t, like, dt, name):
 
 
 def _operands(x, scale, shift, branch, gate, eps):
-    """Checked arguments of a forward call, up to `center`; the sum; the rows and the tensors they lie in."""
+    """(type, the C arguments up to eps, the sum, x as it is read, the tensors that the arguments point into)."""
     dt = _check_rows(x, "x")
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and not negative")
@@ -116,16 +127,14 @@ def _operands(x, scale, shift, branch, gate, eps):
     if gate is not None and branch is None:
         raise ValueError("a gate needs a branch")
     _beside(branch, x, dt, "branch")
-    mods, code, rpg = _modulations(x.shape, dt, x.device, gate=gate, scale=scale, shift=shift)
+    held, code, rpg = _modulations(x, dt, ((gate, "gate"), (scale, "scale"), (shift, "shift")))
     C = x.shape[-1]
     xr, ld_x = _rows(x, C)
     br, ld_b = (None, C) if branch is None else _rows(branch, C)
-    args = [_ptr(xr), ld_x, _ptr(br), ld_b]
-    for n in ("gate", "scale", "shift"):
-        args += [_ptr(mods[n][0]), mods[n][1]]
-    s = x if branch is None else _like(x, xr)
-    held = (xr, br, mods)  # alive until the launch: copies of operands that did not lie well
-    return dt, args + [code, _DTYPE_CODE[dt], x.numel() // C, C, rpg, eps], s, xr, held
+    gt, ld_g, sc, ld_sc, sh, ld_sh = held
+    args = (xr.data_ptr(), ld_x, _ptr(br), ld_b, _ptr(gt), ld_g, _ptr(sc), ld_sc, _ptr(sh), ld_sh, code,
+            _DTYPE_CODE[dt], x.numel() // C, C, rpg, eps)
+    return dt, args, x if branch is None else _like(x, xr), xr, (br, held)
 
 
 def modulated_norm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
@@ -139,10 +148,13 @@ def modulated_norm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, shift:
     dev = x.device
     y = _like(x, xr)
     stats = torch.empty(x.shape[:-1] + (3,), dtype=torch.float32, device=dev)
-    kept, ptrs = None, [None] * 4
+    kept, ptrs = None, (None,) * 4
     if compress:
-        kept = KeptRows(*(None if t is None else activations._empty(x.shape, dt, dev) for t in (x, branch)))
-        ptrs = [_ptr(t) for k in kept for t in ((None, None) if k is None else (k.values, k.scales))]
+        a = activations._empty(x.shape, dt, dev)
+        b = None if branch is None else activations._empty(x.shape, dt, dev)
+        kept = KeptRows(a, b)
+        ptrs = (a.values.data_ptr(), a.scales.data_ptr()) + (
+            (None, None) if b is None else (b.values.data_ptr(), b.scales.data_ptr()))
     _launch("reels_hip_modulated_norm", dev, *args, int(center), None if branch is None else s.data_ptr(),
             y.data_ptr(), stats.data_ptr(), *ptrs, _stream(dev))
     del held
@@ -174,7 +186,7 @@ def modulated_norm_backward(dy: torch.Tensor, s: Union[torch.Tensor, CompressedA
     the gate); and, unless want_modulation is False, of scale, shift and (where the branch is given, kept
     like s) gate, summed in float32 over the rows that share them."""
     dt = _check_rows(dy, "dy")
-    if tuple(s.shape) != tuple(dy.shape):
+    if s.shape != dy.shape:
         raise ValueError(f"s must have shape {tuple(dy.shape)}, got {tuple(s.shape)}")
     kept = isinstance(s, CompressedActivations)
     dev, C = dy.device, dy.shape[-1]
@@ -187,7 +199,7 @@ def modulated_norm_backward(dy: torch.Tensor, s: Union[torch.Tensor, CompressedA
         _same_device(s, dy, "s")
         s, scales[0] = s.values, s.scales
         if want_gate:
-            if tuple(branch.shape) != tuple(dy.shape):
+            if branch.shape != dy.shape:
                 raise ValueError(f"branch must have shape {tuple(dy.shape)}, got {tuple(branch.shape)}")
             branch = activations._checked(branch, "branch")
             _same_device(branch, dy, "branch")
@@ -199,30 +211,32 @@ def modulated_norm_backward(dy: torch.Tensor, s: Union[torch.Tensor, CompressedA
             branch = branch.contiguous()
         s = s.contiguous()
     _beside(dsum, dy, dt, "dsum")
-    if tuple(stats.shape) != tuple(dy.shape[:-1]) + (3,):
+    if stats.shape[-1:] != (3,) or stats.shape[:-1] != dy.shape[:-1]:
         raise ValueError(f"stats must have shape {tuple(dy.shape[:-1]) + (3,)}, got {tuple(stats.shape)}")
     _same_device(stats, dy, "stats")
-    mods, code, rpg = _modulations(dy.shape, dt, dev, gate=gate, scale=scale)
+    held, code, rpg = _modulations(dy, dt, ((gate, "gate"), (scale, "scale")))
+    gt, ld_g, sc, ld_sc = held
     dy, stats = dy.contiguous(), _contig(stats, torch.float32, "stats")
     dsum = None if dsum is None else dsum.contiguous()
     M = dy.numel() // C
     dx = torch.empty_like(dy)
     db = dx if gate is None else torch.empty_like(dy)
 
-    def grad(t, want):
-        return torch.empty(t.shape, dtype=torch.float32, device=dev) if want and t is not None else None
-    dgate, dscale, dshift = grad(gate, want_gate), grad(scale, want_modulation), grad(scale, want_modulation)
+    f32 = torch.float32
+    dgate = torch.empty(gate.shape, dtype=f32, device=dev) if want_gate else None
+    dscale = dshift = None
+    if want_modulation and scale is not None:
+        dscale, dshift = torch.empty(scale.shape, dtype=f32, device=dev), torch.empty(scale.shape, dtype=f32, device=dev)
     ws, nbytes = None, 0
     if dgate is not None or dscale is not None:
         if M == 0:
             for t in (dgate, dscale, dshift):
                 if t is not None:
                     t.zero_()
-        nbytes = _lib.lib().reels_hip_modulated_norm_workspace_bytes(M, C, rpg)
+        nbytes = _workspace_bytes(M, C, rpg)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
     _launch("reels_hip_modulated_norm_bwd", dev, _ptr(dy), _ptr(s), _ptr(scales[0]), _ptr(dsum),
-            _ptr(branch) if want_gate else None, _ptr(scales[1]), _ptr(mods["gate"][0]), mods["gate"][1],
-            _ptr(mods["scale"][0]), mods["scale"][1], _ptr(stats), code, _DTYPE_CODE[dt], M, C, rpg,
+            _ptr(branch) if want_gate else None, _ptr(scales[1]), _ptr(gt), ld_g, _ptr(sc), ld_sc, _ptr(stats), code, _DTYPE_CODE[dt], M, C, rpg,
             int(center), _ptr(dx), None if gate is None else _ptr(db), _ptr(dgate), _ptr(dscale), _ptr(dshift),
             _ptr(ws), nbytes, _stream(dev))
     return ModulatedNormGradients(dx, db, dgate, dscale, dshift)

@@ -103,27 +103,30 @@ def test_mx4_c_refusals():
 
 
 def test_modulations_by_shape():
-    g = modulation._groups
-    assert g((3, 5, 8), torch.zeros(8), "m") == 1 and g((3, 5, 8), torch.zeros(3, 8), "m") == 3
-    assert g((3, 5, 8), torch.zeros(3, 1, 8), "m") == 3 and g((3, 5, 8), torch.zeros(3, 5, 8), "m") == 15
-    assert g((3, 2, 5, 8), torch.zeros(3, 1, 1, 8), "m") == 3 and g((4, 8), torch.zeros(1, 8), "m") == 1
-    assert g((4, 8), torch.zeros(4, 8), "m") == 4
+    def g(shape, t):
+        return modulation._groups(torch.Size(shape), torch.Size(t), "m")
+    assert g((3, 5, 8), (8,)) == 1 and g((3, 5, 8), (3, 8)) == 3
+    assert g((3, 5, 8), (3, 1, 8)) == 3 and g((3, 5, 8), (3, 5, 8)) == 15
+    assert g((3, 2, 5, 8), (3, 1, 1, 8)) == 3 and g((4, 8), (1, 8)) == 1
+    assert g((4, 8), (4, 8)) == 4
     for shape, t in (((3, 5, 8), (5, 8)), ((3, 5, 8), (1, 1, 8)), ((3, 5, 8), (3, 5, 1)), ((4, 8), (2, 8)), ((3, 5, 8), (7,)),
                      ((3, 5, 8), ())):
         with pytest.raises(ValueError):
-            g(shape, torch.zeros(t), "m")
-    mods = lambda **kw: modulation._modulations((3, 5, 8), BF, torch.device("cpu"), **kw)  # noqa: E731
+            g(shape, t)
+
+    def mods(gate, scale, shift=None):
+        return modulation._modulations(torch.zeros(3, 5, 8, dtype=BF), BF, ((gate, "gate"), (scale, "scale"), (shift, "shift")))
     six = torch.zeros(3, 6, 8)
-    out, code, rpg = mods(gate=six[:, 1:2], scale=six[:, 2], shift=None)
-    assert rpg == 5 and code == _lib.F32 and out["gate"][1] == 48 and out["scale"][1] == 48 and out["shift"][0] is None
-    assert out["gate"][0].data_ptr() == six[:, 1:2].data_ptr()  # taken as it lies
-    assert mods(gate=None, scale=torch.zeros(8, dtype=BF), shift=None)[1:] == (_lib.BF16, 15)
+    out, code, rpg = mods(six[:, 1:2], six[:, 2])
+    assert rpg == 5 and code == _lib.F32 and out[1] == 48 and out[3] == 48 and out[4] is None
+    assert out[0].data_ptr() == six[:, 1:2].data_ptr()  # taken as it lies
+    assert mods(None, torch.zeros(8, dtype=BF))[1:] == (_lib.BF16, 15)
     with pytest.raises(ValueError, match="one kind"):
-        mods(gate=torch.zeros(8), scale=torch.zeros(3, 8))
+        mods(torch.zeros(8), torch.zeros(3, 8))
     with pytest.raises(ValueError, match="one kind"):
-        mods(gate=torch.zeros(3, 8, dtype=BF), scale=torch.zeros(3, 8))
+        mods(torch.zeros(3, 8, dtype=BF), torch.zeros(3, 8))
     with pytest.raises(TypeError):
-        mods(gate=torch.zeros(8, dtype=torch.float16))
+        mods(torch.zeros(8, dtype=torch.float16), None)
 
 
 def test_python_refusals():
