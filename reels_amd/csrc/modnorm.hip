@@ -181,6 +181,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
       }
     } else {
       const int tiles = (at.cols + 255) / 256;
+      const double below = -mean * rstd;  // its rounding is 2^-53 of the mean over the spread
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         if (!at.some(i)) continue;
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
         for (int j = 0; j < V; ++j) {
           // the modulations stay in 32 bits between rows: as 64-bit values they take a workgroup's registers
           asm volatile("" : "+v"(up[i][j]), "+v"(shift[i][j]));
-          y[j] = (float)fma(((double)s[i].get(j) - mean) * rstd, 1.0 + (double)up[i][j], (double)shift[i][j]);
+          y[j] = (float)fma(fma((double)s[i].get(j), rstd, below), 1.0 + (double)up[i][j], (double)shift[i][j]);
         }
         if (!at.all(i)) {  // zeros up to the tile's end
 #pragma unroll

@@ -100,6 +100,12 @@ def _workspace_bytes(rows, cols, rows_per_group):
     return _lib.lib().reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group)
 
 
+def _gradient_of(t):
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, dtype=torch.float32, device=t.device)
+
+
 def _check_rows(x, name):
     dt = _act_dtype(x, name)
     if x.dim() < 2 or not 1 <= x.shape[-1] <= _MOST:
@@ -222,11 +228,10 @@ def modulated_norm_backward(dy: torch.Tensor, s: Union[torch.Tensor, CompressedA
     dx = torch.empty_like(dy)
     db = dx if gate is None else torch.empty_like(dy)
 
-    f32 = torch.float32
-    dgate = torch.empty(gate.shape, dtype=f32, device=dev) if want_gate else None
+    dgate = _gradient_of(gate) if want_gate else None
     dscale = dshift = None
     if want_modulation and scale is not None:
-        dscale, dshift = torch.empty(scale.shape, dtype=f32, device=dev), torch.empty(scale.shape, dtype=f32, device=dev)
+        dscale, dshift = _gradient_of(scale), _gradient_of(scale)
     ws, nbytes = None, 0
     if dgate is not None or dscale is not None:
         if M == 0:
