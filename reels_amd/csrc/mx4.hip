@@ -211,6 +211,12 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
     }
   };
   v4i w0[4], w1[4], x[TJ];
+  // TJ = 4: the bias of the wave's columns, asked for here and used after the products
+  typename Store<ELT>::raw bias = 0;
+  if (TJ == 4 && a.bias != nullptr) {
+    const int64_t n = n0 + wn * 64 + lane;
+    bias = ((const typename Store<ELT>::raw*)a.bias)[n < a.N ? n : a.N - 1];
+  }
   issue_scales(0, 0);
 #pragma unroll
   for (int q = 0; q < 8; ++q) issue(q >> 2, q & 3);
@@ -261,69 +267,140 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // no copy outlives the loop
   __syncthreads();
-  uint8_t* out = smem + w * 16384;
-  // Epilogue: f32 values of 64 tokens x 64 columns at a time in the wave's own 16 KiB of LDS (rows of
-  // 256 bytes, 16-byte chunks XOR-swizzled), read back as rows: bias, residual and stores in whole segments
-  constexpr int LPR = 64 / V, RPI = 64 / LPR, ITS = 64 / RPI;  // lanes of a row, rows at once, turns
-  const int c = (lane % LPR) * V, left = cols - (wn * 64 + c);
-  float bs[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) bs[v] = 0.0f;
-  if (a.bias != nullptr && left > 0) load_vec<ELT, V>((const uint8_t*)a.bias + (n0 + wn * 64 + c) * elt_bytes(ELT), left, bs);
-  const bool ahead = a.res != nullptr && a.M * a.N >= V;
-#pragma unroll
-  for (int h = 0; h < TJ / 4; ++h) {
-    // the residual's whole chunks on their way while the values are put in place; from its start where a
-    // lane has none
-    Chunk<ELT> res[ITS];
-    if (ahead) {
-#pragma unroll
-      for (int it = 0; it < ITS; ++it) {
-        const int mr = wm * 16 * TJ + h * 64 + it * RPI + lane / LPR;
-        const int64_t at = mr < rows && left >= V ? (m0 + mr) * a.N + n0 + wn * 64 + c : 0;
-        res[it].d = load_any<u32x4>((const typename Store<ELT>::raw*)((const uint8_t*)a.res + at * elt_bytes(ELT)));
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = j * 32 + l32;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4 o;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) o[v] = acc[i][h * 2 + j][q * 4 + v];
-          *reinterpret_cast<f32x4*>(out + r * 256 + (((i * 8 + q * 2 + hi) ^ (r & 15)) << 4)) = o;
-        }
-    }
+  if constexpr (TJ == 4) {
+    // Outputs straight from the registers (777 x 1000 -> 3001 in f32, whose rows lie at odd offsets: 10.6 us,
+    // by way of LDS 11.7): a lane has four columns each of its tokens; 16-bit types swap halves between lanes
+    // l and l + 32, so that each has eight columns (16 bytes), two lanes 32 bytes of a row
+    constexpr bool SWAP = V == 8;
+    constexpr int PER = 16 / V;  // chunks of a lane's 16 values of a product
+    const int64_t mrow = m0 + wm * 16 * TJ + l32, n1 = n0 + wn * 64;
+    const int here = (int)(a.N - n1 < 64 ? a.N - n1 : 64);  // columns of the wave that exist, or none
+    float* const biases = reinterpret_cast<float*>(smem) + w * 64;
+    asm volatile("" : "+v"(bias));  // its conversion stays here, behind the wait for it
+    biases[lane] = lane < here ? Store<ELT>::get(bias) : 0.0f;
     __builtin_amdgcn_s_waitcnt(0xC07F);
     asm volatile("" ::: "memory");
+    auto column = [&](int i, int p) { return i * 32 + (SWAP ? p * 16 + hi * 8 : p * 8 + hi * 4); };
+    auto leave = [&](auto all) {  // all: the wave's tokens and columns exist
+      constexpr bool ALL = decltype(all)::value;
 #pragma unroll
-    for (int it = 0; it < ITS; ++it) {
-      const int r = it * RPI + lane / LPR, mr = wm * 16 * TJ + h * 64 + r;
-      if (mr >= rows || left <= 0) continue;
-      float o[V];
+      for (int j = 0; j < JT; ++j) {
+        const bool row = ALL || mrow + j * 32 < a.M;
+        const int64_t at = (mrow + j * 32) * a.N + n1;
+        Chunk<ELT> res[2][PER];
+        if (a.res != nullptr) {
 #pragma unroll
-      for (int q = 0; q < V / 4; ++q) {
-        const f32x4 f = *reinterpret_cast<const f32x4*>(out + r * 256 + (((c / 4 + q) ^ (r & 15)) << 4));
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) o[q * 4 + v] = f[v] + bs[q * 4 + v];
+            for (int p = 0; p < PER; ++p) {
+              // whole chunks without a branch, all in flight together: from the residual's start where a lane has none
+              const int c = column(i, p);
+              const int64_t from = ALL || (row && c + V <= here) ? at + c : 0;
+              if (ALL || a.M * a.N >= V) res[i][p].load((const uint8_t*)a.res + from * elt_bytes(ELT), V);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int p = 0; p < PER; ++p) {
+            const int c = column(i, p);
+            float o[V];
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {  // groups of four columns
+              const int g4 = p * (V / 4) + q;
+              const f32x4 b = *reinterpret_cast<const f32x4*>(biases + i * 32 + g4 * 8 + hi * 4);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) o[q * 4 + v] = acc[i][j][g4 * 4 + v] + b[v];
+            }
+            if (a.gelu) {
+#pragma unroll
+              for (int v = 0; v < V; ++v) o[v] = gelu_logistic(o[v]);
+            }
+            if constexpr (SWAP) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[v]), __float_as_uint(o[4 + v]), false, false);
+                o[v] = __uint_as_float(sw[0]);
+                o[4 + v] = __uint_as_float(sw[1]);
+              }
+            }
+            if (a.res != nullptr) {
+              if (!ALL && row && c < here && c + V > here) res[i][p].load((const uint8_t*)a.res + (at + c) * elt_bytes(ELT), here - c);
+#pragma unroll
+              for (int v = 0; v < V; ++v) o[v] += res[i][p].get(v);
+            }
+            if (ALL || (row && c < here)) store_vec<ELT, V>((uint8_t*)a.y + (at + c) * elt_bytes(ELT), ALL ? V : here - c, o);
+          }
       }
-      if (a.gelu) {
+    };
+    if (here == 64 && m0 + (wm + 1) * 16 * TJ <= a.M) leave(std::true_type{});
+    else leave(std::false_type{});
+    return;
+  } else {
+    uint8_t* out = smem + w * 16384;
+    // Epilogue: f32 values of 64 tokens x 64 columns at a time in the wave's own 16 KiB of LDS (rows of
+    // 256 bytes, 16-byte chunks XOR-swizzled), read back as rows: bias, residual and stores in whole segments
+    constexpr int LPR = 64 / V, RPI = 64 / LPR, ITS = 64 / RPI;  // lanes of a row, rows at once, turns
+    const int c = (lane % LPR) * V, left = cols - (wn * 64 + c);
+    float bs[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = gelu_logistic(o[v]);
-      }
-      const int64_t at = (m0 + mr) * a.N + n0 + wn * 64 + c;
-      if (a.res != nullptr) {
-        if (left < V || !ahead) res[it].load((const uint8_t*)a.res + at * elt_bytes(ELT), left);
+    for (int v = 0; v < V; ++v) bs[v] = 0.0f;
+    if (a.bias != nullptr && left > 0) load_vec<ELT, V>((const uint8_t*)a.bias + (n0 + wn * 64 + c) * elt_bytes(ELT), left, bs);
+    const bool ahead = a.res != nullptr && a.M * a.N >= V;
 #pragma unroll
-        for (int v = 0; v < V; ++v) o[v] += res[it].get(v);
+    for (int h = 0; h < TJ / 4; ++h) {
+      // the residual's whole chunks on their way while the values are put in place; from its start where a
+      // lane has none
+      Chunk<ELT> res[ITS];
+      if (ahead) {
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int mr = wm * 16 * TJ + h * 64 + it * RPI + lane / LPR;
+          const int64_t at = mr < rows && left >= V ? (m0 + mr) * a.N + n0 + wn * 64 + c : 0;
+          res[it].d = load_any<u32x4>((const typename Store<ELT>::raw*)((const uint8_t*)a.res + at * elt_bytes(ELT)));
+        }
       }
-      store_vec<ELT, V>((uint8_t*)a.y + at * elt_bytes(ELT), left, o);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = j * 32 + l32;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            f32x4 o;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o[v] = acc[i][h * 2 + j][q * 4 + v];
+            *reinterpret_cast<f32x4*>(out + r * 256 + (((i * 8 + q * 2 + hi) ^ (r & 15)) << 4)) = o;
+          }
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const int r = it * RPI + lane / LPR, mr = wm * 16 * TJ + h * 64 + r;
+        if (mr >= rows || left <= 0) continue;
+        float o[V];
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          const f32x4 f = *reinterpret_cast<const f32x4*>(out + r * 256 + (((c / 4 + q) ^ (r & 15)) << 4));
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[q * 4 + v] = f[v] + bs[q * 4 + v];
+        }
+        if (a.gelu) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) o[v] = gelu_logistic(o[v]);
+        }
+        const int64_t at = (m0 + mr) * a.N + n0 + wn * 64 + c;
+        if (a.res != nullptr) {
+          if (left < V || !ahead) res[it].load((const uint8_t*)a.res + at * elt_bytes(ELT), left);
+#pragma unroll
+          for (int v = 0; v < V; ++v) o[v] += res[it].get(v);
+        }
+        store_vec<ELT, V>((uint8_t*)a.y + at * elt_bytes(ELT), left, o);
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // the rows have been read before the next half's are written
+      asm volatile("" ::: "memory");
     }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // the rows have been read before the next half's are written
-    asm volatile("" ::: "memory");
   }
 }
 
