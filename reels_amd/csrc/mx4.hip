@@ -625,14 +625,20 @@ int launch_small(const Mx4Args& a, int dtype, hipStream_t st) {
   return check_launch("mx4_small_kernel");
 }
 
+// The tiled form with the least estimated time, in microseconds: a workgroup's step of 256 codes takes 0.32 us
+// in the 64 x 64 form with one workgroup on a CU and 0.61 with two, 0.48 and 1.1 in the 128 x 128 form, 1.5 in the
+// 256 x 256 form (one on a CU); beginning and end 4.5, 5 and 6 us. Measured with every form, 64 / 128 / 256 (us):
+// 200 x 1536 -> 1536 7.8 / 8.4 / 15.7, 333 x 5120 -> 5120 16.8 / 15.6 / 32.9, 777 x 1024 -> 3001 11.9 / 9.8 / 15.0,
+// 512 x 4096 -> 10240 29.6 / 23.1 / 29.7, 1560 x 1536 -> 8960 40.3 / 25.0 / 22.6, 2048 x 5120 -> 5120 79.0 / 46.5 /
+// 38.4, 32760 x 1536 -> 1536 148 / 62.1 / 63.6.
 int tile_of(int64_t M, int64_t N, int64_t steps) {
   auto two = [](int64_t blocks, double one, double both) {  // two workgroups fit a CU
     const int64_t full = blocks / 512, rest = blocks % 512;
     return (double)full * both + (rest == 0 ? 0.0 : rest <= 256 ? one : both);
   };
-  const double t64 = 4.5 + steps * two(ceil_div(M, 64) * ceil_div(N, 64), 0.27, 0.55);
-  const double t128 = 4.0 + steps * two(ceil_div(M, 128) * ceil_div(N, 128), 0.75, 1.15);
-  const double t256 = 6.0 + steps * 1.35 * (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), 256);
+  const double t64 = 4.5 + steps * two(ceil_div(M, 64) * ceil_div(N, 64), 0.32, 0.61);
+  const double t128 = 5.0 + steps * two(ceil_div(M, 128) * ceil_div(N, 128), 0.48, 1.1);
+  const double t256 = 6.0 + steps * 1.5 * (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), 256);
   return t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
 }
 
