@@ -14,6 +14,8 @@
 // rounded to f32 before their codes are taken, so a code does not depend on the order of f32 operations.
 #include "modnorm.h"
 
+#include <algorithm>
+
 namespace reels {
 namespace {
 
@@ -229,8 +231,11 @@ int mod_forward(const char* fn, const char* label, int mode, ModArgs a, int dtyp
   a.per_col = 1.0 / (double)a.cols;
   const ModForm f = mod_form(dtype, a.cols);
   // Rows that follow each other in a wave or workgroup: as many as leave every one resident, one where
-  // each row has its own modulations
-  const int64_t per = f.tpr == 64 ? 4 : 1, resident = 256 * (16 * 64 / f.threads) * per;
+  // each row has its own modulations. Long rows take two workgroups a CU, where as many as fit queue for
+  // memory: 32760 x 5120 bf16 256 us with two, 283 with three, and to 4 bits 232 and 239; 4096 wide 195 with two
+  // and 206 with four. Shorter ones take all: 1536 wide 77 us with five, 81 with four, 113 with two.
+  const int64_t per = f.tpr == 64 ? 4 : 1, fit = 16 * 64 / f.threads;
+  const int64_t resident = 256 * (f.tpr == 0 && a.cols > 2048 && f.threads >= 256 ? std::min<int64_t>(fit, 2) : fit) * per;
   const int64_t run = a.rpg == 1 || a.rows < resident ? a.rows : resident, grid = ceil_div(run, per);
   if (!grid_fits(grid, f.threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
   { TraceScope _ts(st, label);
