@@ -79,9 +79,7 @@ extern "C" int reels_hip_modulated_norm_bwd(const void* dy, const void* s, const
   const int64_t groups = rows / rows_per_group;
   const bool sums = rows_per_group > 1 && (dgate != nullptr || dscale != nullptr);
   const int64_t walkers = f.tpr == 64 ? 4 : 1;
-  // without sums a workgroup's rows follow each other as in the forward
-  const ModParts p = sums ? mod_parts(groups, rows_per_group, f)
-                          : ModParts{1, rows};
+  const ModParts p = sums ? mod_parts(groups, rows_per_group, f) : ModParts{1, rows};  // without sums: a row each
   const int64_t parts = p.parts;
   if (parts > 1 && (workspace == nullptr || ws_bytes < reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group)))
     return fail(REELS_HIP_EWORKSPACE, std::string(fn) + ": workspace of reels_hip_modulated_norm_workspace_bytes required");

@@ -98,6 +98,8 @@ template <int ELT> __global__ __launch_bounds__(256) void mx4_unpack_kernel(cons
 }
 
 // ---- product -------------------------------------------------------------------------------------
+constexpr int kFewTokens = 16;  // up to these a kernel of its own
+
 struct Mx4Args {
   const uint8_t *x, *xs;  // codes [M][Kb], scale tiles
   const uint8_t *w, *ws;  // [N][Kb]
@@ -133,7 +135,8 @@ template <int SA, int SB> __device__ __forceinline__ f32x16 mfma(const v4i& a, c
 // are used up; behind the first products of step s, when every wave has the last fragments of step s in
 // registers, a barrier lets the copies of step s + 4 go into its stage, so a copy has three steps to arrive
 // (a step of 256 codes in two stages gave it three quarters of one: 1176 us). Scale words, two steps' worth, go
-// the same way in a ring of three. Rows past the edges read as zeros (the buffer's bounds), columns past K
+// the same way in a ring of three. Rows past the edges read as zeros (the buffer's bounds, which count the
+// scalar offset too and without a wrap), columns past K
 // are zeros in the codes; copies past the last step read nothing, so that every step's waits count the same.
 template <int TJ> struct Tile {
   static constexpr int NW = TJ, NT = NW * 64, WN = NW / 2, BM = 32 * TJ, BN = 64 * WN, BK = 64;
@@ -293,10 +296,11 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
-              // whole chunks without a branch, all in flight together: from the residual's start where a lane has none
+              // whole chunks without a branch, all in flight together: from the residual's start where a lane has
+              // none (more than kFewTokens tokens: it has V elements)
               const int c = column(i, p);
               const int64_t from = ALL || (row && c + V <= here) ? at + c : 0;
-              if (ALL || a.M * a.N >= V) res[i][p].load((const uint8_t*)a.res + from * elt_bytes(ELT), V);
+              res[i][p].load((const uint8_t*)a.res + from * elt_bytes(ELT), V);
             }
         }
 #pragma unroll
@@ -346,13 +350,12 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
 #pragma unroll
     for (int v = 0; v < V; ++v) bs[v] = 0.0f;
     if (a.bias != nullptr && left > 0) load_vec<ELT, V>((const uint8_t*)a.bias + (n0 + wn * 64 + c) * elt_bytes(ELT), left, bs);
-    const bool ahead = a.res != nullptr && a.M * a.N >= V;
 #pragma unroll
     for (int h = 0; h < TJ / 4; ++h) {
       // the residual's whole chunks on their way while the values are put in place; from its start where a
-      // lane has none
+      // lane has none (more than kFewTokens tokens: it has V elements)
       Chunk<ELT> res[ITS];
-      if (ahead) {
+      if (a.res != nullptr) {
 #pragma unroll
         for (int it = 0; it < ITS; ++it) {
           const int mr = wm * 16 * TJ + h * 64 + it * RPI + lane / LPR;
@@ -392,7 +395,7 @@ __global__ __launch_bounds__(Tile<TJ>::NT, 2) void mx4_tile_kernel(Mx4Args a, in
         }
         const int64_t at = (m0 + mr) * a.N + n0 + wn * 64 + c;
         if (a.res != nullptr) {
-          if (left < V || !ahead) res[it].load((const uint8_t*)a.res + at * elt_bytes(ELT), left);
+          if (left < V) res[it].load((const uint8_t*)a.res + at * elt_bytes(ELT), left);
 #pragma unroll
           for (int v = 0; v < V; ++v) o[v] += res[it].get(v);
         }
@@ -516,7 +519,7 @@ template <int ELT> __global__ __launch_bounds__(small::NT) void mx4_small_kernel
 // scale words straight into registers (each code of the weight is used once, so LDS would only add a trip),
 // then add their sums in LDS in wave order. Lanes of tokens that are not there read nothing (an offset past the
 // buffer's bounds). Bound by the weight's bytes and by latency.
-constexpr int kFewTokens = 16, kFewWaves = 8;  // the most waves of a workgroup
+constexpr int kFewWaves = 8;  // the most of a workgroup
 
 template <int ELT> __global__ __launch_bounds__(kFewWaves * 64) void mx4_few_kernel(Mx4Args a) {
   __shared__ f32x4 part[kFewWaves][64];

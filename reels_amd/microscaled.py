@@ -33,7 +33,8 @@ class MicroscaledMatrix:
     """A matrix ``[M][K]`` in 4 bits. codes: uint8 ``[M][Kp / 2]``, K padded with zeros to a multiple of
     256, the even column in the low half of a byte. scales: uint8 ``[ceil(M / 64)][Kp / 256][512]``, the
     exponent + 127 of each block's power of two (255: the block held NaN or an infinity, its values are
-    NaN), in the order in which the matrix cores take them (``block_scales`` gives them by rows).
+    NaN), in the order in which the matrix cores take them (``block_scales`` gives them by rows; what stands
+    in the places of rows past M is never used).
     compute_dtype: the type of what is made from it."""
 
     codes: torch.Tensor
@@ -64,7 +65,7 @@ class MicroscaledMatrix:
     def block_scales(self) -> torch.Tensor:
         """The scales by rows, uint8 ``[M][ceil(K / 32)]``."""
         M, K = self.shape
-        tiles = self.scales.view(-1, _padded(K) // _TILE, 2, 32, 4, 2).permute(0, 5, 3, 1, 4, 2)
+        tiles = self.scales.reshape(-1, _padded(K) // _TILE, 2, 32, 4, 2).permute(0, 5, 3, 1, 4, 2)
         return tiles.reshape(-1, _padded(K) // _BLOCK)[:M, :-(-K // _BLOCK)].contiguous()
 
     @staticmethod

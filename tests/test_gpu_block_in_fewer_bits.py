@@ -101,3 +101,45 @@ def test_training_with_activations_in_8_bits(dev):
     k = ra.compress_activations(t["x"])
     assert k.values.nbytes + k.scales.nbytes == t["x"].numel() * 33 // 32
     assert torch.equal(k.restore().view(-1, C).double(), blocks8(t["x"].double().view(-1, C))[2])
+
+
+def test_two_threads_on_two_streams(dev):
+    """Calls of two threads at once, each on its own stream, with operands of its own."""
+    import threading
+    from reels_amd import _lib
+    cases = []
+    for seed, size in ((1, dict(S=150, C=320, H=900)), (2, dict(S=77, C=1000, H=260))):
+        t = make(dev, seed=seed, **size)
+        w1 = ra.quantize_microscaled(t["w1"])
+        shift, scale, gate = (t["six"][:, i:i + 1] for i in range(3))
+        dy = t["rnd"](t["B"], t["S"], t["C"]).to(BF)
+
+        def work(t=t, w1=w1, shift=shift, scale=scale, gate=gate, dy=dy):
+            n = ra.modulated_norm_quantized(t["x"], scale, shift, branch=t["attn"], gate=gate)
+            h, kept = ra.gelu_tanh_compressed(ra.microscaled_linear(n.output, w1, t["b1"]))
+            r = ra.modulated_norm(t["x"], scale, shift, branch=t["attn"], gate=gate, compress=True)
+            g = ra.modulated_norm_backward(dy, r.kept.sum, r.stats, scale, branch=r.kept.branch, gate=gate)
+            return [h, kept.restore(), ra.gelu_tanh_backward(kept, h), r.output] + list(g)
+        cases.append(work)
+    want = [f() for f in cases]
+    torch.cuda.synchronize()
+    errors = []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = cases[i]()
+                torch.cuda.current_stream().synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+            # a refused call's message belongs to the thread that made it
+            assert _lib.lib().reels_hip_act8_keep(None, 1, 1 if i else -1, 8, None, None, None) != 0
+            assert ("NULL" in _lib.lib().reels_hip_last_error().decode()) == bool(i)
+        except BaseException as e:
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

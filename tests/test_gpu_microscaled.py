@@ -166,7 +166,7 @@ def test_other_stream_and_graph(dev):
 
 def test_offsets_past_32_bits(dev):
     """Codes of more than 2^32 bytes and outputs past 2^32 elements: the last rows are those of a small call."""
-    K, N = 13824, 1030
+    K, N = 13824, 7001
     x = quantize_microscaled(torch.randn(128, K, device=dev).bfloat16())
     w = quantize_microscaled(torch.randn(N, K, device=dev).bfloat16())
     times = 5000  # 640000 rows: 4.4 GB of codes

@@ -391,3 +391,67 @@ def test_kept_rows_of_another_shape(dev):
         modulated_norm_backward(t["dy"], r.kept.sum, r.stats, m["scale"], t["branch"], m["gate"])
     with pytest.raises(ValueError, match="shape"):
         modulated_norm_backward(t["dy"], CompressedActivations(r.kept.sum.values[:1], r.kept.sum.scales[:1]), r.stats)
+
+
+def test_gradients_of_an_ungated_branch_are_two_tensors(dev):
+    """x and the branch have one gradient; what is done to one leaf's does not reach the other's."""
+    t, m = make(2, 6, 64, "bf16", "f32", "sample")
+    x, b = t["x"].clone().requires_grad_(), t["branch"].clone().requires_grad_()
+    y, s = ModulatedNormFunction.apply(x, m["scale"], m["shift"], b, None)
+    torch.autograd.backward((y, s), (t["dy"], t["dsum"]))
+    assert torch.equal(x.grad, b.grad)
+    keep = b.grad.clone()
+    x.grad.zero_()
+    assert torch.equal(b.grad, keep)
+    both = t["x"].clone().requires_grad_()  # one tensor as x and as the branch
+    y, s = ModulatedNormFunction.apply(both, m["scale"], m["shift"], both, m["gate"])
+    (d,) = torch.autograd.grad((y, s), both, (t["dy"], t["dsum"]))
+    r = modulated_norm(t["x"], m["scale"], m["shift"], t["x"], m["gate"])
+    g = modulated_norm_backward(t["dy"], r.sum, r.stats, m["scale"], t["x"], m["gate"], t["dsum"])
+    assert torch.equal(d, g.x + g.branch)
+
+
+def test_rows_without_spread(dev):
+    """Equal elements: the shift with a positive eps; 0 / 0 without one."""
+    x = torch.full((4, 96), 3.25, device=dev)
+    x[2:, 1] = 4.0
+    shift = torch.randn(96, device=dev)
+    y = modulated_norm(x, torch.zeros(96, device=dev), shift).output
+    assert torch.equal(y[0], shift) and torch.isfinite(y).all()
+    r = modulated_norm(x, eps=0.0)
+    assert torch.isnan(r.output[:2]).all() and torch.isfinite(r.output[2:]).all()
+    c = x[2:].double() - x[2:].double().mean(-1, keepdim=True)
+    want = c / c.square().mean(-1, keepdim=True).sqrt()
+    assert_within(r.output[2:], want, 7 * U * want.abs(), "without eps")
+
+
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 elements: the last rows are those of a small call, and so are the sums where all other
+    rows' gradients are zero (bound: the roundings of 64 additions in another order)."""
+    M, C, tail = 140000, 16384, 40
+    assert M * C > 2 ** 31
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn(M, C, generator=g, device=dev, dtype=torch.bfloat16)
+    b = torch.randn(M, C, generator=g, device=dev, dtype=torch.bfloat16)
+    dy = torch.zeros_like(x)
+    dy[-tail:] = torch.randn(tail, C, generator=g, device=dev).bfloat16()
+    gate, scale, shift = (torch.randn(C, generator=g, device=dev) for _ in range(3))
+
+    def ends(t):
+        return t[-tail:]
+    r = modulated_norm(x, scale, shift, b, gate, compress=True)
+    w = modulated_norm(ends(x), scale, shift, ends(b), gate, compress=True)
+    for u, v in ((r.output, w.output), (r.sum, w.sum), (r.stats, w.stats), (r.kept.sum.values, w.kept.sum.values),
+                 (r.kept.sum.scales, w.kept.sum.scales), (r.kept.branch.values, w.kept.branch.values)):
+        assert torch.equal(ends(u), v)
+    for s, sb, ws, wb in ((r.sum, b, w.sum, ends(b)), (r.kept.sum, r.kept.branch, w.kept.sum, w.kept.branch)):
+        d = modulated_norm_backward(dy, s, r.stats, scale, sb, gate)
+        e = modulated_norm_backward(ends(dy), ws, w.stats, scale, wb, gate)
+        assert torch.equal(ends(d.x), e.x) and torch.equal(ends(d.branch), e.branch) and not d.x[:-tail].any()
+        n = (w.sum.double() - (w.stats[:, :1] + w.stats[:, 1:2]).double()) * w.stats[:, 2:].double()
+        for name, mag in (("shift", ends(dy).double().abs()), ("scale", ends(dy).double().abs() * (n.abs() + 0.1)),
+                          ("gate", (e.x.double().abs() + 1e-2) * (ends(b).double().abs() + 0.1))):
+            assert_within(getattr(d, name), getattr(e, name).double(), 128 * U * mag.sum(0), name)
+    q = modulated_norm_quantized(x, scale, shift, b, gate)
+    p = modulated_norm_quantized(ends(x), scale, shift, ends(b), gate)
+    assert torch.equal(ends(q.output.codes), p.output.codes) and torch.equal(ends(q.output.block_scales()), p.output.block_scales())
