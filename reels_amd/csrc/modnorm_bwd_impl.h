@@ -12,6 +12,10 @@ template <int ELT, int TPR, int NCH, int KIND, bool KEPT> struct Held {
   }
   __device__ __forceinline__ void trim(const ModRow<ELT, TPR, NCH, KIND>& at) { at.trim(d); }
   __device__ __forceinline__ float get(int i, int j) const { return d[i].get(j); }
+  __device__ __forceinline__ void hold() {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) d[i].hold();
+  }
 };
 template <int ELT, int TPR, int NCH, int KIND> struct Held<ELT, TPR, NCH, KIND, true> {
   static constexpr int V = Chunk<ELT>::V;
@@ -43,9 +47,15 @@ template <int ELT, int TPR, int NCH, int KIND> struct Held<ELT, TPR, NCH, KIND, 
     }
   }
   __device__ __forceinline__ float get(int i, int j) const { return d[i].get(j); }
+  __device__ __forceinline__ void hold() {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) asm volatile("" : "+v"(d[i].d[j]));
+  }
 };
 
-// A wave or workgroup walks rows begin .. end of one group, the next row's operands on their way meanwhile.
+// A wave or workgroup walks rows begin .. end of one group.
 // SUMS: it leaves the sums of the modulations' gradients over them; otherwise (no such gradient, or groups
 // of one row) rows of several groups may follow each other.
 template <int ELT, int TPR, int NCH, int NT, int KIND, bool KEPT, bool SUMS>
@@ -53,9 +63,15 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
   constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), WALKERS = TPR == 0 ? 1 : 4;
   __shared__ double slots[2][16][2];
   __shared__ float acc[SUMS && WALKERS > 1 ? WALKERS * 64 * NCH * V : 1];
-  // A thread's gates wait in LDS until a row's end: with the sums they do not fit three waves' registers
-  constexpr bool AWAY = SUMS && NT == 512;
-  __shared__ f32x4 gates[AWAY ? NCH * V / 4 : 1][AWAY ? NT : 1];
+  // A thread's gates wait in LDS until a row's end: with the sums they do not fit three waves' registers. Rows
+  // past 8192 elements have one workgroup a CU, 128 registers and all of its LDS: 1 + scale is there, too.
+  constexpr bool AWAY = (SUMS && NT == 512) || NT == 1024, UP_AWAY = NT == 1024;
+  // The next row's s and dy are on their way while a row is worked on where the registers hold them (three waves
+  // on a SIMD have 168 each), otherwise they are asked for at the row's end: 8000 x 13824 bf16 617 us with both
+  // rows and the modulations in registers, 288 so; 4000 x 5120 f32 124 and 113, kept 137 and 100; 8000 x 5120
+  // bf16 112 with the next row on its way, 115 without.
+  constexpr bool AHEAD = NT < 512 || (NT == 512 && ELT != REELS_HIP_F32 && !(KEPT && KIND == kAny));
+  __shared__ f32x4 gates[AWAY ? NCH * V / 4 : 1][AWAY ? NT : 1], ups[UP_AWAY ? NCH * V / 4 : 1][UP_AWAY ? NT : 1];
   const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
   const int sub = TPR == 0 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // rows in 32 bits, so that they and what follows from them stay in scalar registers
@@ -69,8 +85,8 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
 #pragma unroll
       for (int j = 0; j < V; ++j) tg[i][j] = tc[i][j] = th[i][j] = 0.0f;
   }
-  // s and dy of the next row are on their way while a row is worked on, its own branch and dsum until they are
-  // needed after the row's sums (all four a row ahead take 47 registers more than three waves on a SIMD have)
+  // a row's branch and dsum are on their way until they are needed after its sums (with these a row ahead, too,
+  // 47 registers more than three waves on a SIMD have)
   struct Data {
     Held<ELT, TPR, NCH, KIND, KEPT> s;
     Chunk<ELT> dy[NCH];
@@ -96,6 +112,21 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) up[i][j] = gate[i][j] = 1.0f;
+  auto put = [&](auto& lds, const float (&f)[NCH][V]) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int j = 0; j < V; j += 4) lds[(i * V + j) / 4][threadIdx.x] = f32x4{f[i][j], f[i][j + 1], f[i][j + 2], f[i][j + 3]};
+  };
+  auto take = [&](const auto& lds, int i, float (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const f32x4 v = lds[(i * V + j) / 4][threadIdx.x];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[j + q] = v[q];
+    }
+  };
+  if constexpr (UP_AWAY) put(ups, up);
   uint32_t change = begin;
   int turn = 0;
   for (uint32_t r = begin; r < end; r += run, turn ^= 1) {
@@ -109,16 +140,11 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) up[i][j] += 1.0f;
+        if constexpr (UP_AWAY) put(ups, up);
       }
       if (a.gate != nullptr) {
         at.mods(a.gate, a.ld_gate, a.m_f32, group, gate);
-        if constexpr (AWAY) {
-#pragma unroll
-          for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int j = 0; j < V; j += 4)
-              gates[(i * V + j) / 4][threadIdx.x] = f32x4{gate[i][j], gate[i][j + 1], gate[i][j + 2], gate[i][j + 3]};
-        }
+        if constexpr (AWAY) put(gates, gate);
       }
       __builtin_amdgcn_s_waitcnt(0x0F70);  // here, and not at each row's use
     }
@@ -126,7 +152,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
     Chunk<ELT> ds[NCH];
     b.load(at, branch, bs, row);
     at.load((const uint8_t*)dsum + at0, ds);
-    load(r + run, next);
+    if constexpr (AHEAD) load(r + run, next);
     cur.s.trim(at);
     at.trim(cur.dy);
     const float hi = cur.hi, rstd = cur.rstd, k = -cur.lo * rstd;
@@ -134,10 +160,11 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
     // dy is zero where the thread has no element, and so are its shares of the sums
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      float p0 = 0.0f, p1 = 0.0f, up1[V];
+      float p0 = 0.0f, p1 = 0.0f, up1[V], u[V];
+      if constexpr (UP_AWAY) take(ups, i, u);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = cur.dy[i].get(j), n = fmaf(cur.s.get(i, j) - hi, rstd, k), g = d * up[i][j];
+        const float d = cur.dy[i].get(j), n = fmaf(cur.s.get(i, j) - hi, rstd, k), g = d * (UP_AWAY ? u[j] : up[i][j]);
         p0 += g;
         p1 = fmaf(g, n, p1);
         if constexpr (SUMS) {
@@ -163,12 +190,13 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
     const float m0 = a.center ? (float)(g0 * a.per_col) : 0.0f, m1 = (float)(g1 * a.per_col);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      float d[V];
+      float d[V], u[V];
       Chunk<ELT> o;
+      if constexpr (UP_AWAY) take(ups, i, u);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float n = fmaf(cur.s.get(i, j) - hi, rstd, k);
-        const float t = fmaf(-n, m1, fmaf(cur.dy[i].get(j), up[i][j], -m0));
+        const float t = fmaf(-n, m1, fmaf(cur.dy[i].get(j), UP_AWAY ? u[j] : up[i][j], -m0));
         d[j] = a.dsum != nullptr ? fmaf(rstd, t, ds[i].get(j)) : rstd * t;
       }
       o.pack(d);
@@ -189,7 +217,8 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
         at.store((uint8_t*)a.db + at0, i, o);
       }
     }
-    cur = next;
+    if constexpr (AHEAD) cur = next;
+    else load(r + run, cur);
   }
   if constexpr (SUMS) {
     auto leave = [&](float (&v)[NCH][V], float* whole, int which) {

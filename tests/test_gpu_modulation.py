@@ -290,6 +290,21 @@ def test_many_rows(dev):
         check_backward(g, t, r.sum.double(), t["branch"].double(), r.stats, m["gate"], m["scale"], t["dsum"], True, B, S)
 
 
+@pytest.mark.parametrize("compress", [False, True])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("C", [130, 515, 1536, 5120, 5125, 8200, 16384])
+def test_many_rows_of_each_form(dev, C, dtype, compress):
+    """Several rows one after the other in every wave or workgroup, in two groups."""
+    B, S = 2, 2500 if C < 5000 else 1100
+    t, m = make(B, S, C, dtype, "f32", "sample")
+    r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], EPS, True, compress)
+    check_forward(r, t["x"], t["branch"], m["gate"], m["scale"], m["shift"], True, B)
+    s, b = (r.kept.sum, r.kept.branch) if compress else (r.sum, t["branch"])
+    sd, bd = (v.restore(torch.float32).double() if compress else v.double() for v in (s, b))
+    g = modulated_norm_backward(t["dy"], s, r.stats, m["scale"], b, m["gate"], t["dsum"])
+    check_backward(g, t, sd, bd, r.stats, m["gate"], m["scale"], t["dsum"], True, B, S)
+
+
 def test_empty(dev):
     for shape in ((0, 5, 40), (3, 0, 40), (0, 40)):
         x = torch.empty(shape, device=dev)
