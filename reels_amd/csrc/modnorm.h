@@ -115,14 +115,29 @@ template <int ELT, int TPR, int NCH, int KIND> struct ModRow {
     if (all(i)) store_vec<REELS_HIP_F32, V>(row + (uint32_t)col(i), V, f);
     else if (left(i) > 0) store_vec<REELS_HIP_F32, V>(row + (uint32_t)col(i), left(i), f);
   }
-  // a row of modulations in f32 (or the rows' type), zeros where the thread has no element
+  // a row of modulations in f32 (or the rows' type), zeros where the thread has no element; read like the rows
   __device__ __forceinline__ void mods(const void* p, int64_t ld, int f32, int64_t group, float (&f)[NCH][V]) const {
     const uint8_t* r = (const uint8_t*)p + group * ld * (f32 ? 4 : EB);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int l = all(i) ? V : left(i) > 0 ? left(i) : 0, at = l > 0 ? col(i) : 0;
-      if (f32) load_vec<REELS_HIP_F32, V>((const float*)r + (uint32_t)at, l, f[i]);
-      else load_vec<ELT, V>(r + (uint32_t)(at * EB), l, f[i]);
+      int l = left(i);
+      asm volatile("" : "+v"(l));  // what follows from it is not kept between rows
+      const uint32_t at = KIND == kEven || l >= V ? (uint32_t)(cols - l) : KIND == kAny && l > 0 ? (uint32_t)(cols - V) : KIND == kTiny && l > 0 ? (uint32_t)(cols - l) : 0u;
+      const int n = KIND == kTiny ? (l < 0 ? 0 : l) : V;
+      if (f32) load_vec<REELS_HIP_F32, V>((const float*)r + at, n, f[i]);
+      else load_vec<ELT, V>(r + at * EB, n, f[i]);
+    }
+    if constexpr (KIND != kAny) return;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      if (all(i)) continue;
+      const int l = left(i), by = l < V ? V - l : 0;
+#pragma unroll
+      for (int s = V / 2; s > 0; s /= 2)
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[i][j] = by & s ? (j + s < V ? f[i][j + s] : 0.0f) : f[i][j];
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[i][j] = l > 0 ? f[i][j] : 0.0f;
     }
   }
 };

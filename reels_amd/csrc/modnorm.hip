@@ -39,8 +39,9 @@ __device__ __forceinline__ void keep_chunk(const float (&f)[V], int8_t* codes, u
   if (col >= cols) return;
   uint32_t word[V / 4];
   mx8_codes<V>(f, byte, word);
-  mx8_store<V>(codes + row * cols + col, cols - col, word);
-  if (col % kMxBlock == 0) scales[row * ((cols + kMxBlock - 1) / kMxBlock) + col / kMxBlock] = (uint8_t)byte;
+  // 32-bit offsets from scalar bases
+  mx8_store<V>(codes + row * cols + (uint32_t)col, cols - col, word);
+  if (col % kMxBlock == 0) (scales + row * ((cols + kMxBlock - 1) / kMxBlock))[(uint32_t)col / kMxBlock] = (uint8_t)byte;
 }
 
 // MODE 0: y; 1: y and the kept rows; 2: y's rows in 4 bits. A wave or workgroup walks `run` rows one after the
@@ -49,6 +50,8 @@ __device__ __forceinline__ void keep_chunk(const float (&f)[V], int8_t* codes, u
 template <int ELT, int TPR, int NCH, int NT, int KIND, int MODE>
 __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1) void mod_kernel(ModArgs a, uint32_t run) {
   constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT);
+  // f32 rows past 8192 elements leave no registers for the next row, which is asked for at a row's end
+  constexpr bool AHEAD = !(NT == 1024 && ELT == REELS_HIP_F32);
   __shared__ double slots[2][16][2];
   const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
   // rows in 32 bits, so that they and what follows from them stay in scalar registers
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
       }
       __builtin_amdgcn_s_waitcnt(0x0F70);  // here, and not at each row's use
     }
-    load(r + run, next);
+    if constexpr (AHEAD) load(r + run, next);
     // the sum, and its first element, which every thread forms for itself
     Chunk<ELT>(&s)[NCH] = cur.x;  // no branch: the row itself
     float s0 = Store<ELT>::get(cur.x0);
@@ -202,13 +205,14 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
         const int col = at.col(i);
         if (col >= tiles * 256) continue;
         const uint32_t word = mx4_codes<V>(y, byte);
-        uint8_t* p = a.codes + row * tiles * 128 + col / 2;
+        uint8_t* p = a.codes + row * tiles * 128 + (uint32_t)col / 2;
         if constexpr (V == 8) *reinterpret_cast<uint32_t*>(p) = word;
         else *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
-        if (col % kMxBlock == 0) a.scales[mx4_scale_at(row, col / kMxBlock, tiles)] = (uint8_t)byte;
+        if (col % kMxBlock == 0) (a.scales + (row >> 6) * tiles * 512)[(uint32_t)mx4_scale_at(row & 63, col / kMxBlock, tiles)] = (uint8_t)byte;
       }
     }
-    cur = next;
+    if constexpr (AHEAD) cur = next;
+    else load(r + run, cur);
   }
 }
 
