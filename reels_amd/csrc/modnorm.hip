@@ -233,7 +233,7 @@ int mod_forward(const char* fn, const char* label, int mode, ModArgs a, int dtyp
   if (mode == 2 && ((uintptr_t)a.codes & 3) != 0) return fail(REELS_HIP_EINVAL, std::string(fn) + ": codes must be 4-byte aligned");
   a.m_f32 = m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32;
   a.per_col = 1.0 / (double)a.cols;
-  const ModForm f = mod_form(dtype, a.cols);
+  const ModForm f = mod_form(dtype, a.rows, a.cols);
   // Rows that follow each other in a wave or workgroup: as many as leave every one resident, one where
   // each row has its own modulations. Long rows take two workgroups a CU, where as many as fit queue for
   // memory: 32760 x 5120 bf16 256 us with two, 283 with three, and to 4 bits 232 and 239; 4096 wide 195 with two

@@ -50,7 +50,7 @@ extern "C" size_t reels_hip_modulated_norm_workspace_bytes(int64_t rows, int64_t
   const int64_t groups = ceil_div(rows, rows_per_group);
   int64_t n = 0;
   for (int elt : {REELS_HIP_F32, REELS_HIP_BF16}) {  // the most of any element type
-    const int64_t p = mod_parts(groups, rows_per_group, mod_form(elt, cols)).parts;
+    const int64_t p = mod_parts(groups, rows_per_group, mod_form(elt, rows, cols)).parts;
     n = p > n ? p : n;
   }
   return n <= 1 ? 0 : align_up((size_t)(groups * n) * 3 * (size_t)cols * 4, 256);
@@ -75,7 +75,7 @@ extern "C" int reels_hip_modulated_norm_bwd(const void* dy, const void* s, const
   if (dgate != nullptr && (s_scales == nullptr) != (branch_scales == nullptr))
     return fail(REELS_HIP_EINVAL, std::string(fn) + ": s and branch are both kept in 8 bits or neither");
   if (dy == nullptr || s == nullptr || stats == nullptr || dx == nullptr) return fail(REELS_HIP_EINVAL, std::string(fn) + ": NULL operand");
-  const ModForm f = mod_form(dtype, cols);
+  const ModForm f = mod_form(dtype, rows, cols);
   const int64_t groups = rows / rows_per_group;
   const bool sums = rows_per_group > 1 && (dgate != nullptr || dscale != nullptr);
   const int64_t walkers = f.tpr == 64 ? 4 : 1;

@@ -292,7 +292,7 @@ def test_many_rows(dev):
 
 @pytest.mark.parametrize("compress", [False, True])
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("C", [130, 515, 1536, 5120, 5125, 8200, 16384])
+@pytest.mark.parametrize("C", [130, 515, 1000, 1536, 5120, 5125, 8200, 16384])
 def test_many_rows_of_each_form(dev, C, dtype, compress):
     """Several rows one after the other in every wave or workgroup, in two groups."""
     B, S = 2, 2500 if C < 5000 else 1100
