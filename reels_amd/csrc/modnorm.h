@@ -4,21 +4,26 @@
 
 namespace reels {
 
-// Who has a row: a wave (tpr 64, four rows to a workgroup; rows of up to 512 elements), or a workgroup of
-// `threads` (tpr 0) with nch chunks of 16 bytes a thread. 8 elements a thread up to four waves (three waves
+// Who has a row: 16 lanes (tpr 16; rows of up to 256 elements), a wave (tpr 64; up to 512), or a workgroup of
+// `threads` (tpr 0), with nch chunks of 16 bytes a thread. 8 elements a thread up to four waves (three waves
 // at 1536 leave no lane idle), then 16, up to 16 waves. Where there are rows enough a wave has up to 1024
 // elements, 16 a lane: 58514 x 700 bf16 75 us and 98 with two waves to a row, to 4 bits 78 and 94; 3000 x 700
-// forward 10.1 and 9.8, backward 20 and 24; 300 x 700 7.4 and 6.5, 16 and 15.
+// forward 10.1 and 9.8, backward 20 and 24; 300 x 700 7.4 and 6.5, 16 and 15. A wave to a row of 64 is bound by
+// the row's instructions: 131040 x 64 bf16 70 us, 16 lanes
+// 22; 131040 x 200 72 and 38.
 struct ModForm { int tpr, nch, threads; };
 constexpr int64_t kModCols = 16384;  // the longest row
 inline ModForm mod_form(int elt, int64_t rows, int64_t cols) {
   const int64_t waves = ceil_div(cols, 512);
   const int per = elt == REELS_HIP_F32 ? 2 : 1;
+  if (cols <= 256) return {16, cols <= 128 ? per : 2 * per, 256};
   if (waves <= 1) return {64, per, 256};
   if (waves == 2 && rows >= 2048) return {64, 2 * per, 256};
   if (waves <= 4) return {0, per, (int)waves * 64};
   return {0, 2 * per, (int)ceil_div(waves, 2) * 64};
 }
+// rows of a workgroup at once
+inline int64_t mod_walkers(ModForm f) { return f.tpr == 0 ? 1 : f.threads / f.tpr; }
 // How the chunks of a row fall on its threads: every thread has whole ones, or some have a part or none, or
 // the row is shorter than a chunk
 enum ModKind { kEven = 0, kAny = 1, kTiny = 2 };
@@ -28,10 +33,12 @@ template <int N> using ModInt = std::integral_constant<int, N>;
 template <int ELT, typename F> void with_mod_form(ModForm f, int64_t cols, F&& g) {
   constexpr int P = ELT == REELS_HIP_F32 ? 2 : 1, V = Chunk<ELT>::V;
   auto kind = [&](auto tpr, auto nch, auto nt) {
-    if (cols == (int64_t)(f.tpr == 0 ? f.threads : 64) * f.nch * V) g(tpr, nch, nt, ModInt<kEven>{});
+    if (cols == (int64_t)(f.tpr == 0 ? f.threads : f.tpr) * f.nch * V) g(tpr, nch, nt, ModInt<kEven>{});
     else g(tpr, nch, nt, ModInt<kAny>{});
   };
-  if (cols < V) g(ModInt<64>{}, ModInt<P>{}, ModInt<256>{}, ModInt<kTiny>{});
+  if (cols < V) g(ModInt<16>{}, ModInt<P>{}, ModInt<256>{}, ModInt<kTiny>{});
+  else if (f.tpr == 16 && f.nch == P) kind(ModInt<16>{}, ModInt<P>{}, ModInt<256>{});
+  else if (f.tpr == 16) kind(ModInt<16>{}, ModInt<2 * P>{}, ModInt<256>{});
   else if (f.tpr == 64 && f.nch == P) kind(ModInt<64>{}, ModInt<P>{}, ModInt<256>{});
   else if (f.tpr == 64) kind(ModInt<64>{}, ModInt<2 * P>{}, ModInt<256>{});
   else if (f.nch == P) kind(ModInt<0>{}, ModInt<P>{}, ModInt<256>{});
@@ -41,12 +48,13 @@ template <int ELT, typename F> void with_mod_form(ModForm f, int64_t cols, F&& g
 
 namespace {
 
-// a and b summed over a row's threads in 64 bits: a wave's, or a workgroup's of at most 16 waves through LDS,
+// a and b summed over a row's threads in 64 bits: 16 lanes', a wave's, or a workgroup's of at most 16 waves through LDS,
 // wave by wave in one order. slots: one of two in turn, so that a wave may enter the next row's sums while
 // another still reads this one's. The barrier leaves loads in flight.
 template <int TPR> __device__ __forceinline__ void row_sums(double& a, double& b, double (&slots)[16][2]) {
-  a = group_reduce<64, false>(a);
-  b = group_reduce<64, false>(b);
+  constexpr int G = TPR == 16 ? 16 : 64;
+  a = group_reduce<G, false>(a);
+  b = group_reduce<G, false>(b);
   if constexpr (TPR == 0) {
     if ((threadIdx.x & 63) == 0) {
       slots[threadIdx.x >> 6][0] = a;
@@ -75,7 +83,7 @@ template <int ELT, int TPR, int NCH, int KIND> struct ModRow {
     else return TPR;
   }
   __device__ __forceinline__ explicit ModRow(int64_t n) : cols((int)n) {
-    lane = TPR == 0 ? threadIdx.x : threadIdx.x % 64;
+    lane = TPR == 0 ? threadIdx.x : threadIdx.x % (TPR == 0 ? 64 : TPR);
     base = TPR == 0 ? __builtin_amdgcn_readfirstlane(lane & ~63) : 0;
   }
   __device__ __forceinline__ int col(int i) const { return (lane + threads() * i) * V; }
@@ -83,7 +91,7 @@ template <int ELT, int TPR, int NCH, int KIND> struct ModRow {
   // of the whole wave, in scalar registers: whether a lane has a chunk i, and whether all have whole ones
   __device__ __forceinline__ bool some(int i) const { return KIND == kEven || (base + threads() * i) * V < cols; }
   __device__ __forceinline__ bool all(int i) const {
-    return KIND == kEven || (KIND == kAny && (base + threads() * i + 64) * V <= cols);
+    return KIND == kEven || (KIND == kAny && (base + threads() * i + (TPR == 16 ? 16 : 64)) * V <= cols);
   }
   __device__ __forceinline__ void load(const void* row, Chunk<ELT> (&d)[NCH]) const {
     const uint8_t* p = (const uint8_t*)row;

@@ -54,8 +54,9 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
   constexpr bool AHEAD = !(NT == 1024 && ELT == REELS_HIP_F32);
   __shared__ double slots[2][16][2];
   const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
-  // rows in 32 bits, so that they and what follows from them stay in scalar registers
-  const uint32_t begin = TPR == 0 ? blockIdx.x : blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // rows in 32 bits, so that they and what follows from them stay in scalar registers (but for 16 lanes)
+  const uint32_t begin = TPR == 0 ? blockIdx.x : TPR == 64 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
+                                                          : blockIdx.x * 16 + (threadIdx.x >> 4);
   const uint32_t end = (uint32_t)a.rows, rpg = (uint32_t)a.rpg;
   if (begin >= end) return;
   // A row's operands on their way; raw: its first elements, which every thread needs. All loads are
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
       const double below = -mean * rstd;  // its rounding is 2^-53 of the mean over the spread
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        if (!at.some(i)) continue;
+        if (TPR != 16 && !at.some(i)) continue;
         float y[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -210,6 +211,10 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
         else *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
         if (col % kMxBlock == 0) (a.scales + (row >> 6) * tiles * 512)[(uint32_t)mx4_scale_at(row & 63, col / kMxBlock, tiles)] = (uint8_t)byte;
       }
+    }
+    if constexpr (MODE == 2 && TPR == 16 && NCH * V < 16) {  // the other half of the tile's 256 columns
+      reinterpret_cast<uint32_t*>(a.codes + row * 128 + 64)[at.lane] = 0u;
+      if (at.lane < 4) (a.scales + (row >> 6) * 512)[(uint32_t)mx4_scale_at(row & 63, 4 + at.lane, 1)] = 0;
     }
     if constexpr (AHEAD) cur = next;
     else load(r + run, cur);
@@ -238,7 +243,7 @@ int mod_forward(const char* fn, const char* label, int mode, ModArgs a, int dtyp
   // each row has its own modulations. Long rows take two workgroups a CU, where as many as fit queue for
   // memory: 32760 x 5120 bf16 256 us with two, 283 with three, and to 4 bits 232 and 239; 4096 wide 195 with two
   // and 206 with four. Shorter ones take all: 1536 wide 77 us with five, 81 with four, 113 with two.
-  const int64_t per = f.tpr == 64 ? 4 : 1, fit = 16 * 64 / f.threads;
+  const int64_t per = mod_walkers(f), fit = 16 * 64 / f.threads;
   const int64_t resident = 256 * (f.tpr == 0 && a.cols > 2048 && f.threads >= 256 ? std::min<int64_t>(fit, 2) : fit) * per;
   const int64_t run = a.rpg == 1 || a.rows < resident ? a.rows : resident, grid = ceil_div(run, per);
   if (!grid_fits(grid, f.threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(1024) void mod_sum_kernel(const float* __restrict__
 // a small part of the traffic. {partial rows, rows that follow each other}
 struct ModParts { int64_t parts, run; };
 ModParts mod_parts(int64_t groups, int64_t rpg, ModForm f) {
-  const int64_t walkers = f.tpr == 64 ? 4 : 1, wgs = 256 * (12 * 64 / f.threads > 0 ? 12 * 64 / f.threads : 1);
+  const int64_t walkers = mod_walkers(f), wgs = 256 * (12 * 64 / f.threads > 0 ? 12 * 64 / f.threads : 1);
   const int64_t share = ceil_div(wgs, groups) * walkers;
   int64_t run = ceil_div(rpg, share);
   if (run < 2) run = 2;
@@ -78,7 +78,7 @@ extern "C" int reels_hip_modulated_norm_bwd(const void* dy, const void* s, const
   const ModForm f = mod_form(dtype, rows, cols);
   const int64_t groups = rows / rows_per_group;
   const bool sums = rows_per_group > 1 && (dgate != nullptr || dscale != nullptr);
-  const int64_t walkers = f.tpr == 64 ? 4 : 1;
+  const int64_t walkers = mod_walkers(f);
   const ModParts p = sums ? mod_parts(groups, rows_per_group, f) : ModParts{1, rows};  // without sums: a row each
   const int64_t parts = p.parts;
   if (parts > 1 && (workspace == nullptr || ws_bytes < reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group)))

@@ -55,14 +55,14 @@ template <int ELT, int TPR, int NCH, int KIND> struct Held<ELT, TPR, NCH, KIND, 
   }
 };
 
-// A wave or workgroup walks rows begin .. end of one group.
+// 16 lanes, a wave or a workgroup walk rows begin .. end of one group.
 // SUMS: it leaves the sums of the modulations' gradients over them; otherwise (no such gradient, or groups
 // of one row) rows of several groups may follow each other.
 template <int ELT, int TPR, int NCH, int NT, int KIND, bool KEPT, bool SUMS>
 __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdArgs a) {
-  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), WALKERS = TPR == 0 ? 1 : 4;
+  constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), WALKERS = TPR == 0 ? 1 : 256 / (TPR == 0 ? 256 : TPR);
   __shared__ double slots[2][16][2];
-  __shared__ float acc[SUMS && WALKERS > 1 ? WALKERS * 64 * NCH * V : 1];
+  __shared__ float acc[SUMS && WALKERS > 1 ? WALKERS * TPR * NCH * V : 1];
   // A thread's gates wait in LDS until a row's end: with the sums they do not fit three waves' registers. Rows
   // past 8192 elements have one workgroup a CU, 128 registers and all of its LDS: 1 + scale is there, too.
   constexpr bool AWAY = (SUMS && NT == 512) || NT == 1024, UP_AWAY = NT == 1024;
@@ -73,8 +73,8 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
   constexpr bool AHEAD = NT < 512 || (NT == 512 && ELT != REELS_HIP_F32 && !(KEPT && KIND == kAny));
   __shared__ f32x4 gates[AWAY ? NCH * V / 4 : 1][AWAY ? NT : 1], ups[UP_AWAY ? NCH * V / 4 : 1][UP_AWAY ? NT : 1];
   const ModRow<ELT, TPR, NCH, KIND> at(a.cols);
-  const int sub = TPR == 0 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // rows in 32 bits, so that they and what follows from them stay in scalar registers
+  const int sub = TPR == 0 ? 0 : TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x >> 4;
+  // rows in 32 bits, so that they and what follows from them stay in scalar registers (but for 16 lanes)
   const uint32_t wg_group = SUMS ? blockIdx.x / (uint32_t)a.parts : 0, part = SUMS ? blockIdx.x % (uint32_t)a.parts : blockIdx.x;
   const uint32_t rpg = (uint32_t)a.rpg, run = (uint32_t)a.run, last = (uint32_t)a.rows - 1;
   const uint32_t begin = wg_group * rpg + part * WALKERS + sub, end = SUMS ? (wg_group + 1) * rpg : last + 1;
@@ -229,12 +229,12 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) acc[sub * 64 * NCH * V + at.col(i) + j] = v[i][j];
+          for (int j = 0; j < V; ++j) acc[sub * TPR * NCH * V + at.col(i) + j] = v[i][j];
         __syncthreads();
         for (int c = threadIdx.x; c < (int)a.cols; c += 256) {
           float t = acc[c];
 #pragma unroll
-          for (int r = 1; r < WALKERS; ++r) t += acc[r * 64 * NCH * V + c];
+          for (int r = 1; r < WALKERS; ++r) t += acc[r * TPR * NCH * V + c];
           out[c] = t;
         }
       } else {

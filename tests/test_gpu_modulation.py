@@ -2,7 +2,7 @@
 count f32 roundings (u = 2^-24). y: s - mean has 2 u, rstd and its product 2 u, 1 + scale u, the sum u. d:
 g = dy (1 + scale) 2 u, n 4 u; mean g and mean g n add chunks of at most eight terms in f32 (8 u) before
 they go on in 64 bits, and are rounded: 12 u and 18 u of the means of magnitudes; then three differences and
-products. Sums over rows follow each other in a thread, then over at most 4 groups, 32 slices and
+products. Sums over rows follow each other in a thread, then over at most 16 groups, 32 slices and
 parts / 32 partial rows: 100 + rows / 64 roundings at most."""
 import pytest
 import torch
@@ -292,7 +292,7 @@ def test_many_rows(dev):
 
 @pytest.mark.parametrize("compress", [False, True])
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("C", [130, 515, 1000, 1536, 5120, 5125, 8200, 16384])
+@pytest.mark.parametrize("C", [6, 24, 96, 128, 130, 256, 300, 515, 1000, 1536, 5120, 5125, 8200, 16384])
 def test_many_rows_of_each_form(dev, C, dtype, compress):
     """Several rows one after the other in every wave or workgroup, in two groups."""
     B, S = 2, 2500 if C < 5000 else 1100
