@@ -8,9 +8,8 @@ namespace reels {
 // `threads` (tpr 0), with nch chunks of 16 bytes a thread. 8 elements a thread up to four waves (three waves
 // at 1536 leave no lane idle), then 16, up to 16 waves. Where there are rows enough a wave has up to 1024
 // elements, 16 a lane: 58514 x 700 bf16 75 us and 98 with two waves to a row, to 4 bits 78 and 94; 3000 x 700
-// forward 10.1 and 9.8, backward 20 and 24; 300 x 700 7.4 and 6.5, 16 and 15. A wave to a row of 64 is bound by
-// the row's instructions: 131040 x 64 bf16 70 us, 16 lanes
-// 22; 131040 x 200 72 and 38.
+// forward 10.1 and 9.8, backward 20 and 24; 300 x 700 7.4 and 6.5, 16 and 15. A wave to a narrow row is bound
+// by the row's instructions: 131040 x 64 bf16 70 us, with 16 lanes 22; 131040 x 200 72 and 38.
 struct ModForm { int tpr, nch, threads; };
 constexpr int64_t kModCols = 16384;  // the longest row
 inline ModForm mod_form(int elt, int64_t rows, int64_t cols) {

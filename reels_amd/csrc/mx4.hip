@@ -20,7 +20,8 @@ __device__ __forceinline__ v8i wide(const v4i& a) { return v8i{a[0], a[1], a[2],
 
 // ---- rows to 4 bits and back ---------------------------------------------------------------------
 // 64 rows x 256 columns per workgroup, one tile of scale bytes: they are put together in LDS and leave in
-// whole lines. A thread has 16 bytes of a row at a time, all its loads in flight. Bound by memory.
+// whole lines. A thread has 16 bytes of a row at a time, all its loads in flight. Bound by memory: 32760 x 13824
+// bf16 245 us to 4 bits (4.7 TB/s), 204 back (5.6).
 template <int ELT> __global__ __launch_bounds__(256) void mx4_pack_kernel(const void* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                                           int tiles, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), LPR = 256 / V, RP = 256 / LPR, U = 8;
@@ -129,6 +130,9 @@ template <int SA, int SB> __device__ __forceinline__ f32x16 mfma(const v4i& a, c
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, SA, (int)sa, SB, (int)sb);
 }
 
+// At the largest sizes bound by power: 32760 x 13824 -> 5120 takes 1110-1170 us (4.0-4.2 PFLOP/s) at 1.3-1.6 GHz, the
+// products alone on operands in LDS 5.9 PFLOP/s; smaller ones by the first loads and the epilogue.
+//
 // 32 TJ x 32 TJ outputs per workgroup of TJ waves (TJ = 8: 256 x 256, TJ = 4: 128 x 128), each wave 16 TJ
 // tokens x 64 columns, in steps of 128 codes (64 bytes of a row). The operands travel from HBM to LDS directly
 // into a ring of four stages. While the products of step s run, the fragments of step s + 1 replace those that
@@ -435,7 +439,8 @@ template <int ELT> __device__ __forceinline__ void load_bias(const Mx4Args& a, i
 // would leave most CUs idle. Waves w and w + 4 own the same 32 x 32 outputs and take the two halves of a
 // step's codes (their sums are added in LDS at the end). A ring of four stages, three steps in flight and one
 // barrier per step; two workgroups fit a CU. The scale words come the same way, 512 bytes an operand and step,
-// from waves 0 and 1; the others issue a copy that reads nothing, so that the waits count the same.
+// from waves 0 and 1; the others issue a copy that reads nothing, so that the waits count the same. 64 x 5120 -> 5120
+// 11.1 us: 20 steps with a barrier each on 80 workgroups.
 namespace small {
 constexpr int BT = 64, BK = 128, STAGE = 2 * BT * BK + 2048, RING = 4, NT = 512, LDS = RING * STAGE + 1024;
 }
@@ -518,7 +523,8 @@ template <int ELT> __global__ __launch_bounds__(small::NT) void mx4_small_kernel
 // Up to 16 tokens: 16 outputs per workgroup, its waves take lines of 256 codes in turn and read codes and
 // scale words straight into registers (each code of the weight is used once, so LDS would only add a trip),
 // then add their sums in LDS in wave order. Lanes of tokens that are not there read nothing (an offset past the
-// buffer's bounds). Bound by the weight's bytes and by latency.
+// buffer's bounds). Bound by the weight's bytes and by latency: 1 x 5120 -> 13824 12 us (3.1 TB/s) between events,
+// 9.8 a call in a row of calls.
 constexpr int kFewWaves = 8;  // the most of a workgroup
 
 template <int ELT> __global__ __launch_bounds__(kFewWaves * 64) void mx4_few_kernel(Mx4Args a) {
