@@ -54,7 +54,7 @@ class CompressedActivations:
             raise TypeError(f"unsupported dtype {dt}")
         k = _checked(self, "the activations")
         M, C = _rows_of(k.values)
-        out = torch.empty(k.values.shape, dtype=dt, device=k.device)
+        out = torch.empty_like(k.values, dtype=dt)
         _launch("reels_hip_act8_restore", k.device, _ptr(k.values), _ptr(k.scales), _DTYPE_CODE[dt],
                 M, C, _ptr(out), _stream(k.device))
         return out
@@ -84,9 +84,10 @@ def _scales_shape(shape):
     return tuple(shape[:-1]) + (-(-shape[-1] // _BLOCK),)
 
 
-def _empty(shape, dtype, device) -> CompressedActivations:
-    return CompressedActivations(torch.empty(shape, dtype=torch.int8, device=device),
-                                 torch.empty(_scales_shape(shape), dtype=torch.uint8, device=device), dtype)
+def _empty(x: torch.Tensor, dtype) -> CompressedActivations:
+    values = (torch.empty_like(x, dtype=torch.int8) if x.is_contiguous()
+              else torch.empty(x.shape, dtype=torch.int8, device=x.device))
+    return CompressedActivations(values, torch.empty(_scales_shape(x.shape), dtype=torch.uint8, device=x.device), dtype)
 
 
 def _input(x: torch.Tensor):
@@ -99,7 +100,7 @@ def _input(x: torch.Tensor):
 def compress_activations(x: torch.Tensor) -> CompressedActivations:
     """x ``[..., C]`` in 8 bits (bfloat16, float16 or float32)."""
     dt, x = _input(x)
-    k = _empty(x.shape, dt, x.device)
+    k = _empty(x, dt)
     M, C = _rows_of(x)
     _launch("reels_hip_act8_keep", x.device, _ptr(x), _DTYPE_CODE[dt], M, C, _ptr(k.values),
             _ptr(k.scales), _stream(x.device))
@@ -109,7 +110,7 @@ def compress_activations(x: torch.Tensor) -> CompressedActivations:
 def gelu_tanh_compressed(x: torch.Tensor) -> Tuple[torch.Tensor, CompressedActivations]:
     """(gelu_tanh(x), x in 8 bits) in one pass; ``gelu_tanh_backward`` takes the second."""
     dt, x = _input(x)
-    k, y = _empty(x.shape, dt, x.device), torch.empty_like(x)
+    k, y = _empty(x, dt), torch.empty_like(x)
     M, C = _rows_of(x)
     _launch("reels_hip_act8_gelu_tanh", x.device, _ptr(x), _DTYPE_CODE[dt], M, C, _ptr(y),
             _ptr(k.values), _ptr(k.scales), _stream(x.device))

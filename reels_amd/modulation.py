@@ -153,11 +153,11 @@ def modulated_norm(x: torch.Tensor, scale: Optional[torch.Tensor] = None, shift:
     dt, args, s, xr, held = _operands(x, scale, shift, branch, gate, eps)
     dev = x.device
     y = _like(x, xr)
-    stats = torch.empty(x.shape[:-1] + (3,), dtype=torch.float32, device=dev)
+    stats = torch.empty((*x.shape[:-1], 3), dtype=torch.float32, device=dev)
     kept, ptrs = None, (None,) * 4
     if compress:
-        a = activations._empty(x.shape, dt, dev)
-        b = None if branch is None else activations._empty(x.shape, dt, dev)
+        a = activations._empty(x, dt)
+        b = None if branch is None else activations._empty(x, dt)
         kept = KeptRows(a, b)
         ptrs = (a.values.data_ptr(), a.scales.data_ptr()) + (
             (None, None) if b is None else (b.values.data_ptr(), b.scales.data_ptr()))
