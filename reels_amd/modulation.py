@@ -51,7 +51,6 @@ class ModulatedNormGradients(NamedTuple):
     shift: Optional[torch.Tensor]
 
 
-@functools.lru_cache(maxsize=4096)  # a function of the shapes alone
 def _groups(shape, mod, name):
     """How many rows a modulation of shape `mod` has for rows of `shape`: 1, one for each sample, or one each."""
     C = shape[-1]
@@ -65,34 +64,48 @@ def _groups(shape, mod, name):
                      f"got {tuple(mod)}")
 
 
+@functools.lru_cache(maxsize=4096)  # a function of shapes and types alone
+def _kind(shape, dt, mods):
+    """(type code, rows of a group) of modulations given as (name, shape, type) or None."""
+    G, mt, first = None, dt, None
+    for m in mods:
+        if m is None:
+            continue
+        name, mod, t = m
+        n = _groups(shape, mod, name)
+        if t != dt and t != torch.float32:
+            raise TypeError(f"{name} must be {dt} or float32, got {t}")
+        if G is None:
+            G, mt, first = n, t, name
+        elif n != G or t != mt:
+            raise ValueError(f"gate, scale and shift must be of one kind and type; {name} is {tuple(mod)} "
+                             f"{t}, unlike {first}")
+    M = math.prod(shape[:-1])
+    return _DTYPE_CODE[mt], max(M // G, 1) if G else max(M, 1)
+
+
 def _modulations(x, dt, mods):
     """([tensor or None, row stride] for each modulation one after the other, type code, rows of a group). mods:
     (tensor or None, name) pairs. The tensors hold the memory until the launch."""
-    shape, dev, C = x.shape, x.device, x.shape[-1]
-    out, G, mt, first = [], None, dt, None
+    shape, dev = x.shape, x.device
+    C = shape[-1]
+    code, rpg = _kind(shape, dt, tuple([None if t is None else (name, t.shape, t.dtype) for t, name in mods]))
+    out = []
     for t, name in mods:
         if t is None:
             out += (None, C)
             continue
-        n = _groups(shape, t.shape, name)
-        if t.dtype != dt and t.dtype != torch.float32:
-            raise TypeError(f"{name} must be {dt} or float32, got {t.dtype}")
         if t.device != dev:
             raise ValueError(f"{name} is on {t.device}, the rows on {dev}")
-        if G is None:
-            G, mt, first = n, t.dtype, name
-        elif n != G or t.dtype != mt:
-            raise ValueError(f"gate, scale and shift must be of one kind and type; {name} is {tuple(t.shape)} "
-                             f"{t.dtype}, unlike {first}")
         ld = C
         if not t.is_contiguous():
+            G = _groups(shape, t.shape, name)
             t = t.reshape(G, C)
             if C > 1 and t.stride(1) != 1:
                 t = t.contiguous()
             ld = t.stride(0) if G > 1 else C
         out += (t, ld)
-    M = x.numel() // C
-    return out, _DTYPE_CODE[mt], max(M // G, 1) if G else max(M, 1)
+    return out, code, rpg
 
 
 @functools.lru_cache(maxsize=4096)  # a function of the sizes alone
