@@ -168,3 +168,7 @@ def test_blocks_of_a_microscaled_matrix():
     for bad in ((p[:, :3], s, K), (p, s[:, :1], K), (p.int(), s, K), (p[0], s, K), (p, s, 0)):
         with pytest.raises(ValueError):
             ra.MicroscaledMatrix.from_blocks(*bad)
+    empty = ra.MicroscaledMatrix.from_blocks(p[:0], s[:0], K)
+    assert empty.shape == (0, K) and empty.block_scales().shape == (0, s.shape[1])
+    turned = q.scales.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(ra.MicroscaledMatrix(q.codes, turned, q.size).block_scales(), s)
