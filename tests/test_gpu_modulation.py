@@ -255,6 +255,27 @@ def test_strides_and_slices(dev):
                                                     br.transpose(0, 1).contiguous(), one[2]).output)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("S,C", [(300, 6), (300, 100), (300, 200), (300, 512), (2100, 1000), (50, 1500), (50, 5120), (20, 9001)])
+def test_odd_addresses_of_each_form(dev, S, C, dtype):
+    """Operands that start between two vectors, and modulations inside a wider tensor, give the same bits."""
+    t, m = make(2, S, C, dtype, "f32", "token")
+
+    def odd(v):
+        return torch.cat([v.reshape(-1)[:1], v.reshape(-1)])[1:].view(v.shape)
+    wide = torch.stack([odd(m[n]) for n in ("gate", "scale", "shift")], 2)
+    inside = dict(zip(("gate", "scale", "shift"), wide.unbind(2)))
+
+    def both(t, m):
+        r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], compress=True)
+        q = modulated_norm_quantized(t["x"], m["scale"], m["shift"], t["branch"], m["gate"]).output
+        g = modulated_norm_backward(t["dy"], r.sum, r.stats, m["scale"], t["branch"], m["gate"], t["dsum"])
+        k = modulated_norm_backward(t["dy"], r.kept.sum, r.stats, m["scale"], r.kept.branch, m["gate"], t["dsum"])
+        return [r.output, r.sum, r.stats, r.kept.sum.values, r.kept.branch.scales, q.codes, q.block_scales()] + list(g) + list(k)
+    for u, v in zip(both({n: odd(v) for n, v in t.items()}, inside), both(t, m)):
+        assert torch.equal(u, v)
+
+
 def test_over_the_inputs(dev):
     """The sum over x or the branch, dx over dy or the other gradient: what the C entries allow."""
     from reels_amd import _lib
