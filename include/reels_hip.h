@@ -461,7 +461,7 @@ int reels_hip_clip_gradients(const void* const* grads, void* const* outs, const 
  * shift [rows / rows_per_group][cols] of m_dtype (dtype or REELS_HIP_F32), their rows ld_gate, ld_scale
  * and ld_shift elements apart: row m takes row m / rows_per_group; rows is a multiple of rows_per_group.
  * 0 < cols <= 16384. sum receives s where there is a branch (it may be x or branch themselves where
- * their stride is cols); y overlaps no other operand. stats [rows][3] f32: the mean as the sum of two
+ * their stride is cols, and overlaps no other operand); y overlaps no other operand. stats [rows][3] f32: the mean as the sum of two
  * values, and rstd. Means and squares are summed in 64 bits, the squares about the mean. A row of s with
  * NaN or an infinity is NaN throughout, and so is one whose rstd is past f32 (no spread and eps 0).
  * kept_sum, kept_branch with their scales (NULL: not wanted): s and branch as reels_hip_act8_keep would

@@ -31,7 +31,7 @@ struct ModArgs {
   int64_t ld_x, ld_b, ld_gate, ld_scale, ld_shift, rows, cols, rpg;
   double per_col;
   float eps;
-  int center, m_f32;
+  int center, m_f32, over;  // over: the sum is written over x or the branch
 };
 
 // the 8-bit codes of a thread's chunk of a row (all lanes take part; lanes past the row hold zeros)
@@ -89,6 +89,14 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
   int turn = 0;
   for (uint32_t r = begin; r < end; r += run, turn ^= 1) {
     const int64_t row = r;
+    // All threads of a row read its first element, which one of them is about to overwrite: every wave has this
+    // row in registers before any stores its part of the sum.
+    if (a.over) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+      if constexpr (TPR == 0) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
     if (r >= change) {
       const uint32_t group = r / rpg;
       change = (group + 1) * rpg;
@@ -238,7 +246,10 @@ int mod_forward(const char* fn, const char* label, int mode, ModArgs a, int dtyp
       (mode == 2 ? a.codes == nullptr || a.scales == nullptr : a.y == nullptr || a.stats == nullptr))
     return fail(REELS_HIP_EINVAL, std::string(fn) + ": NULL operand");
   if (mode == 2 && ((uintptr_t)a.codes & 3) != 0) return fail(REELS_HIP_EINVAL, std::string(fn) + ": codes must be 4-byte aligned");
+  if (a.branch != nullptr && a.rows > 1 && ((a.sum == a.x && a.ld_x != a.cols) || (a.sum == a.branch && a.ld_b != a.cols)))
+    return fail(REELS_HIP_EINVAL, std::string(fn) + ": sum may be x or branch only where their row stride is cols");
   a.m_f32 = m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32;
+  a.over = a.branch != nullptr && (a.sum == a.x || a.sum == a.branch);
   a.per_col = 1.0 / (double)a.cols;
   const ModForm f = mod_form(dtype, a.rows, a.cols);
   // Rows that follow each other in a wave or workgroup: as many as leave every one resident, one where

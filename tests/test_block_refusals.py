@@ -172,3 +172,14 @@ def test_blocks_of_a_microscaled_matrix():
     assert empty.shape == (0, K) and empty.block_scales().shape == (0, s.shape[1])
     turned = q.scales.transpose(0, 1).contiguous().transpose(0, 1)
     assert torch.equal(ra.MicroscaledMatrix(q.codes, turned, q.size).block_scales(), s)
+
+
+def test_sum_over_strided_rows_is_refused():
+    """sum may be x or branch themselves, but not where their rows lie further apart than the sum's."""
+    L = _lib.lib()
+    G = ctypes.c_void_p(1 << 20)
+    for x, b, ldx, ldb in ((F, G, 9, 8), (G, F, 8, 9)):
+        assert L.reels_hip_modulated_norm(x, ldx, b, ldb, None, 8, None, 8, None, 8, 0, 1, 4, 8, 2, 1e-6, 1, F, G, G, None, None, None,
+                                          None, None) == -1 and "stride" in _err()
+        assert L.reels_hip_modulated_norm_mx4(x, ldx, b, ldb, None, 8, None, 8, None, 8, 0, 1, 4, 8, 2, 1e-6, 1, F, G, G, None) == -1
+        assert "stride" in _err()

@@ -491,3 +491,38 @@ def test_offsets_past_32_bits(dev):
     q = modulated_norm_quantized(x, scale, shift, b, gate)
     p = modulated_norm_quantized(ends(x), scale, shift, ends(b), gate)
     assert torch.equal(ends(q.output.codes), p.output.codes) and torch.equal(ends(q.output.block_scales()), p.output.block_scales())
+
+
+@pytest.mark.parametrize("dtype,B,S,C", [("bf16", 2, 40, 24), ("f32", 2, 40, 200), ("f16", 2, 40, 512), ("f32", 2, 300, 700),
+                                         ("bf16", 2, 300, 700), ("f32", 2, 1400, 700), ("bf16", 2, 1500, 1536), ("f16", 2, 700, 5125),
+                                         ("bf16", 2, 400, 9001), ("f32", 2, 400, 9001), ("f32", 2, 300, 16384)])
+def test_sum_over_the_inputs_of_each_form(dev, dtype, B, S, C):
+    """The sum over x or the branch where a row has 16 lanes, a wave or a workgroup, in every row that a workgroup
+    takes one after the other: the bits of a call with a sum of its own."""
+    from reels_amd import _lib
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    t, m = make(B, S, C, dtype, "f32", "sample")
+    t["x"][..., 0] += 40  # an element far from the others: its row's pivot
+    code = {"f32": 0, "bf16": 1, "f16": 2}[dtype]
+    r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], compress=True)
+    q = modulated_norm_quantized(t["x"], m["scale"], m["shift"], t["branch"], m["gate"]).output
+    p = {n: v.data_ptr() for n, v in m.items()}
+    for over in ("x", "branch"):
+        for mode in ("rows", "kept", "4 bits"):
+            c = {n: t[n].clone() for n in ("x", "branch")}
+            args = (c["x"].data_ptr(), C, c["branch"].data_ptr(), C, p["gate"], C, p["scale"], C, p["shift"], C, 0, code, B * S, C,
+                    S, EPS, 1, c[over].data_ptr())
+            if mode == "4 bits":
+                codes, scales = torch.empty_like(q.codes), torch.empty_like(q.scales)
+                assert L.reels_hip_modulated_norm_mx4(*args, codes.data_ptr(), scales.data_ptr(), st) == 0
+                got, want = (codes,), (q.codes,)
+            else:
+                y, stats = torch.empty_like(r.output), torch.empty_like(r.stats)
+                k = [torch.empty_like(v) for v in (r.kept.sum.values, r.kept.sum.scales, r.kept.branch.values, r.kept.branch.scales)]
+                kept = [v.data_ptr() if mode == "kept" else None for v in k]
+                assert L.reels_hip_modulated_norm(*args, y.data_ptr(), stats.data_ptr(), *kept, st) == 0
+                got, want = (y, stats), (r.output, r.stats)
+                if mode == "kept":
+                    got, want = got + tuple(k), want + (r.kept.sum.values, r.kept.sum.scales, r.kept.branch.values, r.kept.branch.scales)
+            assert torch.equal(c[over], r.sum), (over, mode)
+            assert all(torch.equal(u, v) for u, v in zip(got, want)), (over, mode)
