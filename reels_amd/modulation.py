@@ -48,7 +48,7 @@ class ModulatedNormGradients(NamedTuple):
     branch: torch.Tensor              # without a gate the same tensor as x
     gate: Optional[torch.Tensor]      # float32, of the modulations' shapes
     scale: Optional[torch.Tensor]
-    shift: Optional[torch.Tensor]
+    shift: Optional[torch.Tensor]     # of scale's shape
 
 
 def _groups(shape, mod, name):
@@ -277,7 +277,7 @@ class ModulatedNormFunction(torch.autograd.Function):
             ctx.save_for_backward(k.sum.values, k.sum.scales, *b, r.stats, scale, gate)
         else:
             ctx.save_for_backward(r.sum, None, held, None, r.stats, scale, gate)
-        ctx.shift_dtype = None if shift is None else shift.dtype
+        ctx.shift_dtype, ctx.shift_shape = (None, None) if shift is None else (shift.dtype, shift.shape)
         return r.output if branch is None else (r.output, r.sum)
 
     @staticmethod
@@ -297,6 +297,8 @@ class ModulatedNormFunction(torch.autograd.Function):
 
         def of(t, like, want):
             return t.to(like) if want and t is not None else None
-        return (g.x, of(g.scale, None if scale is None else scale.dtype, need[1]), of(g.shift, ctx.shift_dtype, need[2]),
+        # scale and shift of one kind can differ in shape ([B, C] beside [B, 1, C])
+        dshift = None if g.shift is None else g.shift.view(ctx.shift_shape)
+        return (g.x, of(g.scale, None if scale is None else scale.dtype, need[1]), of(dshift, ctx.shift_dtype, need[2]),
                 g.branch if need[3] else None, of(g.gate, None if gate is None else gate.dtype, need[4]),
                 None, None, None)

@@ -526,3 +526,19 @@ def test_sum_over_the_inputs_of_each_form(dev, dtype, B, S, C):
                     got, want = got + tuple(k), want + (r.kept.sum.values, r.kept.sum.scales, r.kept.branch.values, r.kept.branch.scales)
             assert torch.equal(c[over], r.sum), (over, mode)
             assert all(torch.equal(u, v) for u, v in zip(got, want)), (over, mode)
+
+
+def test_modulations_of_one_kind_in_two_shapes(dev):
+    """scale [B, C] beside shift and gate [B, 1, C], and [1, C] beside [C]: each gradient has its own leaf's shape."""
+    for shape, a, b in (((2, 6, 64), (2, 64), (2, 1, 64)), ((2, 6, 64), (2, 1, 64), (2, 64)), ((7, 64), (64,), (1, 64)),
+                        ((7, 64), (1, 64), (64,))):
+        x, br, dy = (torch.randn(shape, device=dev) for _ in range(3))
+        scale, shift, gate = torch.randn(a, device=dev), torch.randn(b, device=dev), torch.randn(b, device=dev)
+
+        def grads(*mods):
+            leaves = [t.clone().requires_grad_() for t in mods]
+            y, _ = ModulatedNormFunction.apply(x, leaves[0], leaves[1], br, leaves[2])
+            return torch.autograd.grad(y, leaves, dy)
+        got, want = grads(scale, shift, gate), grads(scale, shift.view(a), gate.view(a))
+        for u, v, like in zip(got, want, (scale, shift, gate)):
+            assert u.shape == like.shape and torch.equal(u.flatten(), v.flatten())
