@@ -134,7 +134,9 @@ __device__ __forceinline__ float gelu_f(float x) {
 __device__ __forceinline__ float gelu_grad_f(float x) {
   const float k = 0.7978845608028654f, a = 0.044715f;
   const float t = tanh_f(k * (x + a * x * x * x));
-  return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * k * (1.0f + 3.0f * a * x * x);
+  // 1 - t^2 is 0 from |x| of about 5; the factor after it stays finite up to the end of the range
+  const float b = __builtin_amdgcn_fmed3f(fabsf(x), 0.0f, 1e15f);
+  return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * k * (1.0f + 3.0f * a * b * b);
 }
 template <int ELT> struct Elt;
 

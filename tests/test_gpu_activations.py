@@ -185,3 +185,25 @@ def test_offsets_past_32_bits(dev):
     assert torch.equal(k.restore()[-5:], ks.restore()) and not bool(k.values[:-5].any())
     dx = gelu_tanh_backward(k, x)
     assert torch.equal(dx[-5:], gelu_tanh_backward(ks, tail))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_gelu_pullback_at_the_ends_of_the_range(dev, dtype):
+    """Past 16 the slope is 1 or 0 to the last bit, up to the type's largest value: from kept values, from the
+    values themselves and behind the linear's dX."""
+    dt = DT[dtype]
+    top = torch.finfo(dt).max
+    sizes = [v for v in (17.0, 1e3, 3e4, 1e10, 9e18, 1.3e19, 6e19, 1e25, top / 3, top) if v <= top]
+    x = torch.tensor(sizes + [-v for v in sizes], device=dev, dtype=torch.float64).to(dt)[:, None].repeat(1, 96)
+    g = torch.Generator(device=dev).manual_seed(2)
+    dy = torch.randn(x.shape, generator=g, device=dev).to(dt)
+    k = compress_activations(x)
+    assert torch.isfinite(k.restore(torch.float32)).all()
+    for dx in (gelu_tanh_backward(k, dy), gelu_tanh_backward(x, dy)):
+        assert torch.equal(dx, torch.where(x > 0, dy, torch.zeros_like(dy)))
+    W = ra.quantize_frozen_matrix(torch.randn(64, 96, generator=g, device=dev).to(dt))
+    dz = torch.randn(len(x), 64, generator=g, device=dev).to(dt)
+    dx = ra.i8lora_backward(dz, None, W, want_dA=False, want_dB=False)[0]
+    want = torch.where(x > 0, dx, torch.zeros_like(dx))
+    for gx in (x, k):
+        assert torch.equal(ra.i8lora_backward_gelu(dz, None, gx, W, want_dA=False, want_dB=False)[0], want)
