@@ -89,14 +89,6 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
   int turn = 0;
   for (uint32_t r = begin; r < end; r += run, turn ^= 1) {
     const int64_t row = r;
-    // All threads of a row read its first element, which one of them is about to overwrite: every wave has this
-    // row in registers before any stores its part of the sum.
-    if (a.over) {
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-      if constexpr (TPR == 0) __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-    }
     if (r >= change) {
       const uint32_t group = r / rpg;
       change = (group + 1) * rpg;
@@ -119,6 +111,13 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
 #pragma clang fp contract(off)
       at.trim(cur.b);
       s0 = Store<ELT>::get(Store<ELT>::put(s0 + gate0 * Store<ELT>::get(cur.b0)));
+      // The sum over x or the branch: one thread is about to overwrite what all of the row's threads form s0 from,
+      // so every wave has it before any stores.
+      if (a.over) {
+        asm volatile("" : "+v"(s0) : : "memory");
+        if constexpr (TPR == 0) __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         float f[V];
