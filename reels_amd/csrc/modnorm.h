@@ -2,6 +2,8 @@
 #pragma once
 #include "microscale.h"
 
+#include <cmath>
+
 namespace reels {
 
 // Who has a row: 16 lanes (tpr 16; rows of up to 256 elements), a wave (tpr 64; up to 512), or a workgroup of
@@ -68,6 +70,18 @@ template <int TPR> __device__ __forceinline__ void row_sums(double& a, double& b
     b = group_reduce<16, false>(in ? slots[i][1] : 0.0);
   }
 }
+
+// What n = (s - mean) rstd of a row's elements is formed with: fmaf(s - hi, rstd, k), the mean in two parts.
+// Elements are at most sqrt(cols) spreads from the mean, so s - hi can pass the f32 range only where rstd is
+// below `far` = sqrt(cols) 2^-128 (and 1 / 32 more, for values kept in 7 bits). Such a row's mean is taken off in k
+// alone: |mean| rstd < 1.04 sqrt(cols) there, and n is off by half a step of that.
+struct ModUnit { float hi, k; };
+__device__ __forceinline__ ModUnit mod_unit(float hi, float lo, float rstd, float far) {
+  const float k = -lo * rstd;
+  const bool over = rstd < far;
+  return {over ? 0.0f : hi, over ? fmaf(-hi, rstd, k) : k};
+}
+inline float mod_far(int64_t cols) { return (float)(std::sqrt((double)cols) * 0x1.08p-128); }
 
 // A thread's chunks of a row: chunk i at element col(i). They are read without a branch, so that all loads of
 // a row are in flight together: a thread without a chunk reads the row's first one, and where the row's

@@ -30,7 +30,7 @@ struct ModArgs {
   uint8_t *codes, *scales; // rows in 4 bits
   int64_t ld_x, ld_b, ld_gate, ld_scale, ld_shift, rows, cols, rpg;
   double per_col;
-  float eps;
+  float eps, far;
   int center, m_f32, over;  // over: the sum is written over x or the branch
 };
 
@@ -178,7 +178,8 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
     const double var = fmax(fma(-off, off, sq * a.per_col), 0.0) + (sum - sum);  // NaN stays
     const double rstd = rsqrt64(var + (double)a.eps);
     if constexpr (MODE < 2) {
-      const float hi = (float)mean, lo = (float)(mean - (double)hi), rs = (float)rstd, k = -lo * rs;
+      const float hi = (float)mean, lo = (float)(mean - (double)hi), rs = (float)rstd;
+      const ModUnit n = mod_unit(hi, lo, rs, a.far);
       if (at.lane == 0) {
         float* st = a.stats + row * 3;
         st[0] = hi;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? (ELT == REELS_HIP_F32 ? 3 : 4) : 1)
         float y[V];
         Chunk<ELT> o;
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] = fmaf(fmaf(s[i].get(j) - hi, rs, k), 1.0f + up[i][j], shift[i][j]);
+        for (int j = 0; j < V; ++j) y[j] = fmaf(fmaf(s[i].get(j) - n.hi, rs, n.k), 1.0f + up[i][j], shift[i][j]);
         o.pack(y);
         at.store((uint8_t*)a.y + row * a.cols * EB, i, o);
       }
@@ -250,6 +251,7 @@ int mod_forward(const char* fn, const char* label, int mode, ModArgs a, int dtyp
   a.m_f32 = m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32;
   a.over = a.branch != nullptr && (a.sum == a.x || a.sum == a.branch);
   a.per_col = 1.0 / (double)a.cols;
+  a.far = mod_far(a.cols);
   const ModForm f = mod_form(dtype, a.rows, a.cols);
   // Rows that follow each other in a wave or workgroup: as many as leave every one resident, one where
   // each row has its own modulations. Long rows take two workgroups a CU, where as many as fit queue for

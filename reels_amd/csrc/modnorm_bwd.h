@@ -27,6 +27,7 @@ struct ModBwdArgs {
   int64_t ld_gate, ld_scale, rows, cols, rpg, run;    // run: rows that follow each other in a wave or workgroup
   double per_col;
   int center, m_f32, parts;
+  float far;
 };
 
 template <int ELT> void launch_mod_bwd(const ModBwdArgs& a, ModForm f, bool kept, bool sums, int64_t grid, hipStream_t st);

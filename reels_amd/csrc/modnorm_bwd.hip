@@ -87,7 +87,7 @@ extern "C" int reels_hip_modulated_norm_bwd(const void* dy, const void* s, const
   if (!grid_fits(grid, f.threads)) return fail(REELS_HIP_EINVAL, std::string(fn) + ": too many rows for one launch");
   const ModBwdArgs a{dy, s, dsum, branch, gate, scale, s_scales, branch_scales, stats, dx, dbranch, dgate, dscale, dshift,
                      (float*)workspace, ld_gate, ld_scale, rows, cols, rows_per_group, p.run, 1.0 / (double)cols, center != 0,
-                     m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32, (int)parts};
+                     m_dtype == REELS_HIP_F32 && dtype != REELS_HIP_F32, (int)parts, mod_far(cols)};
   { TraceScope _ts(st, "mod_bwd_kernel");
     with_any_elt(dtype, [&](auto e) { launch_mod_bwd<decltype(e)::value>(a, f, s_scales != nullptr, sums, grid, st); }); }
   if (int rc = check_launch("mod_bwd_kernel")) return rc;

@@ -155,7 +155,12 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
     if constexpr (AHEAD) load(r + run, next);
     cur.s.trim(at);
     at.trim(cur.dy);
-    const float hi = cur.hi, rstd = cur.rstd, k = -cur.lo * rstd;
+    const float rstd = cur.rstd;
+    ModUnit of = mod_unit(cur.hi, cur.lo, rstd, a.far);
+    // A workgroup's row: in a scalar register where the lanes' are scarce (8000 x 13824 bf16 268 us and 260). 512
+    // threads without the sums have enough; there the compiler then takes more than four waves leave (32760 x 5120
+    // 290 us and 360).
+    if constexpr (NT == 1024 || (SUMS && NT == 512)) of.hi = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(of.hi)));
     double g0 = 0.0, g1 = 0.0;
     // dy is zero where the thread has no element, and so are its shares of the sums
 #pragma unroll
@@ -164,7 +169,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
       if constexpr (UP_AWAY) take(ups, i, u);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = cur.dy[i].get(j), n = fmaf(cur.s.get(i, j) - hi, rstd, k), g = d * (UP_AWAY ? u[j] : up[i][j]);
+        const float d = cur.dy[i].get(j), n = fmaf(cur.s.get(i, j) - of.hi, rstd, of.k), g = d * (UP_AWAY ? u[j] : up[i][j]);
         p0 += g;
         p1 = fmaf(g, n, p1);
         if constexpr (SUMS) {
@@ -195,7 +200,7 @@ __global__ __launch_bounds__(NT, NT == 512 ? 3 : 1) void mod_bwd_kernel(ModBwdAr
       if constexpr (UP_AWAY) take(ups, i, u);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float n = fmaf(cur.s.get(i, j) - hi, rstd, k);
+        const float n = fmaf(cur.s.get(i, j) - of.hi, rstd, of.k);
         const float t = fmaf(-n, m1, fmaf(cur.dy[i].get(j), UP_AWAY ? u[j] : up[i][j], -m0));
         d[j] = a.dsum != nullptr ? fmaf(rstd, t, ds[i].get(j)) : rstd * t;
       }

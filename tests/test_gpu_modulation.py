@@ -542,3 +542,72 @@ def test_modulations_of_one_kind_in_two_shapes(dev):
         got, want = grads(scale, shift, gate), grads(scale, shift.view(a), gate.view(a))
         for u, v, like in zip(got, want, (scale, shift, gate)):
             assert u.shape == like.shape and torch.equal(u.flatten(), v.flatten())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,C", [(5, 100), (5, 200), (3, 300), (2100, 700), (4, 700), (3, 1536), (3, 5125), (3, 9001)])
+def test_rows_at_the_ends_of_the_range(dev, S, C, dtype):
+    """Elements whose difference from the mean passes the f32 range: n stays at most sqrt(C), and so do y and the
+    gradients. rstd is subnormal here: its half step is up to 2^-22 of it."""
+    t, m = make(1, S, C, dtype, "f32", "sample")
+    top = torch.finfo(DT[dtype]).max
+    x = torch.where(torch.rand(1, S, C, device=dev) < 0.7, -0.98 * top, 0.98 * top).to(DT[dtype])
+    x[..., 0], x[..., C - 1] = top, -top
+    assert bool(((x.double() - x.double().mean(-1, keepdim=True)).abs().amax(-1) > 2.0 ** 128).all())
+    for compress in (False, True):
+        r = modulated_norm(x, m["scale"], m["shift"], compress=compress)
+        sd, mean, rstd = unit(x, True)
+        st = r.stats.double()
+        assert bool(((st[..., 0] + st[..., 1] - mean[..., 0]).abs() <= 2.0 ** -40 * top).all())
+        assert_within(r.stats[..., 2], rstd[..., 0], U * rstd[..., 0], "rstd")
+        n, up = (sd - mean) * rstd, 1.0 + m["scale"][:, None].double()
+        y = n * up + m["shift"][:, None].double()
+        assert_within(r.output, y, 7 * U * (n * up).abs() + U * y.abs(), "y")
+        s = r.kept.sum if compress else r.sum
+        sd = blocks8(x.double().reshape(-1, C))[2].reshape(1, S, C) if compress else sd
+        g = modulated_norm_backward(t["dy"], s, r.stats, m["scale"])
+        check_backward(g, t, sd, None, r.stats, None, m["scale"], None, True, 1, S)
+        few = modulated_norm_backward(t["dy"], s, r.stats, m["scale"], want_modulation=False)
+        assert torch.equal(few.x, g.x)
+    q = modulated_norm_quantized(x, m["scale"], m["shift"]).output
+    assert torch.isfinite(q.dequantize(torch.float32)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,C", [(5, 6), (5, 100), (5, 200), (3, 300), (2100, 700), (4, 700), (3, 1536), (3, 5125), (3, 9001)])
+def test_rows_at_the_ends_of_the_range(dev, S, C, dtype):
+    """Elements whose difference from the mean passes the f32 range: n stays at most sqrt(C). Bounds (u = 2^-24, m =
+    |mean| rstd): rstd is subnormal, so off by e = 2^-150 / rstd of it, which n takes over; the mean is taken off as a
+    product with one rounding, m u; the rest of y as above. In d that error of n enters the mean of g n and n times
+    that mean; the backward starts from the stored rstd, so e drops out. dscale: m u of the sum of |dy|."""
+    t, m = make(1, S, C, dtype, "f32", "sample")
+    top = torch.finfo(DT[dtype]).max
+    g = torch.Generator(device=dev).manual_seed(C)
+    x = torch.where(torch.rand(1, S, C, generator=g, device=dev) < 0.7, -0.98 * top, 0.98 * top).to(DT[dtype])
+    x[..., 0], x[..., 1:5], x[..., C - 1] = top, -0.98 * top, -top
+    assert bool(((x.double() - x.double().mean(-1, keepdim=True)).abs().amax(-1) > 2.0 ** 128).all())
+    up, dy = 1.0 + m["scale"][:, None].double(), t["dy"].double()
+    for compress in (False, True):
+        r = modulated_norm(x, m["scale"], m["shift"], compress=compress)
+        sd, mean, rstd = unit(x, True)
+        st = r.stats.double()
+        assert bool(((st[..., 0] + st[..., 1] - mean[..., 0]).abs() <= 2.0 ** -40 * top).all())
+        assert_within(r.stats[..., 2], rstd[..., 0], U * rstd[..., 0], "rstd")
+        n, far = (sd - mean) * rstd, U * (mean * rstd).abs()
+        y = n * up + m["shift"][:, None].double()
+        assert_within(r.output, y, ((7 * U + 2.0 ** -150 / rstd) * n.abs() + far) * up.abs() + U * y.abs(), "y")
+        s = r.kept.sum if compress else r.sum
+        sd = blocks8(x.double().reshape(-1, C))[2].reshape(1, S, C) if compress else sd
+        d = modulated_norm_backward(t["dy"], s, r.stats, m["scale"])
+        rs, n = st[..., 2:], (sd - (st[..., 0] + st[..., 1])[..., None]) * st[..., 2:]
+        gd = dy * up
+        m1, a0, a1 = ((v).mean(-1, keepdim=True) for v in (gd * n, gd.abs(), (gd * n).abs()))
+        slack = rs * U * (8 * gd.abs() + 16 * a0 + 28 * n.abs() * a1) + 1.1 * rs * far * (n.abs() * a0 + m1.abs())
+        assert_within(d.x, rs * (gd - gd.mean(-1, keepdim=True) - n * m1), slack, "dx")
+        deep = (100 + S / 64) * U
+        assert_within(d.scale, (dy * n).sum(1), (deep * (dy * n).abs() + 1.1 * far * dy.abs()).sum(1), "dscale")
+        assert_within(d.shift, dy.sum(1), (deep * dy.abs()).sum(1), "dshift")
+        few = modulated_norm_backward(t["dy"], s, r.stats, m["scale"], want_modulation=False)
+        assert torch.equal(few.x, d.x)
+    q = modulated_norm_quantized(x, m["scale"], m["shift"]).output
+    assert torch.isfinite(q.dequantize(torch.float32)).all()
