@@ -209,10 +209,12 @@ def workspace_bytes(M: int, K: int, N: int, r: int, which: int,
     return int(L.reels_hip_i8lora_workspace_bytes(M, K, N, r, which))
 
 
-def _saved_x(x, dtype: torch.dtype, needed: bool) -> Optional[torch.Tensor]:
+def _saved_x(x, dtype: torch.dtype, needed: bool, device) -> Optional[torch.Tensor]:
     """The input of a linear as its backward takes it: activations kept in 8 bits
     (CompressedActivations) become the tensor that they stand for, where the call reads it."""
     if x is not None and not isinstance(x, torch.Tensor):
+        if x.device != device:
+            raise ValueError(f"x is on {x.device}, dy on {device}")
         x = x.restore(dtype) if needed else None
     return _contig(x, dtype, "x")
 
@@ -320,7 +322,7 @@ def i8lora_backward(dy, x, weight: QuantizedMatrix, A=None, B=None, lora_scale=1
     weight = _on_activation_device(weight, dy.device)
     A = _contig(A, dt, "A")
     B = _contig(B, dt, "B")
-    x = _saved_x(x, dt, r > 0 and (want_dA or (want_dB and h is None)))
+    x = _saved_x(x, dt, r > 0 and (want_dA or (want_dB and h is None)), dy.device)
     h = _contig(h, dt, "h")
     dev = dy.device
     dx = torch.empty((M, K), dtype=dt, device=dev) if want_dx else None
@@ -372,7 +374,7 @@ def i8lora_backward_gelu(dy, x, gx, weight: QuantizedMatrix, A=None, B=None, lor
     dy = dy.contiguous()
     weight = _on_activation_device(weight, dy.device)
     A, B, h, gx = _contig(A, dt, "A"), _contig(B, dt, "B"), _contig(h, dt, "h"), _contig(gx, dt, "gx")
-    x = _saved_x(x, dt, r > 0 and (want_dA or (want_dB and h is None)))
+    x = _saved_x(x, dt, r > 0 and (want_dA or (want_dB and h is None)), dy.device)
     dev = dy.device
     dx = torch.empty((M, K), dtype=dt, device=dev)
     dA = torch.empty((K, r), dtype=torch.float32, device=dev) if (want_dA and r) else None

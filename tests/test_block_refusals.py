@@ -183,3 +183,13 @@ def test_sum_over_strided_rows_is_refused():
                                           None, None) == -1 and "stride" in _err()
         assert L.reels_hip_modulated_norm_mx4(x, ldx, b, ldb, None, 8, None, 8, None, 8, 0, 1, 4, 8, 2, 1e-6, 1, F, G, G, None) == -1
         assert "stride" in _err()
+
+
+def test_kept_rows_on_another_device_are_refused():
+    """The restored values would lie on the kept rows' device, where the linear's backward on dy's reads them."""
+    from reels_amd import layers
+    k = ra.CompressedActivations(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.uint8))
+    for needed in (True, False):
+        with pytest.raises(ValueError, match="dy on cuda:1"):
+            layers._saved_x(k, BF, needed, torch.device("cuda", 1))
+    assert layers._saved_x(k, BF, False, torch.device("cpu")) is None
