@@ -61,6 +61,7 @@ template <int TPR> __device__ __forceinline__ void row_sums(double& a, double& b
       slots[threadIdx.x >> 6][0] = a;
       slots[threadIdx.x >> 6][1] = b;
     }
+    asm volatile("" ::: "memory");  // the slots are written on this side of the barrier
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
