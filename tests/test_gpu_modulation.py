@@ -611,3 +611,38 @@ def test_rows_at_the_ends_of_the_range(dev, S, C, dtype):
         assert torch.equal(few.x, d.x)
     q = modulated_norm_quantized(x, m["scale"], m["shift"]).output
     assert torch.isfinite(q.dequantize(torch.float32)).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("S,C", [(14000, 24), (14000, 130), (14000, 256), (3001, 300), (3001, 700), (1001, 1536), (401, 5125),
+                                 (301, 9001), (201, 16384)])
+def test_rows_one_after_the_other(dev, S, C, dtype):
+    """More rows than the forward's 16-lane groups, waves or workgroups, in three groups of rows: every one walks on
+    into another group's modulations, with its rows as they are, kept and in 4 bits."""
+    B = 3
+    t, m = make(B, S, C, dtype, "f32", "sample")
+    r = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+    check_forward(r, t["x"], t["branch"], m["gate"], m["scale"], m["shift"], True, B)
+    k = modulated_norm(t["x"], m["scale"], m["shift"], t["branch"], m["gate"], compress=True)
+    assert torch.equal(k.output, r.output) and torch.equal(k.sum, r.sum) and torch.equal(k.stats, r.stats)
+    for kept, of in ((k.kept.sum, r.sum), (k.kept.branch, t["branch"])):
+        q, sc, _ = blocks8(of.double().reshape(-1, C))
+        assert torch.equal(kept.values.reshape(-1, C), q) and torch.equal(kept.scales.reshape(B * S, -1), sc)
+    q = modulated_norm_quantized(t["x"], m["scale"], m["shift"], t["branch"], m["gate"])
+    assert torch.equal(q.sum, r.sum)
+    codes, scales = nibbles(q.output).view(B, S, C), q.output.block_scales().view(B, S, -1)
+    for b in range(B):
+        # each sample by the definition, 1000 rows at a time; a value within 2^-45 of a border may take either side
+        for i in range(0, S, 1000):
+            sd, mean, rstd = unit(r.sum[b, i:i + 1000], True)
+            part, shift = (sd - mean) * rstd * (1.0 + m["scale"][b].double()), m["shift"][b].double()
+            y, mag = part + shift, part.abs() + shift.abs()
+            c, sc, _ = blocks4(y.float().double())
+            near, far = torch.zeros_like(c, dtype=torch.bool), torch.zeros_like(sc, dtype=torch.bool)
+            for f in (-2.0 ** -45, 2.0 ** -45):
+                cf, sf, _ = blocks4((y + f * mag).float().double())
+                far |= sf != sc
+                near |= (cf != c) | far.repeat_interleave(32, 1)[:, :C]
+            assert not bool(((codes[b, i:i + 1000] != c) & ~near).any())
+            assert not bool(((scales[b, i:i + 1000] != sc) & ~far).any())
+            assert float(near.float().mean()) < 0.01
