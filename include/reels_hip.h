@@ -461,15 +461,19 @@ int reels_hip_clip_gradients(const void* const* grads, void* const* outs, const 
  * shift [rows / rows_per_group][cols] of m_dtype (dtype or REELS_HIP_F32), their rows ld_gate, ld_scale
  * and ld_shift elements apart: row m takes row m / rows_per_group; rows is a multiple of rows_per_group.
  * 0 < cols <= 16384. sum receives s where there is a branch (it may be x or branch themselves where
- * their stride is cols, and overlaps no other operand); y overlaps no other operand. stats [rows][3] f32: the mean as the sum of two
- * values, and rstd. Means and squares are summed in 64 bits, the squares about the mean. A row of s with
- * NaN or an infinity is NaN throughout, and so is one whose rstd is past f32 (no spread and eps 0).
+ * their stride is cols, and overlaps no other operand); y overlaps no other operand. stats [rows][3]
+ * f32: the mean as the sum of two values, and rstd. One pass sums s - s_0 and its square in 64 bits, s_0
+ * the row's first element (0 where center is 0); the mean's share is taken off the squares afterwards,
+ * which loses at most log2(cols) of 53 bits. y is formed in f32 from the stats; where sqrt(cols) / rstd
+ * passes the f32 range, (s - mean) rstd is off by half a step of mean rstd. A row of s with NaN or an
+ * infinity, or without spread where eps is 0, is NaN throughout; one whose rstd is past f32 (spread
+ * below 2^-128 and eps 0) holds no finite value.
  * kept_sum, kept_branch with their scales (NULL: not wanted): s and branch as reels_hip_act8_keep would
  * write them, for the backward; kept_branch only together with kept_sum.
  *
  * reels_hip_modulated_norm_mx4 writes the rows of y in 4 bits instead, as reels_hip_mx4_pack lays them
  * out: codes of reels_hip_mx4_codes_bytes(rows, cols) bytes (4-byte aligned), scales of
- * reels_hip_mx4_scales_bytes. The values are formed in 64 bits and rounded to f32 before the codes.
+ * reels_hip_mx4_scales_bytes. The values are formed in 64 bits, rstd among them, and rounded to f32 before the codes.
  *
  * reels_hip_modulated_norm_bwd, with n = (s - mean) rstd, g = dy (1 + scale), and dsum the gradient
  * that reaches s from elsewhere (NULL for none):
@@ -479,6 +483,9 @@ int reels_hip_clip_gradients(const void* const* grads, void* const* outs, const 
  *     [rows / rows_per_group][cols]; dgate may be NULL, dscale and dshift are both given or both NULL
  * s and branch dense in dtype, or (s_scales, branch_scales not NULL) the kept codes of both, [rows][cols]
  * int8. branch is read for dgate alone. dx may be dy or dsum themselves, dbranch overlaps no other operand.
+ * The sums over a group's rows are f32: a thread adds rows of its group one after the other (a share of
+ * them, or all where some hundred groups of long rows fill the GPU), then partial sums follow in one
+ * order. Products with dy are formed in f32, too.
  * workspace: reels_hip_modulated_norm_workspace_bytes(rows, cols, rows_per_group) bytes where dgate or dscale
  * is wanted (it may be 0). Bitwise reproducible: no atomics, fixed orders of summation. rows = 0 returns at once.
  */

@@ -12,8 +12,9 @@
 // are in 64 bits about the row's first element, which one pass over the row can take; the mean is kept as two
 // f32 values, so that s - mean loses nothing where the mean is many times the spread. Rows in 4 bits are formed in 64 bits and
 // rounded to f32 before their codes are taken, so a code does not depend on the order of f32 operations.
-// 32760 x 5120 bf16 with branch, gate and f32 modulations: 250 us (5.4 TB/s; a copy of 1 GiB runs at 6.0 to 6.5),
-// with both kept 340 (5.0 TB/s), to 4 bits 235-260 (4.2-4.6: 64-bit products and the blocks' maxima beside the loads).
+// 32760 x 5120 bf16 with branch, gate and f32 modulations: 245-257 us (5.2-5.5 TB/s; a copy of 1 GiB by 16 bytes a
+// thread runs at 6.2, past the caches at 6.5), with both kept 335 (5.0 TB/s), to 4 bits 228-267 (4.1-4.8: 64-bit
+// products and the blocks' maxima beside the loads). A modulation for each token, f32: 595 us (5.6 TB/s).
 #include "modnorm.h"
 
 #include <algorithm>

@@ -29,8 +29,10 @@ __global__ __launch_bounds__(1024) void mod_sum_kernel(const float* __restrict__
 
 
 // Walkers (waves or workgroups) of a group's rows with the sums: together as many workgroups as the GPU holds
-// at once by their registers (12 waves of a CU), and at least two rows for each, so that the partial rows stay
-// a small part of the traffic. {partial rows, rows that follow each other}
+// at once by their registers (12 waves of a CU), and at least two rows for each. A workgroup's partial row of f32
+// sums is written and read again, 24 bytes a column, which shows where it has few rows: 2 x 1560 x 1536 f16 14 MB
+// beside 48 of the call's own, the second launch 4.3 of 19 us; twice the rows a partial row were level there and
+// slower at 512 rows. {partial rows, rows that follow each other}
 struct ModParts { int64_t parts, run; };
 ModParts mod_parts(int64_t groups, int64_t rpg, ModForm f) {
   const int64_t walkers = mod_walkers(f), wgs = 256 * (12 * 64 / f.threads > 0 ? 12 * 64 / f.threads : 1);

@@ -21,7 +21,8 @@ __device__ __forceinline__ v8i wide(const v4i& a) { return v8i{a[0], a[1], a[2],
 // ---- rows to 4 bits and back ---------------------------------------------------------------------
 // 64 rows x 256 columns per workgroup, one tile of scale bytes: they are put together in LDS and leave in
 // whole lines. A thread has 16 bytes of a row at a time, all its loads in flight. Bound by memory: 32760 x 13824
-// bf16 245 us to 4 bits (4.7 TB/s), 204 back (5.6).
+// bf16 242 us to 4 bits (4.7 TB/s), 200 back (5.7). Small matrices are bound by their few workgroups: 3001 x 1001 f32
+// 188 of them on 256 CUs, 6.4 us and 6.6 back, where the bytes take 2.1.
 template <int ELT> __global__ __launch_bounds__(256) void mx4_pack_kernel(const void* __restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                                           int tiles, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int V = Chunk<ELT>::V, EB = elt_bytes(ELT), LPR = 256 / V, RP = 256 / LPR, U = 8;
@@ -130,7 +131,7 @@ template <int SA, int SB> __device__ __forceinline__ f32x16 mfma(const v4i& a, c
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, SA, (int)sa, SB, (int)sb);
 }
 
-// At the largest sizes bound by power: 32760 x 13824 -> 5120 takes 1110-1170 us (4.0-4.2 PFLOP/s) at 1.3-1.6 GHz, the
+// At the largest sizes bound by power: 32760 x 13824 -> 5120 takes 1070-1170 us (4.0-4.3 PFLOP/s) at 1.3-1.6 GHz, the
 // products alone on operands in LDS 5.9 PFLOP/s; smaller ones by the first loads and the epilogue.
 //
 // 32 TJ x 32 TJ outputs per workgroup of TJ waves (TJ = 8: 256 x 256, TJ = 4: 128 x 128), each wave 16 TJ
@@ -440,7 +441,8 @@ template <int ELT> __device__ __forceinline__ void load_bias(const Mx4Args& a, i
 // step's codes (their sums are added in LDS at the end). A ring of four stages, three steps in flight and one
 // barrier per step; two workgroups fit a CU. The scale words come the same way, 512 bytes an operand and step,
 // from waves 0 and 1; the others issue a copy that reads nothing, so that the waits count the same. 64 x 5120 -> 5120
-// 11.1 us: 20 steps with a barrier each on 80 workgroups.
+// 9.1 us in a row of calls: 80 workgroups with 20 steps and a barrier each, so 176 CUs have nothing to do; the weight's
+// bytes alone take 2.1. K is not divided among workgroups.
 namespace small {
 constexpr int BT = 64, BK = 128, STAGE = 2 * BT * BK + 2048, RING = 4, NT = 512, LDS = RING * STAGE + 1024;
 }
@@ -636,10 +638,14 @@ int launch_small(const Mx4Args& a, int dtype, hipStream_t st) {
 
 // The tiled form with the least estimated time, in microseconds: a workgroup's step of 256 codes takes 0.32 us
 // in the 64 x 64 form with one workgroup on a CU and 0.61 with two, 0.48 and 1.1 in the 128 x 128 form, 1.5 in the
-// 256 x 256 form (one on a CU); beginning and end 4.5, 5 and 6 us. Measured with every form, 64 / 128 / 256 (us):
-// 200 x 1536 -> 1536 7.8 / 8.4 / 15.7, 333 x 5120 -> 5120 16.8 / 15.6 / 32.9, 777 x 1024 -> 3001 11.9 / 9.8 / 15.0,
-// 512 x 4096 -> 10240 29.6 / 23.1 / 29.7, 1560 x 1536 -> 8960 40.3 / 25.0 / 22.6, 2048 x 5120 -> 5120 79.0 / 46.5 /
-// 38.4, 32760 x 1536 -> 1536 148 / 62.1 / 63.6.
+// 256 x 256 form (one on a CU); beginning and end 4.5, 5 and 6 us. Fitted to one round of tiles; over several the
+// steps are slower and each round has an end of its own (32760 x 1536 -> 1536 is put at 33 us in the 256 form, 32760 x
+// 13824 -> 5120 at 816), which moves the choice by 5% at most in what was measured. Every form, 64 / 128 / 256, us in a
+// row of calls, the rule's own marked:
+// 200 x 1536 -> 1536 7.8* / 7.7 / 13.5, 333 x 5120 -> 5120 14.1 / 13.7* / 31.1, 777 x 1024 -> 3001 9.9 / 7.9* / 12.8,
+// 512 x 4096 -> 10240 28.1 / 21.3* / 28.4, 1560 x 1536 -> 8960 39.2 / 23.5 / 21.4*, 2048 x 5120 -> 5120 73.9 / 43.6 /
+// 38.4*, 4096 x 5120 -> 5120 144 / 79* / 77, 8192 x 5120 -> 5120 277 / 144 / 125*, 32760 x 1536 -> 1536 145 / 62.0 / 63.0*,
+// 32760 x 13824 -> 5120 - / 1517 / 1074*.
 int tile_of(int64_t M, int64_t N, int64_t steps) {
   auto two = [](int64_t blocks, double one, double both) {  // two workgroups fit a CU
     const int64_t full = blocks / 512, rest = blocks % 512;

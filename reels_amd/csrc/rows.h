@@ -1,5 +1,6 @@
-// Rows of a matrix in registers, as the norms hold them: a group of TPR threads has a row, NCH chunks of
-// 16 bytes each.
+// Rows of a matrix in registers, as the root-mean-square norm holds them (norm.hip; the modulated norm has its
+// own form, modnorm.h, whose threads walk several rows): a group of TPR threads has a row, NCH chunks of 16 bytes
+// each.
 #pragma once
 #include "vec.h"
 
