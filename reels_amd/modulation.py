@@ -290,8 +290,11 @@ class ModulatedNormFunction(torch.autograd.Function):
             s = CompressedActivations(s, ss, ctx.dtype)
             b = None if b is None else CompressedActivations(b, bs, ctx.dtype)
         need = ctx.needs_input_grad
-        if dy is None:  # nothing reaches the norm: the sum's gradient alone
-            dy = torch.zeros_like(dsum)
+        if dy is None:
+            # Nothing reaches the norm: the sum's gradient alone, whatever the sum holds. With 1 / the spread at 0 and
+            # finite rows in the sum's place the norm adds zeros.
+            dy, s, stats = torch.zeros_like(dsum), dsum, torch.zeros_like(stats)
+            b = b.restore() if isinstance(b, CompressedActivations) else b
         g = modulated_norm_backward(dy, s, stats, scale, b, gate, dsum, ctx.center,
                                     want_modulation=need[1] or need[2] or need[4])
 

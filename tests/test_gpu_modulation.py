@@ -646,3 +646,24 @@ def test_rows_one_after_the_other(dev, S, C, dtype):
             assert not bool(((codes[b, i:i + 1000] != c) & ~near).any())
             assert not bool(((scales[b, i:i + 1000] != sc) & ~far).any())
             assert float(near.float().mean()) < 0.01
+
+
+@pytest.mark.parametrize("compress", [False, True])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("C", [7, 300, 1536, 9001])
+def test_gradient_of_the_sum_alone(dev, C, dtype, compress):
+    """Where only the sum is used its gradient reaches x, the branch and the gate as it is, also in rows whose sum or
+    spread is not finite."""
+    t, m = make(2, 9, C, dtype, "f32", "sample")
+    t["x"][0, 3, 2], t["x"][1, 5, C - 1], t["x"][1, 7] = float("nan"), float("inf"), 2.0
+    t["branch"][1, 7] = 0.0
+    leaves = [v.clone().requires_grad_() for v in (t["x"], m["scale"], m["shift"], t["branch"], m["gate"])]
+    _, s = ModulatedNormFunction.apply(*leaves, 0.0, True, compress)
+    dx, dscale, dshift, db, dgate = torch.autograd.grad(s, leaves, t["dsum"])
+    assert torch.equal(dx, t["dsum"]) and not dscale.any() and not dshift.any()
+    # one product: rounded once to the type, or to f32 before that (binary16 has an instruction that does it at once)
+    want = t["dsum"].double() * m["gate"][:, None].double()
+    assert_within(db, want, U * want.abs(), "dbranch")
+    b = blocks8(t["branch"].double().reshape(-1, C))[2].view(2, 9, C).to(DT[dtype]) if compress else t["branch"]
+    each = t["dsum"].double() * b.double()
+    assert_within(dgate, each.sum(1), (100 * U * each.abs()).sum(1), "dgate")
